@@ -13,6 +13,7 @@
 #include <nvtx3/nvToolsExt.h>
 
 #include "engine.cuh"
+#include "policy.cuh"
 
 namespace gb {
 cudaError_t launch_steps(StepParams p, cudaStream_t stream);  // step.cu
@@ -1014,6 +1015,98 @@ int goib2d_candidate_pairs(const goib2d_pair_desc *d, int32_t *pair_a, int32_t *
     CUDA_TRY(gb::launch_pair_fill(s, d_start, const_cast<int32_t *>(d_pa), const_cast<int32_t *>(d_pb)));
     CUDA_TRY(cudaMemcpy(pair_a, d_pa, sizeof(int32_t) * start[F], cudaMemcpyDeviceToHost));
     CUDA_TRY(cudaMemcpy(pair_b, d_pb, sizeof(int32_t) * start[F], cudaMemcpyDeviceToHost));
+    return 0;
+}
+
+// ---- the policy's side (delta.cu, clip.cu)
+namespace {
+int delta_check(const goib2d_delta_desc *d) {
+    if (!d) return fail(GOIB2D_EINVAL, "null argument");
+    if (d->n_worlds < 0 || d->n_steps < 0) return fail(GOIB2D_EINVAL, "negative size");
+    if (d->dtype != GOIB2D_FLOAT32 && d->dtype != GOIB2D_BFLOAT16) return fail(GOIB2D_EINVAL, "dtype %d", d->dtype);
+    if (d->heads < 1 || d->key_heads < 1 || d->heads % d->key_heads)
+        return fail(GOIB2D_EINVAL, "%d heads over %d key heads", d->heads, d->key_heads);
+    if (d->key_dim < 1 || d->value_dim < 1) return fail(GOIB2D_EINVAL, "key_dim %d, value_dim %d", d->key_dim,
+                                                        d->value_dim);
+    if (d->key_dim > 128 || d->value_dim > 128)
+        return fail(GOIB2D_ELIMIT, "key_dim %d, value_dim %d (128 at most)", d->key_dim, d->value_dim);
+    if (d->n_worlds > INT32_MAX / d->heads) return fail(GOIB2D_ELIMIT, "%lld worlds of %d heads (2^31 - 1 in all)",
+                                                        (long long)d->n_worlds, d->heads);
+    const int64_t token = (int64_t)d->heads * (d->key_dim + d->value_dim);
+    if (d->n_worlds && d->n_steps > (INT64_MAX >> 6) / d->n_worlds / token) return fail(GOIB2D_ELIMIT, "size overflows");
+    if (d->n_worlds && !d->state_out) return fail(GOIB2D_EINVAL, "null state");
+    if (d->n_worlds && d->n_steps && (!d->q || !d->k || !d->v || !d->g || !d->beta))
+        return fail(GOIB2D_EINVAL, "null input");
+    return 0;
+}
+}  // namespace
+
+int goib2d_delta_step(const goib2d_delta_desc *d, void *stream) {
+    Range range("goib2d_delta_step");
+    int rc = delta_check(d);
+    if (rc) return rc;
+    if (d->n_steps != 1) return fail(GOIB2D_EINVAL, "%lld steps: goib2d_delta_step takes one", (long long)d->n_steps);
+    if (!d->n_worlds) return 0;
+    if (!d->state_in || !d->out) return fail(GOIB2D_EINVAL, "null state or output");
+    CUDA_TRY(gb::launch_delta_step(*d, (cudaStream_t)stream));
+    return 0;
+}
+
+int64_t goib2d_delta_saved_bytes(const goib2d_delta_desc *d) {
+    int rc = delta_check(d);
+    return rc ? rc : gb::delta_saved_bytes(*d);
+}
+
+int64_t goib2d_delta_workspace_bytes(const goib2d_delta_desc *d) {
+    int rc = delta_check(d);
+    return rc ? rc : gb::delta_workspace_bytes(*d);
+}
+
+int goib2d_delta_forward(const goib2d_delta_desc *d, void *saved, void *stream) {
+    Range range("goib2d_delta_forward");
+    int rc = delta_check(d);
+    if (rc) return rc;
+    if (!d->n_worlds) return 0;
+    if (d->n_steps && !d->out) return fail(GOIB2D_EINVAL, "null output");
+    if ((uintptr_t)saved % 16) return fail(GOIB2D_EINVAL, "saved is not 16-byte aligned");
+    CUDA_TRY(gb::launch_delta_forward(*d, saved, (cudaStream_t)stream));
+    return 0;
+}
+
+int goib2d_delta_backward(const goib2d_delta_desc *d, const goib2d_delta_grads *gr, const void *saved,
+                          void *workspace, void *stream) {
+    Range range("goib2d_delta_backward");
+    int rc = delta_check(d);
+    if (rc) return rc;
+    if (!gr) return fail(GOIB2D_EINVAL, "null argument");
+    if (!d->n_worlds) return 0;
+    if (!workspace || (uintptr_t)workspace % 16) return fail(GOIB2D_EINVAL, "workspace is null or not 16-byte aligned");
+    if (d->n_steps && (!saved || (uintptr_t)saved % 16)) return fail(GOIB2D_EINVAL, "saved is null or not 16-byte aligned");
+    if (d->n_steps && (!gr->dq || !gr->dk || !gr->dv || !gr->dg || !gr->dbeta))
+        return fail(GOIB2D_EINVAL, "null gradient");
+    CUDA_TRY(gb::launch_delta_backward(*d, *gr, saved, workspace, (cudaStream_t)stream));
+    return 0;
+}
+
+int64_t goib2d_clip_workspace_bytes(const goib2d_grad *grads, int32_t n) {
+    if (n < 0 || (n && !grads)) return fail(GOIB2D_EINVAL, "bad gradient table");
+    return gb::clip_workspace_bytes(grads, n);
+}
+
+int goib2d_clip_grads(const goib2d_grad *grads, int32_t n, float max_norm, float *norm, void *workspace,
+                      void *stream) {
+    Range range("goib2d_clip_grads");
+    if (n < 0 || (n && !grads)) return fail(GOIB2D_EINVAL, "bad gradient table");
+    if (!(max_norm >= 0.0f)) return fail(GOIB2D_EINVAL, "max_norm %g", (double)max_norm);
+    if (!workspace || (uintptr_t)workspace % 16) return fail(GOIB2D_EINVAL, "workspace is null or not 16-byte aligned");
+    for (int32_t i = 0; i < n; ++i) {
+        const goib2d_grad &g = grads[i];
+        if (g.dtype != GOIB2D_FLOAT32 && g.dtype != GOIB2D_BFLOAT16) return fail(GOIB2D_EINVAL, "tensor %d: dtype %d", i, g.dtype);
+        if (g.numel < 0 || g.numel >> 48) return fail(GOIB2D_EINVAL, "tensor %d: %lld elements", i, (long long)g.numel);
+        if (g.numel && (!g.data || (uintptr_t)g.data % (g.dtype == GOIB2D_BFLOAT16 ? 2 : 4)))
+            return fail(GOIB2D_EINVAL, "tensor %d: null or misaligned data", i);
+    }
+    CUDA_TRY(gb::launch_clip(grads, n, max_norm, norm, workspace, (cudaStream_t)stream));
     return 0;
 }
 

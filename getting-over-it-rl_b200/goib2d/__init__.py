@@ -27,9 +27,12 @@ def __getattr__(name):
     if name in ("step", "step_", "to_device", "to_host", "broadcast", "Engine", "build"):
         from . import api
         return getattr(api, name)
+    if name in ("delta_step_", "delta_rule", "clip_grads_"):
+        from . import policy
+        return getattr(policy, name)
     raise AttributeError(name)
 
 
 __all__ = ["Settings", "WorldDef", "Model", "State", "step", "step_", "GAME_DT", "STATIC", "KINEMATIC", "DYNAMIC",
            "REVOLUTE", "PRISMATIC", "WELD", "MOTOR", "compact_model", "compact_state", "expand_state", "to_device", "to_host",
-           "broadcast", "Engine"]
+           "broadcast", "Engine", "delta_step_", "delta_rule", "clip_grads_"]

@@ -236,6 +236,13 @@ def load():
         "goib2d_spawn": (C.c_int, [vp, C.c_int32, C.c_int32, C.c_int64, C.POINTER(vp), C.POINTER(vp), C.c_int32,
                                    C.c_int32, vp, C.c_int32, _i, vp, vp]),
         "goib2d_seed_placements": (C.c_int, [C.POINTER(SpawnRule), C.c_uint64, C.c_int64, C.c_int64, vp, vp, vp]),
+        "goib2d_delta_step": (C.c_int, [vp, vp]),
+        "goib2d_delta_forward": (C.c_int, [vp, vp, vp]),
+        "goib2d_delta_backward": (C.c_int, [vp, vp, vp, vp, vp]),
+        "goib2d_delta_saved_bytes": (C.c_int64, [vp]),
+        "goib2d_delta_workspace_bytes": (C.c_int64, [vp]),
+        "goib2d_clip_grads": (C.c_int, [vp, C.c_int32, C.c_float, vp, vp, vp]),
+        "goib2d_clip_workspace_bytes": (C.c_int64, [vp, C.c_int32]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)

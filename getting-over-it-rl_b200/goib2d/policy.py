@@ -1,0 +1,247 @@
+"""The policy's side of a batch of worlds: a memory per world (the gated delta rule) and gradient clipping.
+
+    memory = torch.zeros(N, heads, K, V, device="cuda")                       # float32, one matrix per world and head
+    o = goib2d.delta_step_(memory, q, k, v, g, beta, reset=fell)              # acting: one token per world
+    o, last = goib2d.delta_rule(q, k, v, g, beta, state=first, reset=resets)  # training: (N, T, ...) rollouts
+    norm = goib2d.clip_grads_([p.grad for p in net.parameters()], 0.5)        # before the optimiser's step
+
+Per world and head the memory is a matrix S (K, V). A token with decay a = exp(g), key k, value v, query q and write
+strength b = beta does
+
+    S' = a S;  r = v - S'^T k;  S = S' + k (b r)^T;  o = scale S^T q
+
+and a token whose `reset` is set (the world's reset came before it), or whose decay is 0 in float32, starts from
+S' = 0 whatever S held. q and k may have fewer heads than v: value head h reads key head h // (heads // key_heads).
+All of q, k, v, g, beta are float32 or all bfloat16; memories and every sum are float32. The kernels are in
+libgoib2d.so (csrc/delta.cu, csrc/clip.cu; the C calls are goib2d_delta_* and goib2d_clip_grads): there is no CPU
+path. Calls run on the current stream of the tensors' device and return without waiting for it.
+"""
+import struct
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import native
+
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1}
+_DESC = struct.Struct("2q5if9P20q")   # goib2d_delta_desc
+_GRADS = struct.Struct("8P18q")       # goib2d_delta_grads
+_GRAD = struct.Struct("Pqi4x")        # goib2d_grad
+MAX_DIM = 128                         # largest key_dim and value_dim
+
+
+def _rows(name, x, shape, dtype, device, channels=True):
+    """x's address and element strides, for a tensor of this shape whose channels (last axis) are contiguous."""
+    if x.shape != shape or x.dtype != dtype or x.device != device:
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype} on {device}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    st = x.stride()
+    if channels:
+        if st[-1] != 1 and shape[-1] > 1:
+            raise ValueError(f"{name}: the last axis must be contiguous")
+        st = st[:-1]
+    return x.data_ptr(), st
+
+
+def _state(name, x, shape, device):
+    if x.shape != shape or x.dtype != torch.float32 or x.device != device or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {tuple(shape)} float32 tensor on {device}, got "
+                         f"{tuple(x.shape)} {x.dtype} on {x.device}")
+    return x.data_ptr()
+
+
+def _reset(x, shape, device):
+    if x is None:
+        return 0, (0, 0)
+    if x.dtype not in (torch.bool, torch.uint8) or x.shape != shape or x.device != device:
+        raise ValueError(f"reset must be {tuple(shape)} bool or uint8 on {device}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+    return x.data_ptr(), x.stride()
+
+
+def _sizes(q, v, steps):
+    """(worlds, steps, heads, key heads, K, V) of q (N, [T,] key heads, K) and v (N, [T,] heads, V)."""
+    dims = 4 if steps else 3
+    for name, x in (("q", q), ("v", v)):
+        if not isinstance(x, torch.Tensor) or not x.is_cuda:
+            raise TypeError(f"{name} must be a CUDA tensor")
+        if x.dim() != dims or x.dtype not in _DTYPE:
+            raise ValueError(f"{name} must be a float32 or bfloat16 tensor of {dims} axes, got {tuple(x.shape)} {x.dtype}")
+    hk, K = q.shape[-2:]
+    h, V = v.shape[-2:]
+    if h < 1 or hk < 1 or h % hk:
+        raise ValueError(f"{h} value heads over {hk} key heads")
+    if not (1 <= K <= MAX_DIM and 1 <= V <= MAX_DIM):
+        raise ValueError(f"key and value channels must be 1..{MAX_DIM}, got {K} and {V}")
+    return v.shape[0], v.shape[1] if steps else 1, h, hk, K, V
+
+
+def _on(device):
+    """The device's guard, where it is not the current one."""
+    return torch.cuda.device(device)
+
+
+def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
+    """One token for every world: state (N, H, K, V) float32 is updated in place, and o (N, H, V) in v's type is
+    returned. q, k (N, Hk, K), v (N, H, V), g (log decay) and beta (N, H), reset (N,) bool or None; scale defaults
+    to K ** -0.5. Inputs may have any strides with contiguous channels. Not differentiable: rollouts train through
+    delta_rule."""
+    n, _, h, hk, K, V = _sizes(q, v, False)
+    device, dt = v.device, v.dtype
+    if torch.is_grad_enabled() and any(x.requires_grad for x in (state, q, k, v, g, beta)):
+        raise ValueError("delta_step_ is not differentiable: use delta_rule, or torch.no_grad()")
+    sp = _state("state", state, (n, h, K, V), device)
+    qp, qs = _rows("q", q, (n, hk, K), dt, device)
+    kp, ks = _rows("k", k, (n, hk, K), dt, device)
+    vp, vs = _rows("v", v, (n, h, V), dt, device)
+    gp, gs = _rows("g", g, (n, h), dt, device, False)
+    bp, bs = _rows("beta", beta, (n, h), dt, device, False)
+    rp, rs = _reset(reset, (n,), device)
+    if out is None:
+        out = torch.empty((n, h, V), dtype=dt, device=device)
+    op, os_ = _rows("out", out, (n, h, V), dt, device)
+    desc = _DESC.pack(n, 1, h, hk, K, V, _DTYPE[dt], K ** -0.5 if scale is None else scale, qp, kp, vp, gp, bp, rp, sp, sp, op,
+                      qs[0], 0, qs[1], ks[0], 0, ks[1], vs[0], 0, vs[1], gs[0], 0, gs[1], bs[0], 0, bs[1],
+                      os_[0], 0, os_[1], rs[0], 0)
+    lib = native.load()
+    if device.index == torch.cuda.current_device():
+        native.check(lib.goib2d_delta_step(desc, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with _on(device):
+            native.check(lib.goib2d_delta_step(desc, torch.cuda.current_stream(device).cuda_stream))
+    return out
+
+
+def _describe(q, k, v, g, beta, state, reset, scale, last, out):
+    """goib2d_delta_desc of a rollout call."""
+    n, t, h, hk, K, V = _sizes(q, v, True)
+    device, dt = v.device, v.dtype
+    qp, qs = _rows("q", q, (n, t, hk, K), dt, device)
+    kp, ks = _rows("k", k, (n, t, hk, K), dt, device)
+    vp, vs = _rows("v", v, (n, t, h, V), dt, device)
+    gp, gs = _rows("g", g, (n, t, h), dt, device, False)
+    bp, bs = _rows("beta", beta, (n, t, h), dt, device, False)
+    rp, rs = _reset(reset, (n, t), device)
+    sp = 0 if state is None else _state("state", state, (n, h, K, V), device)
+    return _DESC.pack(n, t, h, hk, K, V, _DTYPE[dt], scale, qp, kp, vp, gp, bp, rp, sp, last.data_ptr(),
+                      out.data_ptr(), *qs, *ks, *vs, *gs, *bs, *out.stride()[:3], *rs)
+
+
+def _forward(q, k, v, g, beta, state, reset, scale, train):
+    """(o, last state, what the backward pass keeps or None)."""
+    n, t, h, hk, K, V = _sizes(q, v, True)
+    device = v.device
+    lib = native.load()
+    with _on(device):
+        out = torch.empty((n, t, h, V), dtype=v.dtype, device=device)
+        last = torch.empty((n, h, K, V), dtype=torch.float32, device=device)
+        desc = _describe(q, k, v, g, beta, state, reset, scale, last, out)
+        saved = None
+        if train:
+            size = lib.goib2d_delta_saved_bytes(desc)
+            native.check(min(size, 0))
+            saved = torch.empty(size, dtype=torch.uint8, device=device)
+        native.check(lib.goib2d_delta_forward(desc, saved.data_ptr() if train else None,
+                                              torch.cuda.current_stream(device).cuda_stream))
+    return out, last, saved
+
+
+class _DeltaRule(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, reset, scale):
+        ctx.set_materialize_grads(False)
+        out, last, saved = _forward(q, k, v, g, beta, state, reset, scale, True)
+        ctx.save_for_backward(q, k, v, g, beta, state, reset, last, saved)
+        ctx.scale = scale
+        return out, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dlast):
+        q, k, v, g, beta, state, reset, last, saved = ctx.saved_tensors
+        if dout is None and dlast is None:
+            return (None,) * 8
+        n, t, h, hk, K, V = _sizes(q, v, True)
+        device, dt = v.device, v.dtype
+        lib = native.load()
+        with _on(device):
+            desc = _describe(q, k, v, g, beta, state, reset, ctx.scale, last, last)
+            dop, dos = 0, (0, 0, 0)
+            if dout is not None:
+                dout = dout if dout.stride(-1) == 1 else dout.contiguous()
+                dop, dos = dout.data_ptr(), dout.stride()[:3]
+            dlast = None if dlast is None else dlast.contiguous()
+            dq, dk = (torch.empty((n, t, hk, K), dtype=dt, device=device) for _ in range(2))
+            dv = torch.empty((n, t, h, V), dtype=dt, device=device)
+            dg, dbeta = (torch.empty((n, t, h), dtype=dt, device=device) for _ in range(2))
+            first = None
+            if state is not None and ctx.needs_input_grad[5]:
+                first = torch.empty((n, h, K, V), dtype=torch.float32, device=device)
+            grads = _GRADS.pack(dop, 0 if dlast is None else dlast.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                                dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), 0 if first is None else first.data_ptr(),
+                                *dos, *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *dg.stride(), *dbeta.stride())
+            size = lib.goib2d_delta_workspace_bytes(desc)
+            native.check(min(size, 0))
+            work = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
+            native.check(lib.goib2d_delta_backward(desc, grads, saved.data_ptr(), work.data_ptr(),
+                                                   torch.cuda.current_stream(device).cuda_stream))
+        return dq, dk, dv, dg, dbeta, first, None, None
+
+
+def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
+    """Rollouts of T tokens per world: (o (N, T, H, V) in v's type, last state (N, H, K, V) float32). q, k
+    (N, T, Hk, K), v (N, T, H, V), g (log decay) and beta (N, T, H), state: the first state (N, H, K, V) float32 or
+    None (zeros), reset (N, T) bool or None; scale defaults to K ** -0.5. Any strides with contiguous channels, so a
+    rollout recorded step by step goes in as x.transpose(0, 1). Differentiable in q, k, v, g, beta and state."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state)):
+        return _DeltaRule.apply(q, k, v, g, beta, state, reset, float(scale))
+    return _forward(q, k, v, g, beta, state, reset, float(scale), False)[:2]
+
+
+def _dense(x):
+    """Whether x's elements fill one piece of memory, in any order of its axes."""
+    n = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(x.stride(), x.shape) if sz > 1):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def clip_grads_(grads, max_norm):
+    """Scale all gradients, in place, by min(1, max_norm / (norm + 1e-6)), where norm is the 2-norm of all their
+    elements together; returns norm (a float32 scalar on the device). grads: float32 or bfloat16 CUDA tensors on one
+    device, dense in memory; None entries are skipped. A NaN or an infinity among them makes the result NaN where
+    the formula does."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
+    grads = [x for x in grads if x is not None]
+    if not grads:
+        raise ValueError("no gradients")
+    device = grads[0].device
+    if device.type != "cuda":
+        raise TypeError("gradients must be CUDA tensors")
+    table, seen = [], set()
+    for x in grads:
+        dt = _DTYPE.get(x.dtype)
+        if dt is None or x.device != device or x.layout != torch.strided:
+            raise ValueError(f"gradients must be dense float32 or bfloat16 tensors on {device}, got {x.dtype} on {x.device}")
+        if not (x.is_contiguous() or _dense(x)):
+            raise ValueError(f"a gradient of shape {tuple(x.shape)} and strides {x.stride()} is not dense in memory")
+        p = x.data_ptr()
+        if x.numel():
+            if p in seen:
+                raise ValueError("the same gradient twice")
+            seen.add(p)
+            table.append(_GRAD.pack(p, x.numel(), dt))
+    packed = b"".join(table)
+    lib = native.load()
+    with _on(device):
+        norm = torch.empty((), dtype=torch.float32, device=device)
+        size = lib.goib2d_clip_workspace_bytes(packed, len(table))
+        native.check(min(size, 0))
+        work = torch.empty(size, dtype=torch.uint8, device=device)
+        native.check(lib.goib2d_clip_grads(packed, len(table), max_norm, norm.data_ptr(), work.data_ptr(),
+                                           torch.cuda.current_stream(device).cuda_stream))
+    return norm

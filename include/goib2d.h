@@ -321,6 +321,74 @@ int goib2d_step_noalloc(goib2d_model *model, const goib2d_settings *settings, fl
                         int32_t fixture_rows, int64_t n_worlds, int32_t n_steps, void *const *leaves,
                         const float *actions, void *stream);
 
+/* ---- The policy's side of a batch of worlds (no counterpart in the reference, whose trainer is outside it): a
+ * memory per world that an agent advances by one token per world step and trains over recorded rollouts, and the
+ * update's gradient clipping. These calls need no model handle; they run on the current device, asynchronously on
+ * `stream`, allocate nothing and keep nothing between calls. */
+enum { GOIB2D_FLOAT32 = 0, GOIB2D_BFLOAT16 = 1 };
+
+/* The gated delta rule. World n's head h holds a state S (float32 [key_dim][value_dim]); token t with decay
+ * a = exp(g), key k, value v, query q and write strength b = beta does
+ *     S' = a S;  r = v - S'^T k;  u = b r;  S = S' + k u^T;  out = scale S^T q.
+ * A token with reset set, or with a decay of 0 in float32, starts from S' = 0 whatever S held. Value head h reads
+ * the keys and queries of key head h / (heads / key_heads). q, k, v, g, beta and out have the type `dtype`; every
+ * sum and the state are float32. Strides are in elements, for worlds, steps and heads; channels are contiguous.
+ * state_in / state_out: contiguous [n_worlds][heads][key_dim][value_dim]; state_in NULL = zeros; they may be the
+ * same buffer, and may not overlap otherwise. reset: one byte per world and step, or NULL. key_dim and value_dim
+ * 1..128, heads a multiple of key_heads. */
+typedef struct goib2d_delta_desc {
+    int64_t n_worlds, n_steps;
+    int32_t heads, key_heads, key_dim, value_dim, dtype;
+    float scale;
+    const void *q, *k;      /* [n_worlds][n_steps][key_heads][key_dim] */
+    const void *v;          /* [n_worlds][n_steps][heads][value_dim] */
+    const void *g, *beta;   /* [n_worlds][n_steps][heads] */
+    const uint8_t *reset;   /* [n_worlds][n_steps] */
+    const float *state_in;
+    float *state_out;
+    void *out;              /* as v */
+    int64_t q_stride[3], k_stride[3], v_stride[3], g_stride[3], beta_stride[3], out_stride[3], reset_stride[2];
+} goib2d_delta_desc;
+
+/* Gradients of the rollout's inputs, in their types, from those of its outputs: dout (as out; NULL = zeros) and
+ * dstate_out (of the last state; NULL = zeros). dstate_in may be NULL (not wanted). dq and dk are summed over the
+ * value heads that share a key head; dg is 0 where the state starts afresh. */
+typedef struct goib2d_delta_grads {
+    const void *dout;
+    const float *dstate_out;
+    void *dq, *dk, *dv, *dg, *dbeta;
+    float *dstate_in;
+    int64_t dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3], dg_stride[3], dbeta_stride[3];
+} goib2d_delta_grads;
+
+/* One token per world (n_steps 1): the form an agent acts with; usually state_in == state_out. */
+int goib2d_delta_step(const goib2d_delta_desc *desc, void *stream);
+
+/* n_steps tokens of every world. saved: NULL, or goib2d_delta_saved_bytes(desc) bytes of device memory (16-byte
+ * aligned) that goib2d_delta_backward reads. n_steps 0 copies the state. */
+int goib2d_delta_forward(const goib2d_delta_desc *desc, void *saved, void *stream);
+int64_t goib2d_delta_saved_bytes(const goib2d_delta_desc *desc);
+
+/* The gradients. desc as in the forward call (state_out: the state that it left; out is not read), saved what it
+ * kept; workspace: goib2d_delta_workspace_bytes(desc) bytes of device memory (16-byte aligned). */
+int goib2d_delta_backward(const goib2d_delta_desc *desc, const goib2d_delta_grads *grads, const void *saved,
+                          void *workspace, void *stream);
+int64_t goib2d_delta_workspace_bytes(const goib2d_delta_desc *desc);
+
+/* Gradient clipping by the global norm: norm = sqrt(sum of squares of all elements of all n tensors), then every
+ * element times min(1, max_norm / (norm + 1e-6)), in place. A NaN among the gradients gives NaN everywhere. Sums are
+ * float64 in a fixed order (the same inputs give the same bits). The table is host memory and read before the call
+ * returns; norm: one device float32, or NULL; workspace: goib2d_clip_workspace_bytes(grads, n) bytes of device
+ * memory (16-byte aligned). Tensors are dense and must not overlap. */
+typedef struct goib2d_grad {
+    void *data;
+    int64_t numel;
+    int32_t dtype;
+} goib2d_grad;
+int goib2d_clip_grads(const goib2d_grad *grads, int32_t n, float max_norm, float *norm, void *workspace,
+                      void *stream);
+int64_t goib2d_clip_workspace_bytes(const goib2d_grad *grads, int32_t n);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,526 @@
+"""The policy operators (goib2d.delta_step_, delta_rule, clip_grads_) against their definitions in 64 bits.
+
+Tolerances, on the 2-norm of the difference over the 2-norm of the result. float32: matrix products run on operands
+split into two bfloat16 (a relative error of 2^-17 a product at most, and independent from product to product), in
+chains of at most four products within a chunk: 4 * 2^-17 = 3.1e-5 at most. bfloat16 results: the rounding of the
+result (2^-9) and of the two operands of the product that makes it (2^-9 each) at most: 3 * 2^-9 = 5.9e-3. States are
+float32 whatever the inputs' type."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import goib2d
+from goib2d import native, policy
+
+TOL = {torch.float32: 4 * 2.0**-17, torch.bfloat16: 3 * 2.0**-9}
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def recurrence(q, k, v, g, beta, state, reset, scale=None):
+    """The definition, token by token, on (N, T, ...) float64 tensors; differentiable."""
+    n, t, h, V = v.shape
+    K, group = q.shape[-1], h // q.shape[2]
+    scale = K**-0.5 if scale is None else scale
+    q, k = q.repeat_interleave(group, 2), k.repeat_interleave(group, 2)
+    S = q.new_zeros(n, h, K, V) if state is None else state
+    out = []
+    for i in range(t):
+        decay = torch.exp(g[:, i])
+        fresh = torch.exp(g[:, i].float()) == 0
+        if reset is not None:
+            fresh = fresh | reset[:, i, None].bool()
+        S = torch.where(fresh[..., None, None], torch.zeros_like(S), S * decay[..., None, None])
+        u = beta[:, i, :, None] * (v[:, i] - torch.einsum("nhkv,nhk->nhv", S, k[:, i]))
+        S = S + k[:, i, :, :, None] * u[:, :, None, :]
+        out.append(scale * torch.einsum("nhkv,nhk->nhv", S, q[:, i]))
+    return (torch.stack(out, 1) if out else v.new_zeros(n, 0, h, V)), S
+
+
+def rollout(n, t, h, hk, K, V, dtype, seed=0, resets=True, state=True, alike=0.7, decay=0.2):
+    r = np.random.default_rng(seed)
+
+    def tokens(*shape):
+        return torch.from_numpy(r.standard_normal((n, t) + shape) + alike * r.standard_normal((n, 1) + shape))
+
+    def unit(x):
+        return x / x.norm(dim=-1, keepdim=True)
+
+    a = {"q": unit(tokens(hk, K)), "k": unit(tokens(hk, K)), "v": tokens(h, V), "g": -decay * torch.exp(tokens(h) - 1),
+         "beta": torch.sigmoid(tokens(h))}
+    a = {x: y.to(dtype).cuda() for x, y in a.items()}
+    a["state"] = torch.from_numpy(0.3 * r.standard_normal((n, h, K, V))).float().cuda() if state else None
+    a["reset"] = torch.from_numpy(r.random((n, t)) < 0.08).cuda() if resets else None
+    return a
+
+
+def wide(a):
+    return {x: None if y is None else y.detach().cpu() if y.dtype == torch.bool else y.detach().double().cpu()
+            for x, y in a.items()}
+
+
+def off(got, want):
+    got, want = got.detach().double().cpu(), want.detach()
+    if not want.numel():
+        return 0.0 if got.shape == want.shape else math.inf
+    assert got.shape == want.shape
+    assert torch.isfinite(got).all()
+    return float((got - want).norm() / want.norm().clamp_min(1e-30))
+
+
+# (worlds, steps, heads, key heads, K, V): one token, part of a chunk, whole chunks, one more; odd and largest channels
+SIZES = [(1, 1, 1, 1, 1, 1), (3, 2, 2, 2, 16, 16), (2, 15, 2, 2, 32, 32), (3, 16, 3, 1, 64, 64),
+         (2, 17, 4, 2, 64, 32), (1, 31, 1, 1, 32, 64), (5, 33, 6, 3, 40, 71), (2, 64, 2, 1, 128, 128),
+         (1, 65, 2, 2, 100, 128), (2, 130, 1, 1, 8, 128), (1, 129, 2, 1, 128, 8), (1, 600, 1, 1, 48, 24),
+         (40, 20, 4, 4, 64, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_rollout(size, dtype):
+    a = rollout(*size, dtype, seed=size[1])
+    out, last = goib2d.delta_rule(**a)
+    want, state = recurrence(**wide(a))
+    assert out.dtype == dtype and last.dtype == F32
+    assert off(out, want) <= TOL[dtype]
+    assert off(last, state) <= TOL[F32]
+
+
+GRADS = ("q", "k", "v", "g", "beta", "state")
+
+
+def backward(a, dout, dlast, fn=goib2d.delta_rule):
+    leaves = [a[x].detach().requires_grad_() for x in GRADS if a[x] is not None]
+    named = dict(zip([x for x in GRADS if a[x] is not None], leaves))
+    out, last = fn(**{**a, **named})
+    outs = [(out, dout)] if dlast is None else [(out, dout), (last, dlast)]
+    got = torch.autograd.grad([x for x, _ in outs], leaves, [y for _, y in outs], allow_unused=True)
+    return out, last, dict(zip(named, got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("last", [False, True], ids=["out", "out+state"])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_gradients(size, dtype, last):
+    n, t, h, hk, K, V = size
+    a = rollout(*size, dtype, seed=7 + t, state=last)
+    r = np.random.default_rng(t)
+    dout = torch.from_numpy(r.standard_normal((n, t, h, V))).to(dtype).cuda()
+    dlast = torch.from_numpy(r.standard_normal((n, h, K, V))).float().cuda() if last else None
+    out, state, got = backward(a, dout, dlast)
+    w = wide(a)
+    want_out, want_state, want = backward(w, dout.double().cpu(), None if dlast is None else dlast.double().cpu(),
+                                          recurrence)
+    assert off(out, want_out) <= TOL[dtype]
+    assert off(state, want_state) <= TOL[F32]
+    for name, x in got.items():
+        y = want[name] if want[name] is not None else torch.zeros_like(w[name])
+        if name == "g" and float(y.abs().max()) == 0:
+            assert not x.any()
+            continue
+        assert x.dtype == (F32 if name == "state" else dtype)
+        # the gradient chain runs through the products of the forward and of the backward pass: twice as many
+        assert off(x, y) <= 2 * TOL[x.dtype], name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("n,h,hk,K,V", [(1, 1, 1, 1, 1), (3, 2, 1, 3, 5), (7, 4, 2, 16, 16), (33, 2, 2, 32, 32),
+                                        (257, 3, 1, 64, 64), (5, 6, 2, 40, 71), (4, 2, 2, 128, 128), (9, 1, 1, 128, 4),
+                                        (9, 1, 1, 5, 128), (3, 1, 1, 127, 127), (0, 2, 1, 8, 8), (2100, 1, 1, 64, 64)])
+def test_step(n, h, hk, K, V, dtype):
+    a = rollout(max(n, 1), 3, h, hk, K, V, dtype, seed=n)
+    a = {x: y[:n] for x, y in a.items()}
+    state = a["state"].clone()
+    want, last = recurrence(**wide(a))
+    for t in range(3):
+        out = goib2d.delta_step_(state, *(a[x][:, t] for x in ("q", "k", "v", "g", "beta")), reset=a["reset"][:, t])
+        assert off(out, want[:, t]) <= TOL[dtype]
+    assert off(state, last) <= TOL[F32]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_rollout_in_pieces_equals_whole(dtype):
+    a = rollout(3, 77, 4, 2, 64, 48, dtype, seed=5)
+    whole, last = goib2d.delta_rule(**a)
+    state, outs = a["state"], []
+    for lo, hi in ((0, 1), (1, 20), (20, 20), (20, 52), (52, 77)):
+        part = {x: y[:, lo:hi] for x, y in a.items() if x != "state"}
+        o, state = goib2d.delta_rule(**part, state=state)
+        outs.append(o)
+    assert off(torch.cat(outs, 1), whole.double().cpu()) <= 2 * TOL[dtype]
+    assert off(state, last.double().cpu()) <= 2 * TOL[F32]
+    assert torch.equal(goib2d.delta_rule(**a)[0], whole)  # the same inputs, the same bits
+
+
+def strided(x, kind):
+    """x with other strides: steps first in memory, channels out of a wider row (off the 16-byte boundary), or heads
+    first."""
+    if kind == "time major":
+        return x.transpose(0, 1).contiguous().transpose(0, 1)
+    if kind == "wide rows":
+        y = x.new_full((*x.shape[:-1], x.shape[-1] + 3), math.nan)
+        y[..., 1:-2] = x
+        return y[..., 1:-2]
+    return x.movedim(2, 0).contiguous().movedim(0, 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["time major", "wide rows", "heads first"])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_strides(kind, dtype):
+    a = rollout(3, 37, 4, 2, 32, 64, dtype, seed=11)
+    dout = torch.randn(3, 37, 4, 64, device="cuda").to(dtype)
+    b = {x: strided(y, kind) if x in ("q", "k", "v", "g", "beta") else y for x, y in a.items()}
+    b["reset"] = a["reset"].t().contiguous().t()
+    out, last, grads = backward(a, dout, None)
+    out2, last2, grads2 = backward(b, strided(dout, kind), None)
+    tol = 2 * TOL[dtype]
+    assert off(out2, out.double().cpu()) <= tol and off(last2, last.double().cpu()) <= 2 * TOL[F32]
+    for x in grads:
+        assert off(grads2[x], grads[x].double().cpu()) <= 2 * tol, x
+    state, state2 = a["state"].clone(), a["state"].clone()
+    names = ("q", "k", "v", "g", "beta")
+    o = goib2d.delta_step_(state, *(a[x][:, 5] for x in names), reset=a["reset"][:, 5])
+    o2 = goib2d.delta_step_(state2, *(b[x][:, 5] for x in names), reset=b["reset"][:, 5],
+                            out=strided(torch.empty_like(a["v"]), kind)[:, 5])
+    assert torch.equal(o, o2) and torch.equal(state, state2)
+
+
+@pytest.mark.gpu
+def test_broadcast_inputs_and_gradients():
+    """One key for all worlds, one decay for all heads and steps: inputs of stride 0, their gradients summed."""
+    a = rollout(4, 21, 2, 1, 16, 24, F32, seed=3, resets=False)
+    key, decay = a["k"][:1, :, :, :].clone(), a["g"][:, :1, :1].clone()
+    dout = torch.randn_like(a["v"])
+
+    def of(fn, a, key, decay, dout):
+        key, decay = key.requires_grad_(), decay.requires_grad_()
+        out, _ = fn(a["q"], key.expand_as(a["k"]), a["v"], decay.expand_as(a["g"]), a["beta"], a["state"], None)
+        return torch.autograd.grad([out], [key, decay], [dout])
+
+    got = of(goib2d.delta_rule, a, key, decay, dout)
+    want = of(recurrence, wide(a), key.detach().double().cpu(), decay.detach().double().cpu(), dout.double().cpu())
+    assert off(got[0], want[0]) <= 2 * TOL[F32] and off(got[1], want[1]) <= 2 * TOL[F32]
+    # a gradient of stride 0 comes in (from a sum)
+    a["v"].requires_grad_()
+    out, _ = goib2d.delta_rule(**a)
+    out.sum().backward()
+    w = wide(a)
+    w["v"] = w["v"].detach().requires_grad_()
+    recurrence(**w)[0].sum().backward()
+    assert off(a["v"].grad, w["v"].grad) <= 2 * TOL[F32]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("K,V", [(16, 16), (64, 64), (40, 71), (128, 128)])
+def test_states_that_start_afresh(K, V, dtype):
+    """A reset, a decay of -inf, of the type's lowest value and of -200 all empty the memory, whatever it held:
+    infinities and NaN in the old state are not read. Every token of world 0 is a reset (its own write is all that
+    its query sees)."""
+    n, t, h = 4, 40, 2
+    a = rollout(n, t, h, h, K, V, dtype, seed=1, resets=False)
+    reset = torch.zeros(n, t, dtype=torch.bool, device="cuda")
+    reset[0] = True
+    reset[:, 0] = True
+    reset[1, [15, 16, 17, 31, 39]] = True
+    a["g"][2, 7] = -math.inf
+    a["g"][2, 16] = torch.finfo(dtype).min
+    a["g"][2, 32:34] = -200.0
+    a["g"][3, 20, 0] = -math.inf  # one head only
+    clean = dict(a, reset=reset)
+    want, last = recurrence(**wide(dict(clean, g=a["g"].clamp_min(-1e3))))
+    dirty = torch.full_like(a["state"], math.nan)
+    dirty[:, :, :, ::2] = math.inf
+    dout = torch.randn(n, t, h, V, device="cuda").to(dtype)
+    for state in (a["state"], dirty):
+        out, got_last, grads = backward(dict(clean, state=state), dout, None)
+        assert off(out, want) <= TOL[dtype] and off(got_last, last) <= TOL[F32]
+        assert not grads["state"].any()
+        assert not grads["g"][reset].any() and not grads["g"][2, [7, 16, 32, 33]].any() and not grads["g"][3, 20, 0]
+    w = wide(dict(clean, g=a["g"].clamp_min(-1e3)))
+    _, _, want_grads = backward(w, dout.double().cpu(), None, recurrence)
+    for x in ("q", "k", "v", "beta", "g"):
+        assert off(grads[x], want_grads[x]) <= 2 * TOL[dtype], x
+    step = dirty.clone()
+    o = goib2d.delta_step_(step, *(a[x][:, 0] for x in ("q", "k", "v", "g", "beta")), reset=reset[:, 0])
+    assert off(o, want[:, 0]) <= TOL[dtype]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("g", [0.0, -1e-6, 0.05])
+def test_decays_from_none_to_all(g):
+    """No decay at all, a chunk whose decays multiply to less than float32 holds, and growth."""
+    a = rollout(2, 70, 2, 1, 32, 32, F32, seed=9, resets=False)
+    a["g"] = torch.full_like(a["g"], g)
+    a["g"][:, ::3] *= 0.5
+    dout = torch.randn_like(a["v"])
+    out, last, grads = backward(a, dout, None)
+    want_out, want_last, want = backward(wide(a), dout.double().cpu(), None, recurrence)
+    assert off(out, want_out) <= TOL[F32] and off(last, want_last) <= TOL[F32]
+    for x in grads:
+        if float(want[x].norm()) > 1e-30:
+            assert off(grads[x], want[x]) <= 2 * TOL[F32], x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_same_key_every_step(dtype):
+    """A world at rest: every token has the same key and beta is 1 (or 0: nothing is written), so that the chunk's
+    triangular system is as far from the identity as it gets."""
+    a = rollout(2, 80, 2, 2, 64, 64, dtype, seed=2, resets=False)
+    a["k"] = a["k"][:, :1].expand_as(a["k"])
+    a["g"] = torch.zeros_like(a["g"])
+    a["beta"] = torch.ones_like(a["beta"])
+    a["beta"][:, ::7] = 0
+    dout = torch.randn(2, 80, 2, 64, device="cuda").to(dtype)
+    out, last, grads = backward(a, dout, None)
+    want_out, want_last, want = backward(wide(a), dout.double().cpu(), None, recurrence)
+    assert off(out, want_out) <= TOL[dtype] and off(last, want_last) <= TOL[F32]
+    for x in grads:
+        assert off(grads[x], want[x]) <= 2 * TOL[F32 if x == "state" else dtype], x
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    """The directional derivative of a smooth loss, by central differences of the definition in 64 bits (step 1e-5:
+    an error of about 1e-10 of its own), against the gradients."""
+    a = rollout(2, 41, 2, 1, 24, 40, F32, seed=4)
+    dout, dlast = torch.randn_like(a["v"]), torch.randn_like(a["state"])
+    _, _, grads = backward(a, dout, dlast)
+    w, wd, wl = wide(a), dout.double().cpu(), dlast.double().cpu()
+    for name in GRADS:
+        way = torch.from_numpy(np.random.default_rng(8).standard_normal(tuple(w[name].shape)))
+
+        def loss(e):
+            o, s = recurrence(**{**w, name: w[name] + e * way})
+            return float((o * wd).sum() + (s * wl).sum())
+
+        slope = (loss(1e-5) - loss(-1e-5)) / 2e-5
+        got = float((grads[name].double().cpu() * way).sum())
+        size = float(grads[name].double().norm().cpu() * way.norm())
+        assert abs(got - slope) <= 2 * TOL[F32] * size, name
+
+
+@pytest.mark.gpu
+def test_zero_steps_and_worlds():
+    a = rollout(3, 4, 2, 1, 16, 16, F32)
+    none = {x: y[:, :0] if x not in ("state",) else y for x, y in a.items()}
+    out, last, grads = backward(none, torch.empty(3, 0, 2, 16, device="cuda"), torch.ones_like(a["state"]))
+    assert out.shape == (3, 0, 2, 16) and torch.equal(last, a["state"])
+    assert torch.equal(grads["state"], torch.ones_like(a["state"]))
+    out, last = goib2d.delta_rule(**dict(none, state=None))
+    assert not last.any()
+    out, last = goib2d.delta_rule(**{x: y[:0] for x, y in a.items()})
+    assert out.shape == (0, 4, 2, 16) and last.shape == (0, 2, 16, 16)
+    # only the last state has a gradient
+    state = a["state"].clone().requires_grad_()
+    _, last = goib2d.delta_rule(**dict(a, state=state))
+    got, = torch.autograd.grad([last], [state], [torch.ones_like(last)])
+    w = wide(a)
+    w["state"] = w["state"].detach().requires_grad_()
+    want, = torch.autograd.grad([recurrence(**w)[1].sum()], [w["state"]])
+    assert off(got, want) <= 2 * TOL[F32] if want.any() else not got.any()
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    """Calls follow the current stream: inputs made on a side stream are read there; a captured step replays."""
+    a = rollout(64, 9, 2, 2, 32, 32, BF16, seed=6)
+    want = goib2d.delta_rule(**a)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2_000_000)
+        b = {x: None if y is None else y.clone() for x, y in a.items()}
+        got = goib2d.delta_rule(**b)
+        grads = [torch.randn(100_000, device="cuda") for _ in range(3)]
+        whole = torch.cat(grads).double().norm()
+        norm = goib2d.clip_grads_(grads, 1.0)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert abs(float(norm) - float(whole)) <= 2e-7 * float(whole)
+    names = ("q", "k", "v", "g", "beta")
+    state, now = a["state"].clone(), {x: a[x][:, 0].clone() for x in names}
+    out = torch.empty(64, 2, 32, dtype=BF16, device="cuda")
+    with torch.cuda.stream(side):
+        goib2d.delta_step_(state, **now, out=out)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    state.copy_(a["state"])
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        goib2d.delta_step_(state, **now, out=out)
+    state.copy_(a["state"])
+    for t in range(3):
+        for x in names:
+            now[x].copy_(a[x][:, t])
+        graph.replay()
+    plain = a["state"].clone()
+    for t in range(3):
+        last = goib2d.delta_step_(plain, *(a[x][:, t] for x in names))
+    assert torch.equal(state, plain) and torch.equal(out, last)
+
+
+# ---- clipping
+
+
+def clip_want(grads, max_norm):
+    w = [x.detach().double().cpu() for x in grads]
+    norm = math.sqrt(sum(float((x * x).sum()) for x in w))
+    return norm, [x * min(1.0, max_norm / (norm + 1e-6)) for x in w]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [0.0, 0.5, 1e9])
+@pytest.mark.parametrize("sizes", [[1], [3, 0, 5], [4096, 4097, 1, 8191], [100_003, 7, 1_000_001], [2_500_000, 13],
+                                   [3] * 2100], ids=lambda s: f"{len(s)}x{max(s)}")
+def test_clip(sizes, max_norm):
+    r = torch.Generator(device="cuda").manual_seed(len(sizes))
+    grads = [torch.randn(s, generator=r, device="cuda").to(BF16 if i % 3 == 1 else F32) for i, s in enumerate(sizes)]
+    norm_want, want = clip_want(grads, max_norm)
+    before = [x.clone() for x in grads]
+    norm = goib2d.clip_grads_([None] + grads, max_norm)
+    # the sum is in 64 bits: the norm and the factor are rounded to float32 (2^-24 each, a few times), elements once
+    assert abs(float(norm) - norm_want) <= 4 * 2.0**-24 * norm_want
+    for x, y, b in zip(grads, want, before):
+        if max_norm > norm_want:
+            assert torch.equal(x, b)
+        else:
+            err = (x.double().cpu() - y).abs() - y.abs() * (2.0**-8 if x.dtype == BF16 else 8 * 2.0**-24)
+            assert not x.numel() or float(err.max()) <= 0
+
+
+@pytest.mark.gpu
+def test_clip_same_bits_and_alignment():
+    base = torch.randn(3_000_001, device="cuda")
+    cut = [1, 2, 500_000, 500_003, 1_700_001, 3_000_000]
+    norms = []
+    for _ in range(3):
+        x = base.clone()
+        norms.append(float(goib2d.clip_grads_([x[a:b] for a, b in zip(cut, cut[1:])], 1.0)))
+        assert torch.equal(x[:1], base[:1]) and torch.equal(x[-1:], base[-1:])
+        assert abs(float(x[1:-1].double().norm()) - 1) < 1e-5
+    assert len(set(norms)) == 1
+    m = torch.randn(130, 70, device="cuda").t()  # dense, in another order
+    want = m / (m.norm() + 1e-6) * 0.1
+    goib2d.clip_grads_([m], 0.1)
+    assert torch.allclose(m, want, rtol=1e-5, atol=0)
+
+
+@pytest.mark.gpu
+def test_clip_values_that_are_not_finite_or_extreme():
+    big = [torch.full((10,), 1e30, device="cuda"), torch.full((10,), 1e-30, device="cuda")]
+    norm = goib2d.clip_grads_(big, 1.0)  # squares beyond float32
+    assert abs(float(norm) / (1e30 * math.sqrt(10)) - 1) < 1e-6 and abs(float(big[0][0]) * math.sqrt(10) - 1) < 1e-6
+    x, y = torch.tensor([1.0, math.inf], device="cuda"), torch.ones(5000, device="cuda")
+    assert float(goib2d.clip_grads_([x, y], 1.0)) == math.inf
+    assert float(x[0]) == 0 and math.isnan(float(x[1])) and not y.any()
+    x, y = torch.tensor([1.0, math.nan], device="cuda"), torch.ones(5000, device="cuda")
+    assert math.isnan(float(goib2d.clip_grads_([x, y], 1.0)))
+    assert torch.isnan(y).all()
+    z = torch.zeros(10, device="cuda")
+    assert float(goib2d.clip_grads_([z], 1.0)) == 0 and not z.any()
+    assert float(goib2d.clip_grads_([torch.empty(0, device="cuda")], 1.0)) == 0
+
+
+# ---- what is refused
+
+
+@pytest.mark.gpu
+def test_refusals():
+    a = rollout(2, 5, 4, 2, 16, 16, F32)
+    names = ("q", "k", "v", "g", "beta")
+    bad = {"k": a["k"][:, :4], "q": a["q"].to(BF16), "g": a["g"][..., :2], "beta": a["beta"].cpu(),
+           "state": a["state"].to(BF16), "reset": a["reset"].float(), "v": a["v"].double()}
+    for x, y in bad.items():
+        with pytest.raises((ValueError, TypeError)):
+            goib2d.delta_rule(**{**a, x: y})
+    with pytest.raises(ValueError, match="contiguous"):
+        goib2d.delta_rule(**{**a, "q": a["q"].transpose(-1, -2).contiguous().transpose(-1, -2)})
+    with pytest.raises(ValueError, match="contiguous"):
+        goib2d.delta_rule(**{**a, "state": a["state"].transpose(-1, -2)})
+    with pytest.raises(ValueError, match="heads"):
+        goib2d.delta_rule(**{**a, "q": a["q"].repeat(1, 1, 2, 1)[:, :, :3], "k": a["k"].repeat(1, 1, 2, 1)[:, :, :3]})
+    wide_v = torch.zeros(2, 5, 4, 129, device="cuda")
+    with pytest.raises(ValueError, match="128"):
+        goib2d.delta_rule(**{**a, "v": wide_v, "state": None})
+    one = {x: a[x][:, 0] for x in names}
+    with pytest.raises(ValueError, match="differentiable"):
+        goib2d.delta_step_(a["state"], **{**one, "q": one["q"].clone().requires_grad_()})
+    with pytest.raises(ValueError, match="state"):
+        goib2d.delta_step_(a["state"][:1], **one)
+    with pytest.raises(ValueError, match="out"):
+        goib2d.delta_step_(a["state"], **one, out=torch.empty(2, 4, 16, dtype=BF16, device="cuda"))
+    x = torch.ones(4, device="cuda")
+    for grads, most in (([x.double()], 1.0), ([x], -1.0), ([x], math.nan), ([], 1.0), ([x, x], 1.0), ([x[::2]], 1.0),
+                        ([x, torch.ones(2)], 1.0), ([x.to_sparse()], 1.0)):
+        with pytest.raises((ValueError, TypeError)):
+            goib2d.clip_grads_(grads, most)
+    assert torch.equal(x, torch.ones_like(x))
+
+
+def test_cpu_tensors_are_refused():
+    a = {x: torch.zeros(s) for x, s in (("q", (2, 3, 1, 8)), ("k", (2, 3, 1, 8)), ("v", (2, 3, 1, 8)), ("g", (2, 3, 1)),
+                                         ("beta", (2, 3, 1)))}
+    with pytest.raises(TypeError, match="CUDA"):
+        goib2d.delta_rule(**a)
+    with pytest.raises(TypeError, match="CUDA"):
+        goib2d.delta_step_(torch.zeros(2, 1, 8, 8), *(x[:, 0] for x in a.values()))
+    with pytest.raises(TypeError, match="CUDA"):
+        goib2d.clip_grads_([torch.ones(3)], 1.0)
+
+
+def desc(**kw):
+    f = dict(n=1, t=1, h=2, hk=1, K=8, V=8, dtype=0, scale=1.0, q=16, k=16, v=16, g=16, beta=16, reset=0, s_in=16, s_out=16,
+             out=16)
+    f.update(kw)
+    return policy._DESC.pack(*f.values(), *[0] * 20)
+
+
+def test_c_entries_refuse_bad_arguments():
+    """The C calls check sizes and pointers before any launch (so these need no GPU)."""
+    lib = native.load()
+    einval, elimit = -1, -4
+    for call in (lambda d: lib.goib2d_delta_step(d, None), lambda d: lib.goib2d_delta_forward(d, None, None),
+                 lambda d: lib.goib2d_delta_saved_bytes(d), lambda d: lib.goib2d_delta_workspace_bytes(d),
+                 lambda d: lib.goib2d_delta_backward(d, policy._GRADS.pack(*[16] * 8, *[0] * 18), 16, 16, None)):
+        assert call(None) == einval
+        assert call(desc(n=-1)) == einval and call(desc(t=-1)) == einval and call(desc(dtype=2)) == einval
+        assert call(desc(hk=0)) == einval and call(desc(h=3, hk=2)) == einval and call(desc(K=0)) == einval
+        assert call(desc(K=129)) == elimit and call(desc(V=129)) == elimit
+        assert call(desc(n=1 << 31)) == elimit and call(desc(n=1 << 20, t=1 << 50)) == elimit
+        assert call(desc(q=0)) == einval and call(desc(beta=0)) == einval and call(desc(s_out=0)) == einval
+        assert call(desc(n=0, q=0, s_out=0)) >= 0
+    assert lib.goib2d_delta_step(desc(t=2), None) == einval and lib.goib2d_delta_step(desc(s_in=0), None) == einval
+    assert lib.goib2d_delta_step(desc(out=0), None) == einval and lib.goib2d_delta_forward(desc(out=0), None, None) == einval
+    assert lib.goib2d_delta_forward(desc(), 8, None) == einval
+    grads = policy._GRADS.pack(*[16] * 8, *[0] * 18)
+    assert lib.goib2d_delta_backward(desc(), None, 16, 16, None) == einval
+    assert lib.goib2d_delta_backward(desc(), grads, None, 16, None) == einval
+    assert lib.goib2d_delta_backward(desc(), grads, 16, None, None) == einval
+    assert lib.goib2d_delta_backward(desc(), policy._GRADS.pack(16, 0, 0, *[16] * 5, *[0] * 18), 16, 16, None) == einval
+    assert b"null" in lib.goib2d_last_error()
+    one = policy._GRAD.pack
+    assert lib.goib2d_clip_grads(None, 1, 1.0, None, 16, None) == einval
+    assert lib.goib2d_clip_grads(one(16, 4, 0), -1, 1.0, None, 16, None) == einval
+    assert lib.goib2d_clip_grads(one(16, 4, 0), 1, -1.0, None, 16, None) == einval
+    assert lib.goib2d_clip_grads(one(16, 4, 0), 1, math.nan, None, 16, None) == einval
+    assert lib.goib2d_clip_grads(one(16, 4, 0), 1, 1.0, None, None, None) == einval
+    assert lib.goib2d_clip_grads(one(0, 4, 0), 1, 1.0, None, 16, None) == einval
+    assert lib.goib2d_clip_grads(one(18, 4, 0), 1, 1.0, None, 16, None) == einval
+    assert lib.goib2d_clip_grads(one(16, -4, 0), 1, 1.0, None, 16, None) == einval
+    assert lib.goib2d_clip_grads(one(16, 4, 7), 1, 1.0, None, 16, None) == einval
+    assert lib.goib2d_clip_workspace_bytes(None, 2) == einval
+
+
+def test_struct_layouts():
+    """The packed structures are the header's (sizes as a C compiler lays them out)."""
+    assert (policy._DESC.size, policy._GRADS.size, policy._GRAD.size) == (272, 208, 24)
+    assert C.sizeof(C.c_void_p) == 8
