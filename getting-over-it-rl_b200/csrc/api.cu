@@ -1018,7 +1018,7 @@ int goib2d_candidate_pairs(const goib2d_pair_desc *d, int32_t *pair_a, int32_t *
     return 0;
 }
 
-// ---- the policy's side (delta.cu, clip.cu)
+// ---- the policy's side (delta_*.cu, clip.cu)
 namespace {
 int delta_check(const goib2d_delta_desc *d) {
     if (!d) return fail(GOIB2D_EINVAL, "null argument");
@@ -1034,6 +1034,10 @@ int delta_check(const goib2d_delta_desc *d) {
                                                         (long long)d->n_worlds, d->heads);
     const int64_t token = (int64_t)d->heads * (d->key_dim + d->value_dim);
     if (d->n_worlds && d->n_steps > (INT64_MAX >> 6) / d->n_worlds / token) return fail(GOIB2D_ELIMIT, "size overflows");
+    const int64_t spans = (d->n_steps + 31) / 32;
+    if (d->n_worlds && spans > INT32_MAX / (d->n_worlds * d->heads))
+        return fail(GOIB2D_ELIMIT, "%lld steps of %lld worlds of %d heads (2^31 - 1 pieces of 32 steps in all)",
+                    (long long)d->n_steps, (long long)d->n_worlds, d->heads);
     if (d->n_worlds && !d->state_out) return fail(GOIB2D_EINVAL, "null state");
     if (d->n_worlds && d->n_steps && (!d->q || !d->k || !d->v || !d->g || !d->beta))
         return fail(GOIB2D_EINVAL, "null input");

@@ -1,0 +1,79 @@
+// What the kernels of the gated delta rule share (delta_step.cu, delta_forward.cu, delta_backward.cu): each (world, head)
+// holds a matrix S [K][V] in float32. Token t with decay a = exp(g), key k, value v, query q, write strength b:
+//     S' = a S,  r = v - S'^T k,  u = b r,  S = S' + k u^T,  o = scale S^T q.
+// A token whose reset flag is set, or whose decay is 0 in float32, starts from S' = 0 without reading the old state
+// (so what the old state held, infinities included, does not matter).
+#pragma once
+#include "policy.cuh"
+
+namespace gb {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// A strided (world, step, head, channel) tensor's row at (n, t, h); channels are contiguous.
+template <class T>
+__device__ __forceinline__ const T *row(const void *p, const int64_t *s, int64_t n, int64_t t, int h) {
+    return (const T *)p + n * s[0] + t * s[1] + h * s[2];
+}
+template <class T>
+__device__ __forceinline__ T *row(void *p, const int64_t *s, int64_t n, int64_t t, int h) {
+    return (T *)p + n * s[0] + t * s[1] + h * s[2];
+}
+
+// The decay of token t, 0 where the state starts afresh.
+template <class T>
+__device__ __forceinline__ float decay_at(const goib2d_delta_desc &d, int64_t n, int64_t t, int h) {
+    if (d.reset && d.reset[n * d.reset_stride[0] + t * d.reset_stride[1]]) return 0.0f;
+    return expf(to_float(*row<T>(d.g, d.g_stride, n, t, h)));
+}
+
+// Whether 16-byte accesses to the rows of a strided tensor are aligned.
+inline bool rows_aligned(const void *p, const int64_t (&s)[3], int64_t n0, int64_t n1, int64_t n2, int cols, int size) {
+    const int64_t e = 16 / size;
+    return (uintptr_t)p % 16 == 0 && cols % e == 0 && (n0 == 1 || s[0] % e == 0) && (n1 == 1 || s[1] % e == 0) &&
+           (n2 == 1 || s[2] % e == 0);
+}
+
+// Gradients whose products run in full precision (mma.cuh, Full): those of float32 inputs, and those of few tokens in
+// bfloat16. A gradient such as dg or db is a sum that may cancel; over many tokens the rounding of bfloat16 operands
+// (2^-9) averages out to 2^-9 of their norm, over a few it need not, and a call of so few tokens waits for latencies,
+// not for products.
+inline bool delta_full(const goib2d_delta_desc &d) {
+    return d.dtype == GOIB2D_FLOAT32 || d.n_worlds * d.n_steps * d.heads <= 4096;
+}
+
+// What goib2d_delta_forward keeps for goib2d_delta_backward: r [n][h][t][V], and S at every keep-th token, its S^T cut
+// into 16 x 16 tiles [n][h][t / keep][V tile][K tile], a tile's values as the 32 threads of a warp hold them in
+// accumulators (8 values a thread). Both in bfloat16, or in float32 (delta_full).
+struct Saved {
+    int64_t r, states, bytes;   // bytes: both
+    int32_t keep, tiles_v, tiles_k, size;
+};
+inline int padded_keys(int K) { return K <= 16 ? 16 : K <= 32 ? 32 : K <= 64 ? 64 : 128; }
+inline Saved delta_saved(const goib2d_delta_desc &d) {
+    const int64_t nh = d.n_worlds * d.heads;
+    Saved s;
+    s.size = delta_full(d) ? 4 : 2;
+    // spans of 64 tokens; of 32 where 64 tokens of float32 with their state do not fit in shared memory
+    s.keep = s.size == 2 || (d.key_dim <= 64 && d.value_dim <= 64) ? 64 : 32;
+    s.tiles_v = (d.value_dim + 15) / 16, s.tiles_k = padded_keys(d.key_dim) / 16;
+    s.r = (nh * d.n_steps * d.value_dim * s.size + 15) / 16 * 16;
+    s.states = nh * ((d.n_steps + s.keep - 1) / s.keep) * s.tiles_v * s.tiles_k * 256 * s.size;
+    s.bytes = s.r + s.states;
+    return s;
+}
+
+template <class F>
+cudaError_t allow_smem(F *f, size_t bytes) {
+    return bytes <= 48 << 10 ? cudaSuccess
+                             : cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+}  // namespace gb

@@ -1,0 +1,266 @@
+// Chunks of 16 tokens of the gated delta rule as small matrix products (delta_forward.cu, delta_backward.cu).
+//
+// With G the running sum of g in the chunk, a_i = exp(G_i) and D_ij = exp(G_i - G_j) (both 0 across a token that
+// starts afresh), W_ij = D_ij k_i.k_j for j < i and P_ij = scale D_ij q_i.k_j for j <= i, the tokens of the chunk obey
+//     (I + W diag(b)) r = V - a (K S0),   u = b r,   O = scale a (Q S0) + P u,   S1 = a_16 S0 + K^T (d u),
+// d_j = exp(G_16 - G_j). Chunks of 16 because that is one tile of the matrix instructions in both directions: the
+// work inside a chunk grows with its length, that on the state does not shrink below it, and the triangular system is
+// solved in registers. The inverse Z of its matrix is formed by forward substitution in float32: a product of
+// powers of W would cancel catastrophically where the keys of neighbouring tokens are alike.
+//
+// The products' precision (mma.cuh): Half for bfloat16 inputs, Full for float32 ones. Gradients of a few tokens in
+// bfloat16 take Full too (delta_full).
+#pragma once
+#include "delta.cuh"
+#include "mma.cuh"
+
+namespace gb {
+
+constexpr int kChunk = 16;
+constexpr int kTile = 32;  // tokens that a block holds at a time
+
+// A 16 x 16 matrix that a chunk's products use: two bfloat16 each, or float32.
+template <class P>
+struct Square;
+template <>
+struct Square<Half> {
+    bf16 hi[kChunk][24], lo[kChunk][24];
+    __device__ __forceinline__ void put(int r, int c, float x, float y) {  // (r, c) and (r, c + 1), c even
+        uint32_t h, l;
+        split(x, y, h, l);
+        *(uint32_t *)&hi[r][c] = h, *(uint32_t *)&lo[r][c] = l;
+    }
+    __device__ __forceinline__ void put(int r, int c, float x) {
+        hi[r][c] = __float2bfloat16_rn(x);
+        lo[r][c] = __float2bfloat16_rn(x - __bfloat162float(hi[r][c]));
+    }
+    __device__ __forceinline__ Half::B1 n_rows1(int lane) const { return Half::n_rows(&hi[0][0], 24, 0, 0, lane); }
+    __device__ __forceinline__ Half::B2 n_rows(int lane) const {
+        Half::B2 b;
+        ldsm(b.hi, at_b(&hi[0][0], 24, 0, 0, lane)), ldsm(b.lo, at_b(&lo[0][0], 24, 0, 0, lane));
+        return b;
+    }
+    __device__ __forceinline__ Half::B2 k_rows(int lane) const {
+        Half::B2 b;
+        ldsm_t(b.hi, at_a(&hi[0][0], 24, 0, 0, lane)), ldsm_t(b.lo, at_a(&lo[0][0], 24, 0, 0, lane));
+        return b;
+    }
+};
+template <>
+struct Square<Full> {
+    float x[kChunk][24];
+    __device__ __forceinline__ void put(int r, int c, float u, float v) { *(float2 *)&x[r][c] = make_float2(u, v); }
+    __device__ __forceinline__ void put(int r, int c, float u) { x[r][c] = u; }
+    __device__ __forceinline__ Full::B1 n_rows1(int lane) const { return Full::n_rows(&x[0][0], 24, 0, 0, lane); }
+    __device__ __forceinline__ Full::B1 n_rows(int lane) const { return Full::n_rows(&x[0][0], 24, 0, 0, lane); }
+    __device__ __forceinline__ Full::B1 k_rows(int lane) const { return Full::k_rows(&x[0][0], 24, 0, 0, lane); }
+};
+
+// What one chunk needs besides its rows: Z (or T), P, and the tokens' factors.
+template <class P>
+struct alignas(16) Chunk {
+    Square<P> z, p;
+    float wt[kChunk][20];   // the strictly lower matrix, transposed
+    float a[kChunk], d[kChunk], b[kChunk];
+    int since[kChunk];      // tokens of the chunk up to this one that start afresh
+    float a_end;
+};
+
+// A token's gates, held by lanes i and i + 16 of the warp that prepares the chunk.
+struct Gate {
+    float g, b;
+    bool fresh;
+};
+
+template <class T>
+__device__ __forceinline__ Gate load_gate(const goib2d_delta_desc &d, int64_t n, int64_t t, int h) {
+    if (t < 0 || t >= d.n_steps) return {0.0f, 0.0f, false};
+    Gate r;
+    r.g = to_float(*row<T>(d.g, d.g_stride, n, t, h));
+    r.b = to_float(*row<T>(d.beta, d.beta_stride, n, t, h));
+    r.fresh = (d.reset && d.reset[n * d.reset_stride[0] + t * d.reset_stride[1]]) || expf(r.g) == 0.0f;
+    return r;
+}
+
+// A warp prepares one chunk from its 16 rows of Q and K. BACK: (I + diag(b) W)^-1, else (I + W diag(b))^-1.
+template <class P, int KP, bool BACK>
+__device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, const typename P::E *K, int pitch, Gate gate,
+                                        float scale, int lane) {
+    const int i = lane & 15, g = lane >> 2, t = lane & 3;
+    // G in float64: differences of sums over a chunk of strong decays keep float32's precision
+    double G = gate.fresh ? 0.0 : (double)gate.g;
+#pragma unroll
+    for (int o = 1; o < kChunk; o *= 2) {
+        const double y = __shfl_up_sync(~0u, G, o, 16);
+        if (i >= o) G += y;
+    }
+    const uint32_t fresh = __ballot_sync(~0u, gate.fresh) & 0xffffu;
+    const int since = __popc(fresh & ((2u << i) - 1)), all = __popc(fresh);
+    const double end = __shfl_sync(~0u, G, 15);
+    if (lane < 16) {
+        c.a[i] = since ? 0.0f : expf((float)G);
+        c.d[i] = since == all ? expf((float)(end - G)) : 0.0f;
+        c.b[i] = gate.b;
+        c.since[i] = since;
+        if (lane == 0) c.a_end = all ? 0.0f : expf((float)end);
+    }
+    float kk[2][4] = {}, qk[2][4] = {};
+#pragma unroll
+    for (int x = 0; x < KP; x += 16) {
+        const auto kb = P::n_rows(K, pitch, 0, x, lane);
+        P::mul(kk[0], kk[1], P::a_rows(K, pitch, 0, x, lane), kb);
+        P::mul(qk[0], qk[1], P::a_rows(Q, pitch, 0, x, lane), kb);
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        const int row = g + 8 * r;
+        const double Gi = __shfl_sync(~0u, G, row);
+        const int si = __popc(fresh & ((2u << row) - 1));
+        const float bi = __shfl_sync(~0u, gate.b, row);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float p[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int col = n * 8 + 2 * t + e;
+                const double Gj = __shfl_sync(~0u, G, col);
+                const float bj = __shfl_sync(~0u, gate.b, col);
+                const bool seen = col <= row && __popc(fresh & ((2u << col) - 1)) == si;
+                const float D = seen ? expf((float)(Gi - Gj)) : 0.0f;
+                c.wt[col][row] = seen && col < row ? D * kk[n][2 * r + e] * (BACK ? bi : bj) : 0.0f;
+                p[e] = seen ? scale * D * qk[n][2 * r + e] : 0.0f;
+            }
+            c.p.put(row, n * 8 + 2 * t, p[0], p[1]);
+        }
+    }
+    __syncwarp();
+    // column i of the inverse, right-looking
+    float z[kChunk];
+#pragma unroll
+    for (int r = 0; r < kChunk; ++r) z[r] = r == i ? 1.0f : 0.0f;
+#pragma unroll
+    for (int j = 0; j < kChunk - 1; ++j) {
+        const float zj = j < i ? 0.0f : z[j];  // 0 above the diagonal, whatever W holds there
+#pragma unroll
+        for (int q4 = (j + 1) / 4 * 4; q4 < kChunk; q4 += 4) {
+            const float4 w = *(const float4 *)&c.wt[j][q4];
+            if (q4 > j) z[q4] -= w.x * zj;
+            if (q4 + 1 > j) z[q4 + 1] -= w.y * zj;
+            if (q4 + 2 > j) z[q4 + 2] -= w.z * zj;
+            z[q4 + 3] -= w.w * zj;
+        }
+    }
+    if (fresh)  // 0 times what is not finite before such a token
+#pragma unroll
+        for (int r = 0; r < kChunk; ++r)
+            if (r < i || __popc(fresh & ((2u << r) - 1)) != since) z[r] = 0.0f;
+    if (lane < 16) {
+#pragma unroll
+        for (int r = 0; r < kChunk; ++r) c.z.put(r, i, z[r]);
+    }
+}
+
+// Rows of a strided tensor into shared memory, zeros past `rows` and `cols`. Aligned rows of the same type come by
+// asynchronous copies.
+template <class E, class T>
+__device__ __forceinline__ void load_rows(E *to, int pitch, const T *from, int64_t stride, int rows, int count, int cols,
+                                          int padded, bool wide, int tid, int threads) {
+    if constexpr (sizeof(T) == sizeof(E)) {
+        if (wide) {
+            constexpr int N = 16 / sizeof(E);
+            const int per = padded / N;
+            for (int x = tid; x < count * per; x += threads) {
+                const int r = x / per, c = (x - r * per) * N;
+                E *p = to + r * pitch + c;
+                if (r < rows && c < cols) cp_async16(p, from + r * stride + c);
+                else *(uint4 *)p = make_uint4(0, 0, 0, 0);
+            }
+            return;
+        }
+    }
+    const int per = padded / 2;
+    for (int x = tid; x < count * per; x += threads) {
+        const int r = x / per, c = (x - r * per) * 2;
+        const T *p = from + (int64_t)r * stride + c;
+        const float u = r < rows && c < cols ? to_float(p[0]) : 0.0f, v = r < rows && c + 1 < cols ? to_float(p[1]) : 0.0f;
+        if constexpr (sizeof(E) == 2) *(uint32_t *)(to + r * pitch + c) = pack(u, v);
+        else *(float2 *)(to + r * pitch + c) = make_float2(u, v);
+    }
+}
+
+// 16 x 16 values (rows v, columns tokens) of one accumulator pair, to the rows of a strided tensor; tokens: a bit each
+template <class T>
+__device__ __forceinline__ void store_direct(T *to, int64_t stride, uint32_t tokens, int v0, int V, const float (&c)[2][4],
+                                             int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int token = n * 8 + 2 * t + (e & 1), v = v0 + g + (e >> 1) * 8;
+            if (tokens >> token & 1 && v < V) to[token * stride + v] = from_float<T>(c[n][e]);
+        }
+}
+
+// The same for MT tiles by way of the warp's own columns of a [token][v] buffer, for rows of 16-byte pieces.
+template <int MT>
+__device__ __forceinline__ void store_rows(bf16 *to, int64_t stride, uint32_t tokens, int v0, int V, bool wide, bf16 *buf,
+                                           int pitch, const float (&c)[MT][2][4], int lane) {
+    __syncwarp();
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+        stsm_t((void *)at_b(buf, pitch, 0, v0 + 16 * m, lane), Half::rounded(c[m][0], c[m][1]).x);
+    __syncwarp();
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int x = lane + 32 * m, token = x / (2 * MT), v = v0 + x % (2 * MT) * 8;
+        if (!(tokens >> token & 1) || v >= V) continue;
+        const bf16 *p = buf + token * pitch + v;
+        bf16 *q = to + token * stride + v;
+        if (wide) *(uint4 *)q = *(const uint4 *)p;
+        else
+            for (int e = 0; e < 8 && v + e < V; ++e) q[e] = p[e];
+    }
+    __syncwarp();
+}
+
+// A 16-row tile of S^T to the fragments kept for the backward pass (Saved), and a thread's 8 values back: rows v = g,
+// g + 8 and columns 2 t, 2 t + 1, 8 on, as two accumulator tiles.
+template <class E, int KT>
+__device__ __forceinline__ void keep_state(void *kept, int64_t tile, const float (&S)[2 * KT][4], int lane) {
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+        const int64_t x = (tile + j) * 32 + lane;
+        const float(&c0)[4] = S[2 * j], (&c1)[4] = S[2 * j + 1];
+        if constexpr (sizeof(E) == 2) {
+            const Half::A1 y = Half::rounded(c0, c1);
+            ((uint4 *)kept)[x] = make_uint4(y.x[0], y.x[1], y.x[2], y.x[3]);
+        } else {
+            ((float4 *)kept)[2 * x] = make_float4(c0[0], c0[1], c0[2], c0[3]);
+            ((float4 *)kept)[2 * x + 1] = make_float4(c1[0], c1[1], c1[2], c1[3]);
+        }
+    }
+}
+template <class E>
+__device__ __forceinline__ void kept_values(float (&v)[8], const void *kept, int64_t x) {
+    if constexpr (sizeof(E) == 2) {
+        const uint4 y = ((const uint4 *)kept)[x];
+        v[0] = low(y.x), v[1] = high(y.x), v[2] = low(y.y), v[3] = high(y.y);
+        v[4] = low(y.z), v[5] = high(y.z), v[6] = low(y.w), v[7] = high(y.w);
+    } else {
+        *(float4 *)v = ((const float4 *)kept)[2 * x], *(float4 *)(v + 4) = ((const float4 *)kept)[2 * x + 1];
+    }
+}
+// The 8 values of a thread into rows of S^T in shared memory.
+template <class E>
+__device__ __forceinline__ void put_state(E *St, int pitch, int tile_v, int tile_k, const float (&v)[8], int lane) {
+    E *p = St + (tile_v * 16 + (lane >> 2)) * pitch + tile_k * 16 + 2 * (lane & 3);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        E *q = p + (e & 1) * 8 * pitch + (e >> 1) * 8;
+        if constexpr (sizeof(E) == 2) *(uint32_t *)q = pack(v[2 * e], v[2 * e + 1]);
+        else *(float2 *)q = make_float2(v[2 * e], v[2 * e + 1]);
+    }
+}
+
+}  // namespace gb

@@ -1,0 +1,259 @@
+// The gated delta rule over rollouts (goib2d_delta_forward), in chunks of 16 tokens (delta_chunk.cuh).
+//
+// One block per (world, head); each warp owns MT * 16 columns of S, as the transposed accumulators S^T [V][K] of its
+// matrix products, for the whole rollout: q, k, v are read once, o written once, and the state never leaves the
+// registers. A chunk's products chain without shared memory: S^T is the A operand of S^T K^T and S^T Q^T, their
+// result (V - a Y)^T that of (..) Z^T, its result u^T that of u^T P^T and of the update u^T K. Tiles of two chunks are
+// loaded ahead by asynchronous copies while the warps solve the current one; the warps share out the chunks' Z and P.
+#include "delta_chunk.cuh"
+
+namespace gb {
+namespace {
+
+struct Forward {
+    goib2d_delta_desc d;
+    void *r;          // [n][h][t][V], or NULL
+    void *kept;       // S at the start of every span, in fragments (Saved), or NULL
+    int32_t keep;     // tokens of a span
+    int32_t tiles_v;  // 16-column tiles of V
+    bool wide_q, wide_k, wide_v, wide_o, wide_r;
+};
+
+template <class P, int KP, int MT>
+struct Layout {
+    static constexpr int pitch = KP + 8, E = sizeof(typename P::E);
+    __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (E == 2 ? 8 : 4); }
+    __host__ __device__ static int stage(int warps) { return kTile * (2 * pitch + v_pitch(warps)) * E; }
+    __host__ __device__ static int bytes(int warps) { return 2 * stage(warps) + kTile / kChunk * (int)sizeof(Chunk<P>); }
+};
+
+template <class T, class P, int KP, int MT>
+__global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_forward_kernel(const __grid_constant__ Forward f) {
+    using L = Layout<P, KP, MT>;
+    using E = typename P::E;
+    constexpr int KT = KP / 16;
+    constexpr bool half = sizeof(E) == 2;
+    extern __shared__ __align__(16) char sm[];
+    const goib2d_delta_desc &d = f.d;
+    const int K = d.key_dim, V = d.value_dim, threads = blockDim.x, warps = threads / 32;
+    const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
+    const int64_t nh = blockIdx.x, n = nh / d.heads, steps = d.n_steps;
+    const int h = (int)(nh - n * d.heads), hk = h / (d.heads / d.key_heads);
+    const int stage = L::stage(warps), vp = L::v_pitch(warps), v0 = w * 16 * MT;
+    Chunk<P> *chunks = (Chunk<P> *)(sm + 2 * stage);
+
+    float S[MT][KP / 8][4];  // S^T: rows v, columns k
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < KP / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = v0 + 16 * m + g + (e >> 1) * 8, k = j * 8 + 2 * t + (e & 1);
+                S[m][j][e] = d.state_in && v < V && k < K ? d.state_in[(nh * K + k) * V + v] : 0.0f;
+            }
+
+    const T *q0 = row<T>(d.q, d.q_stride, n, 0, hk), *k0 = row<T>(d.k, d.k_stride, n, 0, hk);
+    const T *v_0 = row<T>(d.v, d.v_stride, n, 0, h);
+    auto load = [&](int64_t tile) {
+        E *Q = (E *)(sm + (tile & 1) * stage), *Kb = Q + kTile * L::pitch, *Vb = Kb + kTile * L::pitch;
+        const int64_t at = tile * kTile;
+        const int left = (int)(steps - at < kTile ? steps - at : kTile);
+        load_rows(Q, L::pitch, q0 + at * d.q_stride[1], d.q_stride[1], left, kTile, K, KP, f.wide_q, tid, threads);
+        load_rows(Kb, L::pitch, k0 + at * d.k_stride[1], d.k_stride[1], left, kTile, K, KP, f.wide_k, tid, threads);
+        load_rows(Vb, vp, v_0 + at * d.v_stride[1], d.v_stride[1], left, kTile, V, warps * 16 * MT, f.wide_v, tid, threads);
+        cp_commit();
+    };
+    const int64_t tiles = (steps + kTile - 1) / kTile;
+    if (tiles) load(0);
+    Gate gate[kTile / kChunk];
+    auto gates = [&](int64_t tile) {
+#pragma unroll
+        for (int s = 0; s < kTile / kChunk; ++s)
+            if (s % warps == w) gate[s] = load_gate<T>(d, n, tile * kTile + s * kChunk + (lane & 15), h);
+    };
+    gates(0);
+    for (int64_t tile = 0; tile < tiles; ++tile) {
+        const E *Q = (const E *)(sm + (tile & 1) * stage), *Kb = Q + kTile * L::pitch;
+        E *Vb = (E *)(Kb + kTile * L::pitch);
+        cp_wait<0>();
+        __syncthreads();
+        if (tile + 1 < tiles) load(tile + 1);
+#pragma unroll
+        for (int s = 0; s < kTile / kChunk; ++s)
+            if (s % warps == w)
+                prepare<P, KP, false>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
+                                      d.scale, lane);
+        if (tile + 1 < tiles) gates(tile + 1);
+        __syncthreads();
+        if (f.kept && tile * kTile % f.keep == 0) {
+            const int64_t at = nh * ((steps + f.keep - 1) / f.keep) + tile * kTile / f.keep;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+                if (w * MT + m < f.tiles_v) keep_state<E, KT>(f.kept, (at * f.tiles_v + w * MT + m) * KT, S[m], lane);
+        }
+#pragma unroll 1
+        for (int s = 0; s < kTile / kChunk; ++s) {
+            const int64_t at = tile * kTile + s * kChunk;
+            if (at >= steps) break;
+            const Chunk<P> &c = chunks[s];
+            const E *Qs = Q + s * kChunk * L::pitch, *Ks = Kb + s * kChunk * L::pitch;
+            E *Vs = Vb + s * kChunk * vp;
+            const uint32_t whole = steps - at < kChunk ? (1u << (steps - at)) - 1 : 0xffffu;
+            // All tokens of the chunk at once (only == -1). Within the products a token meets the others as 0 times
+            // them, which infinities and NaN pass; a chunk that holds any is done again token by token, each with
+            // the tokens before it that its state has seen and nothing else.
+            int only = -1;
+        again:
+            auto in = [&](int e) {  // whether the thread's column e (tokens 2 t, 2 t + 1, and 8 on) takes part
+                const int i = (e >> 1) * 8 + 2 * t + (e & 1);
+                return i <= only && c.since[i] == c.since[only];
+            };
+            float Y[MT][2][4] = {}, O[MT][2][4] = {};
+#pragma unroll
+            for (int j = 0; j < KT; ++j) {
+                const typename P::B1 kb = P::n_rows(Ks, L::pitch, 0, 16 * j, lane), qb = P::n_rows(Qs, L::pitch, 0, 16 * j, lane);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const typename P::A2 a = P::exact(S[m][2 * j], S[m][2 * j + 1]);
+                    P::mul(Y[m][0], Y[m][1], a, kb);
+                    P::mul(O[m][0], O[m][1], P::first(a), qb);  // Half: o is rounded to bfloat16, S once before it
+                }
+            }
+            const typename P::B2 z = c.z.n_rows(lane);
+            const typename P::B1 p = c.p.n_rows1(lane);
+            float bad = 0.0f;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                float x[2][4];
+                P::values_t(x, Vs, vp, 0, v0 + 16 * m, lane);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float a = c.a[j * 8 + 2 * t + (e & 1)];
+                        x[j][e] -= a == 0.0f ? 0.0f : a * Y[m][j][e];  // nothing of the old state, not even NaN
+                        if (only >= 0 && !in(2 * j + (e & 1))) x[j][e] = 0.0f;
+                        O[m][j][e] = a == 0.0f ? 0.0f : O[m][j][e] * (d.scale * a);
+                        Y[m][j][e] = 0.0f;
+                    }
+                P::mul(Y[m][0], Y[m][1], P::exact(x[0], x[1]), z);  // r
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) bad += 0.0f * (Y[m][j][e] * c.b[j * 8 + 2 * t + (e & 1)]);
+            }
+            if (only < 0 && __any_sync(~0u, bad != 0.0f)) {
+                only = 0;
+                goto again;
+            }
+            const uint32_t tokens = only < 0 ? whole : whole & 1u << only;
+            if (f.r) {
+                E *to = (E *)f.r + (nh * steps + at) * V;
+                if (half && only < 0)
+                    store_rows<MT>((bf16 *)to, V, tokens, v0, V, f.wide_r, (bf16 *)Vs, vp, Y, lane);
+                else
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) store_direct<E>(to, V, tokens, v0 + 16 * m, V, Y[m], lane);
+            }
+            typename P::A2 u[MT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        Y[m][j][e] *= c.b[j * 8 + 2 * t + (e & 1)];
+                        if (only >= 0 && !in(2 * j + (e & 1))) Y[m][j][e] = 0.0f;
+                    }
+                P::mul(O[m][0], O[m][1], P::rounded(Y[m][0], Y[m][1]), p);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float dd = c.d[j * 8 + 2 * t + (e & 1)];
+                        Y[m][j][e] = dd == 0.0f ? 0.0f : dd * Y[m][j][e];
+                    }
+                u[m] = P::exact(Y[m][0], Y[m][1]);
+            }
+            T *to = row<T>(d.out, d.out_stride, n, at, h);
+            if (half && only < 0)
+                store_rows<MT>((bf16 *)to, d.out_stride[1], tokens, v0, V, f.wide_o, (bf16 *)Vs, vp, O, lane);
+            else
+#pragma unroll
+                for (int m = 0; m < MT; ++m) store_direct<T>(to, d.out_stride[1], tokens, v0 + 16 * m, V, O[m], lane);
+            if (only >= 0 && only < kChunk - 1) {
+                ++only;
+                goto again;
+            }
+            const float a_end = c.a_end;
+#pragma unroll
+            for (int j = 0; j < KT; ++j) {
+                typename P::B1 kb = P::k_rows(Ks, L::pitch, 0, 16 * j, lane);
+                if (only >= 0) P::mask_k(kb, in(0) | in(1) << 1 | in(2) << 2 | in(3) << 3);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    float(&c0)[4] = S[m][2 * j], (&c1)[4] = S[m][2 * j + 1];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        c0[e] = a_end == 0.0f ? 0.0f : a_end * c0[e], c1[e] = a_end == 0.0f ? 0.0f : a_end * c1[e];
+                    P::mul(c0, c1, u[m], kb);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < KP / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int v = v0 + 16 * m + g + (e >> 1) * 8, k = j * 8 + 2 * t + (e & 1);
+                if (v < V && k < K) d.state_out[(nh * K + k) * V + v] = S[m][j][e];
+            }
+}
+
+template <class T, class P, int KP, int MT>
+cudaError_t forward_of(const Forward &f, cudaStream_t s) {
+    const int warps = (f.d.value_dim + 16 * MT - 1) / (16 * MT);
+    const size_t smem = Layout<P, KP, MT>::bytes(warps);
+    cudaError_t e = allow_smem(goib2d_delta_forward_kernel<T, P, KP, MT>, smem);
+    if (e != cudaSuccess) return e;
+    goib2d_delta_forward_kernel<T, P, KP, MT><<<(unsigned)(f.d.n_worlds * f.d.heads), 32 * warps, smem, s>>>(f);
+    return cudaGetLastError();
+}
+
+template <class T, class P, int KP>
+cudaError_t forward_wide(const Forward &f, cudaStream_t s) {
+    return f.d.value_dim <= 16 ? forward_of<T, P, KP, 1>(f, s) : forward_of<T, P, KP, 2>(f, s);
+}
+
+template <class T, class P>
+cudaError_t forward_typed(const goib2d_delta_desc &d, void *saved, cudaStream_t s) {
+    Forward f{d};
+    const Saved at = delta_saved(d);
+    f.r = saved, f.kept = saved ? (char *)saved + at.r : nullptr, f.keep = at.keep, f.tiles_v = at.tiles_v;
+    const int V = d.value_dim, z = sizeof(T);
+    f.wide_q = rows_aligned(d.q, d.q_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
+    f.wide_k = rows_aligned(d.k, d.k_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
+    f.wide_v = rows_aligned(d.v, d.v_stride, d.n_worlds, d.n_steps, d.heads, V, z);
+    f.wide_o = rows_aligned(d.out, d.out_stride, d.n_worlds, d.n_steps, d.heads, V, z);
+    f.wide_r = V % 8 == 0;
+    switch (padded_keys(d.key_dim)) {
+        case 16: return forward_wide<T, P, 16>(f, s);
+        case 32: return forward_wide<T, P, 32>(f, s);
+        case 64: return forward_wide<T, P, 64>(f, s);
+        default: return forward_wide<T, P, 128>(f, s);
+    }
+}
+
+}  // namespace
+
+int64_t delta_saved_bytes(const goib2d_delta_desc &d) { return delta_saved(d).bytes; }
+
+cudaError_t launch_delta_forward(const goib2d_delta_desc &d, void *saved, cudaStream_t s) {
+    if (d.dtype == GOIB2D_FLOAT32) return forward_typed<float, Full>(d, saved, s);
+    return saved && delta_full(d) ? forward_typed<bf16, Full>(d, saved, s) : forward_typed<bf16, Half>(d, saved, s);
+}
+
+}  // namespace gb

@@ -1,4 +1,4 @@
-// The policy's side of a batch of worlds (delta.cu, clip.cu): parameters shared by the kernels and the C entries.
+// The policy's side of a batch of worlds (delta_*.cu, clip.cu): parameters shared by the kernels and the C entries.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -9,7 +9,7 @@
 
 namespace gb {
 
-// ---- the gated delta rule (delta.cu)
+// ---- the gated delta rule (delta_step.cu, delta_forward.cu, delta_backward.cu)
 
 cudaError_t launch_delta_step(const goib2d_delta_desc &d, cudaStream_t s);
 cudaError_t launch_delta_forward(const goib2d_delta_desc &d, void *saved, cudaStream_t s);

@@ -13,7 +13,7 @@ strength b = beta does
 and a token whose `reset` is set (the world's reset came before it), or whose decay is 0 in float32, starts from
 S' = 0 whatever S held. q and k may have fewer heads than v: value head h reads key head h // (heads // key_heads).
 All of q, k, v, g, beta are float32 or all bfloat16; memories and every sum are float32. The kernels are in
-libgoib2d.so (csrc/delta.cu, csrc/clip.cu; the C calls are goib2d_delta_* and goib2d_clip_grads): there is no CPU
+libgoib2d.so (csrc/delta_*.cu, csrc/clip.cu; the C calls are goib2d_delta_* and goib2d_clip_grads): there is no CPU
 path. Calls run on the current stream of the tensors' device and return without waiting for it.
 """
 import struct

@@ -1,8 +1,8 @@
 """The policy operators (goib2d.delta_step_, delta_rule, clip_grads_) against their definitions in 64 bits.
 
 Tolerances, on the 2-norm of the difference over the 2-norm of the result. float32: matrix products run on operands
-split into two bfloat16 (a relative error of 2^-17 a product at most, and independent from product to product), in
-chains of at most four products within a chunk: 4 * 2^-17 = 3.1e-5 at most. bfloat16 results: the rounding of the
+split in two parts (a relative error of 2^-17 a product at most with bfloat16 parts, less with tf32 ones, and independent
+from product to product), in chains of at most four products within a chunk: 4 * 2^-17 = 3.1e-5 at most. bfloat16 results: the rounding of the
 result (2^-9) and of the two operands of the product that makes it (2^-9 each) at most: 3 * 2^-9 = 5.9e-3. States are
 float32 whatever the inputs' type."""
 import ctypes as C
@@ -71,7 +71,7 @@ def off(got, want):
 
 
 # (worlds, steps, heads, key heads, K, V): one token, part of a chunk, whole chunks, one more; odd and largest channels
-SIZES = [(1, 1, 1, 1, 1, 1), (3, 2, 2, 2, 16, 16), (2, 15, 2, 2, 32, 32), (3, 16, 3, 1, 64, 64),
+SIZES = [(1, 1, 1, 1, 1, 1), (2, 1, 2, 1, 3, 5), (3, 2, 2, 2, 16, 16), (2, 15, 2, 2, 32, 32), (3, 16, 3, 1, 64, 64),
          (2, 17, 4, 2, 64, 32), (1, 31, 1, 1, 32, 64), (5, 33, 6, 3, 40, 71), (2, 64, 2, 1, 128, 128),
          (1, 65, 2, 2, 100, 128), (2, 130, 1, 1, 8, 128), (1, 129, 2, 1, 128, 8), (1, 600, 1, 1, 48, 24),
          (40, 20, 4, 4, 64, 64)]
@@ -254,7 +254,35 @@ def test_states_that_start_afresh(K, V, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("g", [0.0, -1e-6, 0.05])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("V", [16, 40, 64])
+def test_a_world_recovers_from_values_that_are_not_finite(V, dtype, bad):
+    """A world whose simulation blew up sends NaN or infinities until it is reset: what comes after the reset, in the
+    same chunk of tokens or later, is as if the memory had been empty, and other worlds do not notice."""
+    n, t, h, K = 6, 70, 2, 32
+    a = rollout(n, t, h, 1, K, V, dtype, seed=13, resets=False)
+    reset = torch.zeros(n, t, dtype=torch.bool, device="cuda")
+    spoilt = torch.zeros(n, t, dtype=torch.bool, device="cuda")
+    for world, (name, first, last) in enumerate((("v", 3, 5), ("k", 4, 8), ("q", 7, 8), ("k", 14, 15), ("v", 15, 33))):
+        a[name][world, first:last + 1] = bad
+        reset[world, [first - 2, last + 1, last + 4]] = True
+        spoilt[world, first:last + 1] = True
+    out, last = goib2d.delta_rule(**dict(a, reset=reset))
+    state, steps = a["state"].clone(), []
+    for i in range(t):
+        steps.append(goib2d.delta_step_(state, *(a[x][:, i] for x in ("q", "k", "v", "g", "beta")), reset=reset[:, i]))
+    clean = {x: torch.where(spoilt.view(n, t, *[1] * (y.dim() - 2)), 0, y) if x in ("q", "k", "v") else y
+             for x, y in a.items()}
+    want, want_last = recurrence(**wide(dict(clean, reset=reset)))
+    for got, got_last in ((out, last), (torch.stack(steps, 1), state)):
+        assert off(got[~spoilt], want[~spoilt.cpu()]) <= TOL[dtype]
+        assert off(got_last, want_last) <= TOL[F32]
+        assert not torch.isfinite(got[spoilt]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("g", [0.0, -1e-6, -30.0, -90.0, 0.05])
 def test_decays_from_none_to_all(g):
     """No decay at all, a chunk whose decays multiply to less than float32 holds, and growth."""
     a = rollout(2, 70, 2, 1, 32, 32, F32, seed=9, resets=False)
