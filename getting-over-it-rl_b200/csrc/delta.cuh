@@ -70,10 +70,13 @@ inline Saved delta_saved(const goib2d_delta_desc &d) {
     return s;
 }
 
+// Allow a kernel `bytes` of dynamic shared memory, and the SM's largest share of it for its blocks.
 template <class F>
 cudaError_t allow_smem(F *f, size_t bytes) {
-    return bytes <= 48 << 10 ? cudaSuccess
-                             : cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess && bytes > 48 << 10)
+        e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e;
 }
 
 }  // namespace gb

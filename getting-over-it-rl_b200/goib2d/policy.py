@@ -17,6 +17,8 @@ libgoib2d.so (csrc/delta_*.cu, csrc/clip.cu; the C calls are goib2d_delta_* and 
 path. Calls run on the current stream of the tensors' device and return without waiting for it.
 """
 import struct
+from array import array
+from contextlib import nullcontext
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -26,7 +28,7 @@ from . import native
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1}
 _DESC = struct.Struct("2q5if9P20q")   # goib2d_delta_desc
 _GRADS = struct.Struct("8P18q")       # goib2d_delta_grads
-_GRAD = struct.Struct("Pqi4x")        # goib2d_grad
+_GRAD = struct.Struct("Pqi4x")        # goib2d_grad (as three int64 words in clip_grads_' table)
 MAX_DIM = 128                         # largest key_dim and value_dim
 
 
@@ -75,8 +77,19 @@ def _sizes(q, v, steps):
 
 
 def _on(device):
-    """The device's guard, where it is not the current one."""
-    return torch.cuda.device(device)
+    """The device's guard, where it is not the current one (the C calls run on the current device)."""
+    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _alike(dt, device, *tensors):
+    for x in tensors:
+        if x.dtype is not dt or x.device != device:
+            return False
+    return True
 
 
 def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
@@ -86,27 +99,31 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     delta_rule."""
     n, _, h, hk, K, V = _sizes(q, v, False)
     device, dt = v.device, v.dtype
-    if torch.is_grad_enabled() and any(x.requires_grad for x in (state, q, k, v, g, beta)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
+                                    beta.requires_grad or state.requires_grad):
         raise ValueError("delta_step_ is not differentiable: use delta_rule, or torch.no_grad()")
-    sp = _state("state", state, (n, h, K, V), device)
-    qp, qs = _rows("q", q, (n, hk, K), dt, device)
-    kp, ks = _rows("k", k, (n, hk, K), dt, device)
-    vp, vs = _rows("v", v, (n, h, V), dt, device)
-    gp, gs = _rows("g", g, (n, h), dt, device, False)
-    bp, bs = _rows("beta", beta, (n, h), dt, device, False)
-    rp, rs = _reset(reset, (n,), device)
     if out is None:
         out = torch.empty((n, h, V), dtype=dt, device=device)
-    op, os_ = _rows("out", out, (n, h, V), dt, device)
-    desc = _DESC.pack(n, 1, h, hk, K, V, _DTYPE[dt], K ** -0.5 if scale is None else scale, qp, kp, vp, gp, bp, rp, sp, sp, op,
+    qs, ks, vs, gs, bs, os_ = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride(), out.stride()
+    # all of it in one expression first: an acting loop calls this once per world step
+    if not (_alike(dt, device, q, k, v, g, beta, out) and q.shape == k.shape and q.shape[0] == n and
+            out.shape == v.shape and g.shape == beta.shape == (n, h) and state.shape == (n, h, K, V) and
+            qs[2] == ks[2] == vs[2] == os_[2] == 1 and state.is_contiguous() and
+            _alike(torch.float32, device, state)):
+        _state("state", state, (n, h, K, V), device)
+        for name, x, shape in (("q", q, (n, hk, K)), ("k", k, (n, hk, K)), ("v", v, (n, h, V)), ("out", out, (n, h, V))):
+            _rows(name, x, shape, dt, device)
+        for name, x in (("g", g), ("beta", beta)):
+            _rows(name, x, (n, h), dt, device, False)
+    rp, rs = _reset(reset, (n,), device)
+    sp = state.data_ptr()
+    desc = _DESC.pack(n, 1, h, hk, K, V, _DTYPE[dt], K ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
+                      v.data_ptr(), g.data_ptr(), beta.data_ptr(), rp, sp, sp, out.data_ptr(),
                       qs[0], 0, qs[1], ks[0], 0, ks[1], vs[0], 0, vs[1], gs[0], 0, gs[1], bs[0], 0, bs[1],
                       os_[0], 0, os_[1], rs[0], 0)
     lib = native.load()
-    if device.index == torch.cuda.current_device():
-        native.check(lib.goib2d_delta_step(desc, torch.cuda.current_stream(device).cuda_stream))
-    else:
-        with _on(device):
-            native.check(lib.goib2d_delta_step(desc, torch.cuda.current_stream(device).cuda_stream))
+    with _on(device):
+        native.check(lib.goib2d_delta_step(desc, _raw_stream(device.index)))
     return out
 
 
@@ -140,7 +157,7 @@ def _forward(q, k, v, g, beta, state, reset, scale, train):
             native.check(min(size, 0))
             saved = torch.empty(size, dtype=torch.uint8, device=device)
         native.check(lib.goib2d_delta_forward(desc, saved.data_ptr() if train else None,
-                                              torch.cuda.current_stream(device).cuda_stream))
+                                              _raw_stream(device.index)))
     return out, last, saved
 
 
@@ -182,7 +199,7 @@ class _DeltaRule(torch.autograd.Function):
             native.check(min(size, 0))
             work = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
             native.check(lib.goib2d_delta_backward(desc, grads, saved.data_ptr(), work.data_ptr(),
-                                                   torch.cuda.current_stream(device).cuda_stream))
+                                                   _raw_stream(device.index)))
         return dq, dk, dv, dg, dbeta, first, None, None
 
 
@@ -222,26 +239,26 @@ def clip_grads_(grads, max_norm):
     device = grads[0].device
     if device.type != "cuda":
         raise TypeError("gradients must be CUDA tensors")
-    table, seen = [], set()
+    table = array("q")
     for x in grads:
         dt = _DTYPE.get(x.dtype)
-        if dt is None or x.device != device or x.layout != torch.strided:
+        if dt is None or x.device != device or x.layout is not torch.strided:
             raise ValueError(f"gradients must be dense float32 or bfloat16 tensors on {device}, got {x.dtype} on {x.device}")
         if not (x.is_contiguous() or _dense(x)):
             raise ValueError(f"a gradient of shape {tuple(x.shape)} and strides {x.stride()} is not dense in memory")
-        p = x.data_ptr()
-        if x.numel():
-            if p in seen:
-                raise ValueError("the same gradient twice")
-            seen.add(p)
-            table.append(_GRAD.pack(p, x.numel(), dt))
-    packed = b"".join(table)
+        n = x.numel()
+        if n:
+            table.extend((x.data_ptr(), n, dt))
+    count = len(table) // 3
+    if len(set(table[::3])) != count:
+        raise ValueError("the same gradient twice")
+    packed = table.buffer_info()[0]
     lib = native.load()
     with _on(device):
         norm = torch.empty((), dtype=torch.float32, device=device)
-        size = lib.goib2d_clip_workspace_bytes(packed, len(table))
+        size = lib.goib2d_clip_workspace_bytes(packed, count)
         native.check(min(size, 0))
         work = torch.empty(size, dtype=torch.uint8, device=device)
-        native.check(lib.goib2d_clip_grads(packed, len(table), max_norm, norm.data_ptr(), work.data_ptr(),
-                                           torch.cuda.current_stream(device).cuda_stream))
+        native.check(lib.goib2d_clip_grads(packed, count, max_norm, norm.data_ptr(), work.data_ptr(),
+                                           _raw_stream(device.index)))
     return norm
