@@ -27,6 +27,7 @@ struct Backward {
     int64_t dv_stride[3];
     int32_t keep, tiles_v;
     bool wide_q, wide_k, wide_do, wide_dv, wide_r;
+    bool wide_dqk;           // pairs of channels of dq and dk are aligned
 };
 
 // ---- dS through the rollout, dv and db
@@ -58,15 +59,7 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_back_state_k
     float *db = (float *)(chunks + kTile / kChunk);  // [warp][token of the tile]
 
     float S[MT][KP / 8][4];  // dS^T: rows v, columns k
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < KP / 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = v0 + 16 * m + g + (e >> 1) * 8, k = j * 8 + 2 * t + (e & 1);
-                S[m][j][e] = f.gr.dstate_out && v < V && k < K ? f.gr.dstate_out[(nh * K + k) * V + v] : 0.0f;
-            }
+    load_state<MT, KP>(S, f.gr.dstate_out ? f.gr.dstate_out + nh * K * V : nullptr, K, V, v0, lane);
     const int64_t tiles = (steps + kTile - 1) / kTile;
     const T *q0 = row<T>(d.q, d.q_stride, n, 0, hk), *k0 = row<T>(d.k, d.k_stride, n, 0, hk);
     const T *o0 = f.gr.dout ? row<T>(f.gr.dout, f.gr.dout_stride, n, 0, h) : nullptr;
@@ -186,9 +179,8 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_back_state_k
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float a = c.a[j * 8 + 2 * t + (e & 1)];
-                        x[j][e] *= d.scale * a;
-                        X[m][j][e] *= -a;
+                        x[j][e] *= c.sa[j * 8 + 2 * t + (e & 1)];
+                        X[m][j][e] *= -c.a[j * 8 + 2 * t + (e & 1)];
                     }
                 o[m] = P::exact(x[0], x[1]);
                 y[m] = P::exact(X[m][0], X[m][1]);
@@ -212,344 +204,397 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_back_state_k
     }
     __syncthreads();
     if (tiles) finish(0);
-    if (f.gr.dstate_in)
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int j = 0; j < KP / 8; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int v = v0 + 16 * m + g + (e >> 1) * 8, k = j * 8 + 2 * t + (e & 1);
-                    if (v < V && k < K) f.gr.dstate_in[(nh * K + k) * V + v] = S[m][j][e];
-                }
+    if (f.gr.dstate_in) store_state<MT, KP>(f.gr.dstate_in + nh * K * V, S, K, V, v0, lane);
 }
 
 // ---- dq, dk and dg, span by span
+//
+// A span is cut into blocks of 16 tokens, one a warp. Between two blocks D_ij = a_i m d_j, a_i the decay from i's
+// block's start, d_j that to j's block's end, m that of the blocks between: products instead of exponentials, all of
+// them at most what they make. A warp takes its tokens first as i, over the blocks before them, then as j, over those
+// behind: A and M go through shared memory where they fit (Half), and are made again from the other side otherwise.
 
 template <class P, int KP, int C>
 struct Span {
-    static constexpr int RB = C / 16;                   // row blocks: warps that share the tokens
+    using E = typename P::E;
+    static constexpr int RB = C / 16;                   // blocks
     static constexpr int KH = KP < 64 ? KP : 64;        // channels of dq and dk a warp holds
     static constexpr int warps = RB * (KP / KH);
     static constexpr int pitch = KP + 8;
+    static constexpr bool store = sizeof(E) == 2;
     struct Tokens {
-        float a[C], d[C], b[C], hi[C], lo[C];           // hi + lo: the running sum of g
-        int since[C];
-        float row[KP / KH][C], col[KP / KH][C], pairs[RB][C], end[warps];
-        float a_end;
+        float a[C], d[C], b[C], hi[C], lo[C];           // within the block; hi + lo: the running sum of g / ln 2
+        float through[RB];                              // a block's whole decay
+        int since[C];                                   // tokens of the block up to this one that start afresh
+        float row[KP / KH][C], col[KP / KH][C];         // what a token reads of S0, leaves in the last state
+        float own[C], rows[C], cols[RB][C], end[warps]; // the pairs of a decay, see below
     };
+    E *Q, *K, *O, *V, *R, *S, *A, *M;                   // S: S0^T, then dS1^T (rows v, columns k); A, M: 16 x 24 a block
+    Tokens *x;
     __host__ __device__ static int v_pitch(int tiles_v) { return tiles_v * 16 + 8; }
     __host__ __device__ static int bytes(int tiles_v) {
-        return (int)sizeof(typename P::E) * (2 * C * pitch + 3 * C * v_pitch(tiles_v) + tiles_v * 16 * pitch) +
-               (int)sizeof(Tokens);
+        return (int)sizeof(E) * (2 * C * pitch + 3 * C * v_pitch(tiles_v) + tiles_v * 16 * pitch +
+                                 (store ? RB * (RB + 1) * 16 * 24 : 0)) + (int)sizeof(Tokens);
     }
+    __device__ Span(char *sm, int tiles_v) {
+        const int vp = v_pitch(tiles_v);
+        Q = (E *)sm, K = Q + C * pitch, O = K + C * pitch, V = O + C * vp, R = V + C * vp, S = R + C * vp;
+        A = S + tiles_v * 16 * pitch, M = A + (store ? RB * (RB + 1) / 2 * 16 * 24 : 0);
+        x = (Tokens *)(M + (store ? RB * (RB + 1) / 2 * 16 * 24 : 0));
+    }
+    static __device__ __forceinline__ int block(int ib, int jb) { return (ib * (ib + 1) / 2 + jb) * 16 * 24; }
 };
 
+__device__ __forceinline__ void store_pair(bf16 *p, float x, float y) { *(uint32_t *)p = pack(x, y); }
+__device__ __forceinline__ void store_pair(float *p, float x, float y) { *(float2 *)p = make_float2(x, y); }
+__device__ __forceinline__ void put_block(bf16 *p, const Half::A1 &a, int lane) {  // rows and columns as accumulators
+    bf16 *q = p + (lane >> 2) * 24 + 2 * (lane & 3);
+    *(uint32_t *)q = a.x[0], *(uint32_t *)(q + 8 * 24) = a.x[1];
+    *(uint32_t *)(q + 8) = a.x[2], *(uint32_t *)(q + 8 * 24 + 8) = a.x[3];
+}
+
 template <class T, class P, int KP, int C>
-__global__ void __launch_bounds__(Span<P, KP, C>::warps * 32) goib2d_delta_back_span_kernel(const __grid_constant__ Backward f) {
+__global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof(typename P::E) == 2 ? 3 : 1)
+    goib2d_delta_back_span_kernel(const __grid_constant__ Backward f) {
     using L = Span<P, KP, C>;
     using E = typename P::E;
-    constexpr int RB = L::RB, KH = L::KH, threads = L::warps * 32;
+    constexpr int RB = L::RB, KH = L::KH, threads = L::warps * 32, PL = C / 32;
     extern __shared__ __align__(16) char sm[];
     const goib2d_delta_desc &d = f.d;
     const int K = d.key_dim, V = d.value_dim, tv = f.tiles_v, vp = L::v_pitch(tv), cols = tv * 16;
     const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
-    const int rb = w % RB, part = w / RB, k0 = part * KH;  // 16 tokens, and KH channels of keys
+    const int rb = w % RB, part = w / RB, k0 = part * KH;  // the warp's block of tokens, and its channels
+    const int i0 = rb * 16 + g;                            // the thread's rows: i0, i0 + 8
     const int64_t steps = d.n_steps, spans = (steps + C - 1) / C;
     const int64_t item = blockIdx.x / spans, span = blockIdx.x - item * spans, at = span * C, n = item / d.key_heads;
     const int hk = (int)(item - n * d.key_heads), group = d.heads / d.key_heads;
     const int left = (int)(steps - at < C ? steps - at : C);
+    const L s(sm, tv);
+    auto &x = *s.x;
 
-    E *Q = (E *)sm, *Kb = Q + C * L::pitch, *Ob = Kb + C * L::pitch, *Vb = Ob + C * vp, *Rb = Vb + C * vp;
-    E *St = Rb + C * vp;                                // S0^T, then dS1^T: rows v, columns k
-    auto &x = *(typename L::Tokens *)(St + cols * L::pitch);
-
-    load_rows(Q, L::pitch, row<T>(d.q, d.q_stride, n, at, hk), d.q_stride[1], left, C, K, KP, f.wide_q, tid, threads);
-    load_rows(Kb, L::pitch, row<T>(d.k, d.k_stride, n, at, hk), d.k_stride[1], left, C, K, KP, f.wide_k, tid, threads);
+    load_rows(s.Q, L::pitch, row<T>(d.q, d.q_stride, n, at, hk), d.q_stride[1], left, C, K, KP, f.wide_q, tid, threads);
+    load_rows(s.K, L::pitch, row<T>(d.k, d.k_stride, n, at, hk), d.k_stride[1], left, C, K, KP, f.wide_k, tid, threads);
     float dq[KH / 8][4] = {}, dk[KH / 8][4] = {};
+#pragma unroll 1
     for (int j = 0; j < group; ++j) {
         const int h = hk * group + j;
-        const int64_t nh = n * d.heads + h;
+        const int64_t nh = n * d.heads + h, kept = (nh * spans + span) * tv * (KP / 16) * 32;
         __syncthreads();
         const bool o = f.gr.dout != nullptr;
-        load_rows(Ob, vp, o ? row<T>(f.gr.dout, f.gr.dout_stride, n, at, h) : nullptr, f.gr.dout_stride[1], o ? left : 0, C, V,
+        load_rows(s.O, vp, o ? row<T>(f.gr.dout, f.gr.dout_stride, n, at, h) : nullptr, f.gr.dout_stride[1], o ? left : 0, C, V,
                   cols, f.wide_do, tid, threads);
-        load_rows(Vb, vp, row<E>((const void *)f.dv, f.dv_stride, n, at, h), f.dv_stride[1], left, C, V, cols, f.wide_dv, tid,
+        load_rows(s.V, vp, row<E>((const void *)f.dv, f.dv_stride, n, at, h), f.dv_stride[1], left, C, V, cols, f.wide_dv, tid,
                   threads);
-        load_rows(Rb, vp, (const E *)f.r + (nh * steps + at) * V, V, left, C, V, cols, f.wide_r, tid, threads);
+        load_rows(s.R, vp, (const E *)f.r + (nh * steps + at) * V, V, left, C, V, cols, f.wide_r, tid, threads);
         cp_commit();
-        const int64_t kept = (nh * spans + span) * tv * (KP / 16) * 32;
+        // S0, which may hold anything where the span's first token starts afresh
+        const bool anew = load_gate<T>(d, n, at, h).fresh;
         float end = 0.0f;
         for (int i = tid; i < tv * (KP / 16) * 32; i += threads) {
-            float s[8], ds[8];
-            kept_values<E>(s, f.kept_s, kept + i);
-            kept_values<E>(ds, f.kept_ds, kept + i);
-            put_state<E>(St, L::pitch, i / 32 / (KP / 16), i / 32 % (KP / 16), s, i % 32);
+            if (!anew) {
+                float u[8], v[8];
+                kept_values<E>(u, f.kept_s, kept + i), kept_values<E>(v, f.kept_ds, kept + i);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) end += s[e] * ds[e];
+                for (int e = 0; e < 8; ++e) end += u[e] * v[e];
+            }
+            put_state(s.S, L::pitch, i / 32 / (KP / 16), i / 32 % (KP / 16), f.kept_s, kept + i, i % 32);
         }
         for (int i = 16; i > 0; i >>= 1) end += __shfl_xor_sync(~0u, end, i);
         if (lane == 0) x.end[w] = end;
-        if (w == 0) {
-            // the tokens' gates: C / 32 neighbouring tokens a lane
-            constexpr int PL = C / 32;
-            Gate gt[PL];
-            double G = 0.0;
-            uint32_t fresh[PL];
-#pragma unroll
-            for (int e = 0; e < PL; ++e) {
-                gt[e] = load_gate<T>(d, n, at + lane * PL + e, h);
-                G += gt[e].fresh ? 0.0 : (double)gt[e].g;
-                fresh[e] = __ballot_sync(~0u, gt[e].fresh);
+        if (part == 0) {
+            const int i = lane & 15;
+            const Gate gate = load_gate<T>(d, n, at + rb * 16 + i, h);
+            const double G = running_sum(gate, lane), last = __shfl_sync(~0u, G, 15);
+            const uint32_t fresh = __ballot_sync(~0u, gate.fresh) & 0xffffu;
+            const int since = __popc(fresh & ((2u << i) - 1)), all = __popc(fresh);
+            if (lane < 16) {
+                const int l = rb * 16 + i;
+                x.a[l] = since ? 0.0f : exp2f((float)G), x.d[l] = since == all ? exp2f((float)(last - G)) : 0.0f;
+                x.b[l] = gate.b, x.hi[l] = (float)G, x.lo[l] = (float)(G - (double)(float)G), x.since[l] = since;
+                if (i == 0) x.through[rb] = all ? 0.0f : exp2f((float)last);
             }
-            const double mine = G;
-#pragma unroll
-            for (int i = 1; i < 32; i *= 2) {
-                const double y = __shfl_up_sync(~0u, G, i);
-                if (lane >= i) G += y;
-            }
-            const double last = __shfl_sync(~0u, G, 31);
-            int all = 0, before = 0;
-#pragma unroll
-            for (int e = 0; e < PL; ++e) all += __popc(fresh[e]), before += __popc(fresh[e] & ((1u << lane) - 1));
-            G -= mine;
-#pragma unroll
-            for (int e = 0; e < PL; ++e) {
-                const int i = lane * PL + e;
-                G = (e == 0 && lane == 0 ? 0.0 : G) + (gt[e].fresh ? 0.0 : (double)gt[e].g);
-                before += gt[e].fresh;
-                const float hi = (float)G;
-                x.hi[i] = hi, x.lo[i] = (float)(G - (double)hi), x.b[i] = gt[e].b, x.since[i] = before;
-                x.a[i] = before ? 0.0f : expf(hi);
-                x.d[i] = before == all ? expf((float)(last - G)) : 0.0f;
-            }
-            if (lane == 0) x.a_end = all ? 0.0f : expf((float)last);
         }
         cp_wait<0>();
         __syncthreads();
 
-        const int i0 = rb * 16 + g;  // the thread's rows: i0, i0 + 8
+        const float a_i[2] = {x.a[i0], x.a[i0 + 8]}, b_i[2] = {x.b[i0], x.b[i0 + 8]}, d_i[2] = {x.d[i0], x.d[i0 + 8]};
+        float to = 1.0f, from = 1.0f;  // the decay of the blocks before, and behind
+        for (int i = 0; i < rb; ++i) to *= x.through[i];
+        for (int i = rb + 1; i < RB; ++i) from *= x.through[i];
         // what the tokens read of S0
-        float row_sum[2] = {};
+        float sum[2] = {};
+        if (!anew) {
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                float acc[KH / 8][4] = {};
+                const E *A = which ? s.V : s.O, *with = which ? s.K : s.Q;
 #pragma unroll 1
-        for (int which = 0; which < 2; ++which) {
-            float acc[KH / 8][4] = {};
-            const E *A = which ? Vb : Ob, *with = which ? Kb : Q;
-#pragma unroll 1
-            for (int v = 0; v < tv; ++v) {
-                const typename P::A1 fa = P::a_rows(A, vp, rb * 16, v * 16, lane);
+                for (int v = 0; v < tv; ++v) {
+                    const typename P::A1 fa = P::a_rows(A, vp, rb * 16, v * 16, lane);
 #pragma unroll
-                for (int c = 0; c < KH / 16; ++c)
-                    P::mul(acc[2 * c], acc[2 * c + 1], fa, P::k_rows(St, L::pitch, v * 16, k0 + c * 16, lane));
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const float a = x.a[i0 + 8 * r], scaled = which ? -a : d.scale * a;
-                const E *p = with + (i0 + 8 * r) * L::pitch + k0 + 2 * t;
-                float sum = 0.0f;
-#pragma unroll
-                for (int c = 0; c < KH / 8; ++c) {
-                    float(&y)[4] = acc[c];
-                    y[2 * r] = a == 0.0f ? 0.0f : scaled * y[2 * r];
-                    y[2 * r + 1] = a == 0.0f ? 0.0f : scaled * y[2 * r + 1];
-                    sum += to_float(p[8 * c]) * y[2 * r] + to_float(p[8 * c + 1]) * y[2 * r + 1];
+                    for (int c = 0; c < KH / 16; ++c)
+                        P::mul(acc[2 * c], acc[2 * c + 1], fa, P::k_rows(s.S, L::pitch, v * 16, k0 + c * 16, lane));
                 }
-                row_sum[r] += sum;
-            }
-            if (which == 0) {
 #pragma unroll
-                for (int c = 0; c < KH / 8; ++c)
+                for (int r = 0; r < 2; ++r) {
+                    const float scaled = (which ? -1.0f : d.scale) * a_i[r] * to;
+                    const E *p = with + (i0 + 8 * r) * L::pitch + k0 + 2 * t;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) dq[c][e] += acc[c][e];
-            } else {
-#pragma unroll
-                for (int c = 0; c < KH / 8; ++c)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) dk[c][e] += acc[c][e];
+                    for (int c = 0; c < KH / 8; ++c) {
+                        const float y0 = scaled * acc[c][2 * r], y1 = scaled * acc[c][2 * r + 1];
+                        const float2 z = pair_at(p + 8 * c);
+                        sum[r] += z.x * y0 + z.y * y1;
+                        if (which) dk[c][2 * r] += y0, dk[c][2 * r + 1] += y1;
+                        else dq[c][2 * r] += y0, dq[c][2 * r + 1] += y1;
+                    }
+                }
             }
         }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            row_sum[r] += __shfl_xor_sync(~0u, row_sum[r], 1);
-            row_sum[r] += __shfl_xor_sync(~0u, row_sum[r], 2);
-            if (t == 0) x.row[part][i0 + 8 * r] = row_sum[r];
-        }
-        const float hi_i[2] = {x.hi[i0], x.hi[i0 + 8]}, lo_i[2] = {x.lo[i0], x.lo[i0 + 8]};
-        const int since_i[2] = {x.since[i0], x.since[i0 + 8]};
-        // the warp's tokens as i, those before them as j
-        float before[2] = {};  // sum over the columns so far
+        // the tokens as i: A and M over the tokens up to them. For dg, the pairs A_ij q_i.k_j + M_ij k_i.k_j: those of one
+        // block by the tokens l between (own[l]), the others by rows (rows[i]) and by columns (cols[block of i][j])
+        float rows[2] = {}, m = 1.0f;
 #pragma unroll 1
-        for (int jb = 0; jb <= rb; ++jb) {
+        for (int jb = rb; jb >= 0; --jb) {
             float A[2][4] = {}, M[2][4] = {}, qk[2][4] = {}, kk[2][4] = {};
-#pragma unroll 1
+#pragma unroll 2
             for (int v = 0; v < tv; ++v) {
-                const typename P::B1 fr = P::n_rows(Rb, vp, jb * 16, v * 16, lane);
-                P::mul(A[0], A[1], P::a_rows(Ob, vp, rb * 16, v * 16, lane), fr);
-                P::mul(M[0], M[1], P::a_rows(Vb, vp, rb * 16, v * 16, lane), fr);
+                const typename P::B1 fr = P::n_rows(s.R, vp, jb * 16, v * 16, lane);
+                P::mul(A[0], A[1], P::a_rows(s.O, vp, rb * 16, v * 16, lane), fr);
+                P::mul(M[0], M[1], P::a_rows(s.V, vp, rb * 16, v * 16, lane), fr);
             }
+            if (part == 0)
 #pragma unroll
-            for (int c = 0; c < KP / 16; ++c) {
-                const typename P::B1 fj = P::n_rows(Kb, L::pitch, jb * 16, c * 16, lane);
-                P::mul(qk[0], qk[1], P::a_rows(Q, L::pitch, rb * 16, c * 16, lane), fj);
-                P::mul(kk[0], kk[1], P::a_rows(Kb, L::pitch, rb * 16, c * 16, lane), fj);
+                for (int c = 0; c < KP / 16; ++c) {
+                    const typename P::B1 fj = P::n_rows(s.K, L::pitch, jb * 16, c * 16, lane);
+                    P::mul(qk[0], qk[1], P::a_rows(s.Q, L::pitch, rb * 16, c * 16, lane), fj);
+                    P::mul(kk[0], kk[1], P::a_rows(s.K, L::pitch, rb * 16, c * 16, lane), fj);
+                }
+            if (jb == rb) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float hi = x.hi[i0 + 8 * r], lo = x.lo[i0 + 8 * r];
+                    const int since = x.since[i0 + 8 * r];
+                    float upto = 0.0f;  // the sum over the columns before
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        float pair[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int col = nt * 8 + 2 * t + e, jj = rb * 16 + col;
+                            const bool seen = col <= g + 8 * r && x.since[jj] == since, past = seen && col < g + 8 * r;
+                            const float D = seen ? exp2f((hi - x.hi[jj]) + (lo - x.lo[jj])) * x.b[jj] : 0.0f;
+                            float &y = A[nt][2 * r + e], &z = M[nt][2 * r + e];
+                            y = seen ? d.scale * D * y : 0.0f;
+                            z = past ? -D * z : 0.0f;
+                            pair[e] = past ? y * qk[nt][2 * r + e] + z * kk[nt][2 * r + e] : 0.0f;
+                        }
+                        float incl = pair[0] + pair[1], y = __shfl_up_sync(~0u, incl, 1, 4);
+                        if (t >= 1) incl += y;
+                        y = __shfl_up_sync(~0u, incl, 2, 4);
+                        if (t >= 2) incl += y;
+                        const float excl = __shfl_up_sync(~0u, incl, 1, 4), before = upto + (t ? excl : 0.0f);
+                        // tokens l = these columns, up to the row: pairs over the columns before l
+                        qk[nt][2 * r] = nt * 8 + 2 * t <= g + 8 * r ? before : 0.0f;
+                        qk[nt][2 * r + 1] = nt * 8 + 2 * t < g + 8 * r ? before + pair[0] : 0.0f;
+                        upto += __shfl_sync(~0u, incl, 3, 4);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float y = qk[nt][e] + qk[nt][2 + e];
+                        for (int i = 4; i < 32; i *= 2) y += __shfl_xor_sync(~0u, y, i);
+                        if (part == 0 && g == 0) x.own[rb * 16 + nt * 8 + 2 * t + e] = y;
+                    }
+            } else {
+                const float f0 = a_i[0] * m, f1 = a_i[1] * m;
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int jj = jb * 16 + nt * 8 + 2 * t + e;
+                        const float fc = x.d[jj] * x.b[jj], fs = fc * d.scale;
+                        float &y0 = A[nt][e], &y1 = A[nt][2 + e], &z0 = M[nt][e], &z1 = M[nt][2 + e];
+                        y0 *= f0 * fs, y1 *= f1 * fs, z0 *= -f0 * fc, z1 *= -f1 * fc;
+                        const float p0 = y0 * qk[nt][e] + z0 * kk[nt][e], p1 = y1 * qk[nt][2 + e] + z1 * kk[nt][2 + e];
+                        rows[0] += p0, rows[1] += p1;
+                        float y = p0 + p1;
+                        for (int i = 4; i < 32; i *= 2) y += __shfl_xor_sync(~0u, y, i);
+                        if (part == 0 && g == 0) x.cols[rb][jj] = y;
+                    }
+                m *= x.through[jb];
             }
-            float pair[2][4];
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int jj = jb * 16 + nt * 8 + 2 * t + (e & 1), r = e >> 1, i = i0 + 8 * r;
-                    const bool seen = jj <= i && x.since[jj] == since_i[r];
-                    const float D = seen ? expf((hi_i[r] - x.hi[jj]) + (lo_i[r] - x.lo[jj])) * x.b[jj] : 0.0f;
-                    A[nt][e] = seen ? d.scale * D * A[nt][e] : 0.0f;
-                    M[nt][e] = seen && jj < i ? -D * M[nt][e] : 0.0f;
-                    pair[nt][e] = seen && jj < i ? A[nt][e] * qk[nt][e] + M[nt][e] * kk[nt][e] : 0.0f;
-                }
-            // pairs[l] = sum over rows i >= l of the sums over columns j < l
-            float upto[2][2][2];  // [row][tile][column]
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                float base = before[r];
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    const float p0 = pair[nt][2 * r], p1 = pair[nt][2 * r + 1];
-                    float incl = p0 + p1;
-                    float y = __shfl_up_sync(~0u, incl, 1, 4);
-                    if (t >= 1) incl += y;
-                    y = __shfl_up_sync(~0u, incl, 2, 4);
-                    if (t >= 2) incl += y;
-                    float excl = __shfl_up_sync(~0u, incl, 1, 4);
-                    excl = t ? excl : 0.0f;
-                    upto[r][nt][0] = base + excl, upto[r][nt][1] = base + excl + p0;
-                    base += __shfl_sync(~0u, incl, 3, 4);
-                }
-                before[r] = base;
-            }
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int l = jb * 16 + nt * 8 + 2 * t + e;
-                    float y = (l <= i0 ? upto[0][nt][e] : 0.0f) + (l <= i0 + 8 ? upto[1][nt][e] : 0.0f);
-                    for (int o = 4; o < 32; o *= 2) y += __shfl_xor_sync(~0u, y, o);
-                    if (part == 0 && g == 0) x.pairs[rb][l] = y;
-                }
             const typename P::A1 fa = P::rounded(A[0], A[1]), fm = P::rounded(M[0], M[1]);
+            if constexpr (L::store)
+                if (part == 0) put_block(s.A + L::block(rb, jb), fa, lane), put_block(s.M + L::block(rb, jb), fm, lane);
 #pragma unroll
             for (int c = 0; c < KH / 16; ++c) {
-                const typename P::B1 fk = P::k_rows(Kb, L::pitch, jb * 16, k0 + c * 16, lane);
+                const typename P::B1 fk = P::k_rows(s.K, L::pitch, jb * 16, k0 + c * 16, lane);
                 P::mul(dq[2 * c], dq[2 * c + 1], fa, fk);
                 P::mul(dk[2 * c], dk[2 * c + 1], fm, fk);
             }
         }
-        // the warp's tokens as j, those after them as i
-        const float b_j[2] = {x.b[i0], x.b[i0 + 8]};
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            for (int i = 1; i < 4; i *= 2) sum[r] += __shfl_xor_sync(~0u, sum[r], i), rows[r] += __shfl_xor_sync(~0u, rows[r], i);
+            if (t == 0) x.row[part][i0 + 8 * r] = sum[r];
+            if (t == 0 && part == 0) x.rows[i0 + 8 * r] = rows[r];
+        }
+        __syncthreads();
+        for (int i = tid; i < tv * (KP / 16) * 32; i += threads)
+            put_state(s.S, L::pitch, i / 32 / (KP / 16), i / 32 % (KP / 16), f.kept_ds, kept + i, i % 32);
+        // the tokens as j: A and M over the tokens from them on
+        m = 1.0f;
 #pragma unroll 1
         for (int ib = rb; ib < RB; ++ib) {
-            float A[2][4] = {}, M[2][4] = {};
-#pragma unroll 1
-            for (int v = 0; v < tv; ++v) {
-                const typename P::A1 fr = P::a_rows(Rb, vp, rb * 16, v * 16, lane);
-                P::mul(A[0], A[1], fr, P::n_rows(Ob, vp, ib * 16, v * 16, lane));
-                P::mul(M[0], M[1], fr, P::n_rows(Vb, vp, ib * 16, v * 16, lane));
-            }
-#pragma unroll
-            for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int i = ib * 16 + nt * 8 + 2 * t + (e & 1), r = e >> 1, jj = i0 + 8 * r;
-                    const bool seen = jj <= i && x.since[i] == since_i[r];
-                    const float D = seen ? expf((x.hi[i] - hi_i[r]) + (x.lo[i] - lo_i[r])) * b_j[r] : 0.0f;
-                    A[nt][e] = seen ? d.scale * D * A[nt][e] : 0.0f;
-                    M[nt][e] = seen && jj < i ? -D * M[nt][e] : 0.0f;
+            typename P::A1 fa, fm;
+            if constexpr (L::store) {
+                fa = P::a_cols(s.A + L::block(ib, rb), 24, 0, 0, lane), fm = P::a_cols(s.M + L::block(ib, rb), 24, 0, 0, lane);
+            } else {
+                float A[2][4] = {}, M[2][4] = {};
+#pragma unroll 2
+                for (int v = 0; v < tv; ++v) {
+                    const typename P::A1 fr = P::a_rows(s.R, vp, rb * 16, v * 16, lane);
+                    P::mul(A[0], A[1], fr, P::n_rows(s.O, vp, ib * 16, v * 16, lane));
+                    P::mul(M[0], M[1], fr, P::n_rows(s.V, vp, ib * 16, v * 16, lane));
                 }
-            const typename P::A1 fa = P::rounded(A[0], A[1]), fm = P::rounded(M[0], M[1]);
+                if (ib == rb) {
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = e >> 1, jj = i0 + 8 * r, i = ib * 16 + nt * 8 + 2 * t + (e & 1);
+                            const bool seen = jj <= i && x.since[i] == x.since[jj];
+                            const float D = seen ? exp2f((x.hi[i] - x.hi[jj]) + (x.lo[i] - x.lo[jj])) * b_i[r] : 0.0f;
+                            A[nt][e] = seen ? d.scale * D * A[nt][e] : 0.0f;
+                            M[nt][e] = seen && jj < i ? -D * M[nt][e] : 0.0f;
+                        }
+                } else {
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float D = x.a[ib * 16 + nt * 8 + 2 * t + (e & 1)] * m * (d_i[e >> 1] * b_i[e >> 1]);
+                            A[nt][e] *= d.scale * D, M[nt][e] *= -D;
+                        }
+                    m *= x.through[ib];
+                }
+                fa = P::rounded(A[0], A[1]), fm = P::rounded(M[0], M[1]);
+            }
 #pragma unroll
             for (int c = 0; c < KH / 16; ++c) {
-                P::mul(dk[2 * c], dk[2 * c + 1], fa, P::k_rows(Q, L::pitch, ib * 16, k0 + c * 16, lane));
-                P::mul(dk[2 * c], dk[2 * c + 1], fm, P::k_rows(Kb, L::pitch, ib * 16, k0 + c * 16, lane));
+                P::mul(dk[2 * c], dk[2 * c + 1], fa, P::k_rows(s.Q, L::pitch, ib * 16, k0 + c * 16, lane));
+                P::mul(dk[2 * c], dk[2 * c + 1], fm, P::k_rows(s.K, L::pitch, ib * 16, k0 + c * 16, lane));
             }
         }
-        // what the tokens leave in the last state
         __syncthreads();
-        for (int i = tid; i < tv * (KP / 16) * 32; i += threads) {
-            float ds[8];
-            kept_values<E>(ds, f.kept_ds, kept + i);
-            put_state<E>(St, L::pitch, i / 32 / (KP / 16), i / 32 % (KP / 16), ds, i % 32);
-        }
-        __syncthreads();
+        // what they leave in the last state
         {
             float acc[KH / 8][4] = {};
 #pragma unroll 1
             for (int v = 0; v < tv; ++v) {
-                const typename P::A1 fa = P::a_rows(Rb, vp, rb * 16, v * 16, lane);
+                const typename P::A1 fa = P::a_rows(s.R, vp, rb * 16, v * 16, lane);
 #pragma unroll
                 for (int c = 0; c < KH / 16; ++c)
-                    P::mul(acc[2 * c], acc[2 * c + 1], fa, P::k_rows(St, L::pitch, v * 16, k0 + c * 16, lane));
+                    P::mul(acc[2 * c], acc[2 * c + 1], fa, P::k_rows(s.S, L::pitch, v * 16, k0 + c * 16, lane));
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float dd = x.d[i0 + 8 * r], scaled = dd * b_j[r];
-                const E *p = Kb + (i0 + 8 * r) * L::pitch + k0 + 2 * t;
-                float sum = 0.0f;
+                const float scaled = d_i[r] * from * b_i[r];
+                const E *p = s.K + (i0 + 8 * r) * L::pitch + k0 + 2 * t;
+                float y = 0.0f;
 #pragma unroll
                 for (int c = 0; c < KH / 8; ++c) {
-                    const float y0 = dd == 0.0f ? 0.0f : scaled * acc[c][2 * r], y1 = dd == 0.0f ? 0.0f : scaled * acc[c][2 * r + 1];
-                    sum += to_float(p[8 * c]) * y0 + to_float(p[8 * c + 1]) * y1;
+                    const float y0 = scaled * acc[c][2 * r], y1 = scaled * acc[c][2 * r + 1];
+                    const float2 z = pair_at(p + 8 * c);
+                    y += z.x * y0 + z.y * y1;
                     dk[c][2 * r] += y0, dk[c][2 * r + 1] += y1;
                 }
-                sum += __shfl_xor_sync(~0u, sum, 1);
-                sum += __shfl_xor_sync(~0u, sum, 2);
-                if (t == 0) x.col[part][i0 + 8 * r] = sum;
+                y += __shfl_xor_sync(~0u, y, 1);
+                y += __shfl_xor_sync(~0u, y, 2);
+                if (t == 0) x.col[part][i0 + 8 * r] = y;
             }
         }
         __syncthreads();
-        if (w == 0) {
-            constexpr int PL = C / 32;
-            float rows[PL], before_l[PL], row_all = 0.0f, col_all = 0.0f;
+        if (w == 0) {  // dg, PL neighbouring tokens a lane
+            float reads[PL], leaves[PL], own[PL], behind[PL];
+            float read_sum = 0.0f, leave_sum = 0.0f, own_sum = 0.0f, behind_sum = 0.0f, middle[RB] = {};
+            const int lb = lane * PL / 16;
 #pragma unroll
             for (int e = 0; e < PL; ++e) {
                 const int l = lane * PL + e;
-                before_l[e] = col_all;
-                float rs = 0.0f, cs = 0.0f;
-                for (int i = 0; i < KP / KH; ++i) rs += x.row[i][l], cs += x.col[i][l];
-                rows[e] = rs, row_all += rs, col_all += cs;
+                reads[e] = x.row[0][l], leaves[e] = x.col[0][l], own[e] = x.rows[l], behind[e] = 0.0f;
+                for (int i = 1; i < KP / KH; ++i) reads[e] += x.row[i][l], leaves[e] += x.col[i][l];
+#pragma unroll
+                for (int i = 1; i < RB; ++i) {
+                    const float y = i > lb ? x.cols[i][l] : 0.0f;
+                    behind[e] += y;
+#pragma unroll
+                    for (int b = 1; b < i; ++b) middle[b] += lb < b ? y : 0.0f;  // pairs that pass over the whole block b
+                }
+                read_sum += reads[e], leave_sum += leaves[e], own_sum += own[e], behind_sum += behind[e];
             }
-            float after = row_all, ahead = col_all;  // of this lane on; up to this lane
+            float read_all = read_sum, leave_all = leave_sum, own_all = own_sum, behind_all = behind_sum;
+            constexpr int LB = 16 / PL;  // lanes of a block
 #pragma unroll
             for (int i = 1; i < 32; i *= 2) {
-                const float y = __shfl_down_sync(~0u, after, i), z = __shfl_up_sync(~0u, ahead, i);
-                if (lane + i < 32) after += y;
-                if (lane >= i) ahead += z;
+                float y = __shfl_down_sync(~0u, read_all, i);
+                if (lane + i < 32) read_all += y;
+                y = __shfl_up_sync(~0u, leave_all, i);
+                if (lane >= i) leave_all += y;
+                if (i < LB) {
+                    y = __shfl_down_sync(~0u, own_all, i, LB);
+                    if (lane % LB + i < LB) own_all += y;
+                    y = __shfl_up_sync(~0u, behind_all, i, LB);
+                    if (lane % LB >= i) behind_all += y;
+                }
+#pragma unroll
+                for (int b = 1; b < RB - 1; ++b) middle[b] += __shfl_xor_sync(~0u, middle[b], i);
             }
-            after = __shfl_down_sync(~0u, after, 1);  // of the lanes behind
-            if (lane == 31) after = 0.0f;
-            ahead = __shfl_up_sync(~0u, ahead, 1);
-            if (lane == 0) ahead = 0.0f;
-            float through = 0.0f;
+            float through = 0.0f, y;
             for (int i = 0; i < L::warps; ++i) through += x.end[i];
-            through = x.a_end == 0.0f ? 0.0f : x.a_end * through;
-            float suffix = after;
+            for (int i = 0; i < RB; ++i) through *= x.through[i];
+            // of the lanes behind (reads; own pairs' rows in the block), and of the lanes before (leaves; columns in the block)
+            y = __shfl_down_sync(~0u, read_all, 1), read_sum = lane < 31 ? y : 0.0f;
+            y = __shfl_up_sync(~0u, leave_all, 1), leave_sum = lane ? y : 0.0f;
+            y = __shfl_down_sync(~0u, own_all, 1, LB), own_sum = lane % LB < LB - 1 ? y : 0.0f;
+            y = __shfl_up_sync(~0u, behind_all, 1, LB), behind_sum = lane % LB ? y : 0.0f;
+#pragma unroll
+            for (int b = 1; b < RB - 1; ++b)
+                if (b == lb) through += middle[b];
+            float mine[PL];
+#pragma unroll
+            for (int e = 0; e < PL; ++e) {
+                mine[e] = through + leave_sum + behind_sum + x.own[lane * PL + e];
+                leave_sum += leaves[e], behind_sum += behind[e];
+            }
 #pragma unroll
             for (int e = PL - 1; e >= 0; --e) {
                 const int l = lane * PL + e;
-                suffix += rows[e];
-                float y = through + suffix + (ahead + before_l[e]);
-                for (int i = l / 16; i < RB; ++i) y += x.pairs[i][l];
-                const bool is_fresh = x.since[l] != (l ? x.since[l - 1] : 0);
-                if (l < left) *row<T>(f.gr.dg, f.gr.dg_stride, n, at + l, h) = from_float<T>(is_fresh ? 0.0f : y);
+                read_sum += reads[e], own_sum += own[e];
+                const bool fresh = x.since[l] != (l % 16 ? x.since[l - 1] : 0);
+                if (l < left)
+                    *row<T>(f.gr.dg, f.gr.dg_stride, n, at + l, h) = from_float<T>(fresh ? 0.0f : mine[e] + read_sum + own_sum);
             }
         }
     }
 #pragma unroll
-    for (int c = 0; c < KH / 8; ++c)
+    for (int r = 0; r < 2; ++r) {
+        if (i0 + 8 * r >= left) continue;
+        T *q = row<T>(f.gr.dq, f.gr.dq_stride, n, at + i0 + 8 * r, hk) + k0 + 2 * t;
+        T *k = row<T>(f.gr.dk, f.gr.dk_stride, n, at + i0 + 8 * r, hk) + k0 + 2 * t;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = rb * 16 + g + (e >> 1) * 8, k = k0 + c * 8 + 2 * t + (e & 1);
-            if (i >= left || k >= K) continue;
-            row<T>(f.gr.dq, f.gr.dq_stride, n, at + i, hk)[k] = from_float<T>(dq[c][e]);
-            row<T>(f.gr.dk, f.gr.dk_stride, n, at + i, hk)[k] = from_float<T>(dk[c][e]);
+        for (int c = 0; c < KH / 8; ++c) {
+            const int left_k = K - (k0 + c * 8 + 2 * t);
+            if (left_k >= 2 && f.wide_dqk) {
+                store_pair(q + 8 * c, dq[c][2 * r], dq[c][2 * r + 1]), store_pair(k + 8 * c, dk[c][2 * r], dk[c][2 * r + 1]);
+            } else {
+                if (left_k >= 1) q[8 * c] = from_float<T>(dq[c][2 * r]), k[8 * c] = from_float<T>(dk[c][2 * r]);
+                if (left_k >= 2) q[8 * c + 1] = from_float<T>(dq[c][2 * r + 1]), k[8 * c + 1] = from_float<T>(dk[c][2 * r + 1]);
+            }
         }
+    }
 }
 
 template <class T, class P, int KP, int MT>
@@ -601,6 +646,8 @@ cudaError_t backward_typed(const goib2d_delta_desc &d, const goib2d_delta_grads 
     f.wide_do = rows_aligned(gr.dout, gr.dout_stride, d.n_worlds, d.n_steps, d.heads, V, z);
     f.wide_dv = rows_aligned(f.dv, f.dv_stride, d.n_worlds, d.n_steps, d.heads, V, sizeof(typename P::E));
     f.wide_r = V % 8 == 0;
+    f.wide_dqk = (uintptr_t)gr.dq % (2 * z) == 0 && (uintptr_t)gr.dk % (2 * z) == 0;
+    for (int i = 0; i < 3; ++i) f.wide_dqk = f.wide_dqk && gr.dq_stride[i] % 2 == 0 && gr.dk_stride[i] % 2 == 0;
     switch (padded_keys(d.key_dim)) {
         case 16: return backward_of<T, P, 16>(f, s);
         case 32: return backward_of<T, P, 32>(f, s);

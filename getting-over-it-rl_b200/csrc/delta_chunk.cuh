@@ -61,9 +61,11 @@ template <class P>
 struct alignas(16) Chunk {
     Square<P> z, p;
     float wt[kChunk][20];   // the strictly lower matrix, transposed
-    float a[kChunk], d[kChunk], b[kChunk];
+    float a[kChunk], sa[kChunk], d[kChunk], b[kChunk], bd[kChunk];  // sa = scale a, bd = b d
+    float hi[kChunk], lo[kChunk];  // hi + lo: G / ln 2
     int since[kChunk];      // tokens of the chunk up to this one that start afresh
     float a_end;
+    int odd;                // whether a write strength is not finite
 };
 
 // A token's gates, held by lanes i and i + 16 of the warp that prepares the chunk.
@@ -82,27 +84,34 @@ __device__ __forceinline__ Gate load_gate(const goib2d_delta_desc &d, int64_t n,
     return r;
 }
 
-// A warp prepares one chunk from its 16 rows of Q and K. BACK: (I + diag(b) W)^-1, else (I + W diag(b))^-1.
+// The running sums of 16 tokens' g / ln 2, in float64: differences of sums over a chunk of strong decays keep
+// float32's precision. Lanes i and i + 16 hold token i.
+__device__ __forceinline__ double running_sum(const Gate &gate, int lane) {
+    double G = gate.fresh ? 0.0 : (double)gate.g * 1.4426950408889634;
+#pragma unroll
+    for (int o = 1; o < 16; o *= 2) {
+        const double y = __shfl_up_sync(~0u, G, o, 16);
+        if ((lane & 15) >= o) G += y;
+    }
+    return G;
+}
+
+// A warp prepares one chunk from its 16 rows of Q and K. Forwards Z = (I + W diag(b))^-1 and P diag(b); BACK: T =
+// (I + diag(b) W)^-1 and P.
 template <class P, int KP, bool BACK>
 __device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, const typename P::E *K, int pitch, Gate gate,
                                         float scale, int lane) {
     const int i = lane & 15, g = lane >> 2, t = lane & 3;
-    // G in float64: differences of sums over a chunk of strong decays keep float32's precision
-    double G = gate.fresh ? 0.0 : (double)gate.g;
-#pragma unroll
-    for (int o = 1; o < kChunk; o *= 2) {
-        const double y = __shfl_up_sync(~0u, G, o, 16);
-        if (i >= o) G += y;
-    }
+    const double G = running_sum(gate, lane), end = __shfl_sync(~0u, G, 15);
     const uint32_t fresh = __ballot_sync(~0u, gate.fresh) & 0xffffu;
     const int since = __popc(fresh & ((2u << i) - 1)), all = __popc(fresh);
-    const double end = __shfl_sync(~0u, G, 15);
+    const int odd = __any_sync(~0u, 0.0f * gate.b != 0.0f);
     if (lane < 16) {
-        c.a[i] = since ? 0.0f : expf((float)G);
-        c.d[i] = since == all ? expf((float)(end - G)) : 0.0f;
-        c.b[i] = gate.b;
+        const float a = since ? 0.0f : exp2f((float)G), d = since == all ? exp2f((float)(end - G)) : 0.0f;
+        c.a[i] = a, c.sa[i] = scale * a, c.d[i] = d, c.b[i] = gate.b, c.bd[i] = gate.b * d;
+        c.hi[i] = (float)G, c.lo[i] = (float)(G - (double)(float)G);
         c.since[i] = since;
-        if (lane == 0) c.a_end = all ? 0.0f : expf((float)end);
+        if (lane == 0) c.a_end = all ? 0.0f : exp2f((float)end), c.odd = odd;
     }
     float kk[2][4] = {}, qk[2][4] = {};
 #pragma unroll
@@ -111,24 +120,23 @@ __device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, con
         P::mul(kk[0], kk[1], P::a_rows(K, pitch, 0, x, lane), kb);
         P::mul(qk[0], qk[1], P::a_rows(Q, pitch, 0, x, lane), kb);
     }
+    __syncwarp();
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
         const int row = g + 8 * r;
-        const double Gi = __shfl_sync(~0u, G, row);
-        const int si = __popc(fresh & ((2u << row) - 1));
-        const float bi = __shfl_sync(~0u, gate.b, row);
+        const float hi = c.hi[row], lo = c.lo[row], bi = c.b[row];
+        const int si = c.since[row];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             float p[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = n * 8 + 2 * t + e;
-                const double Gj = __shfl_sync(~0u, G, col);
-                const float bj = __shfl_sync(~0u, gate.b, col);
-                const bool seen = col <= row && __popc(fresh & ((2u << col) - 1)) == si;
-                const float D = seen ? expf((float)(Gi - Gj)) : 0.0f;
+                const float bj = c.b[col];
+                const bool seen = col <= row && c.since[col] == si;
+                const float D = seen ? exp2f((hi - c.hi[col]) + (lo - c.lo[col])) : 0.0f;
                 c.wt[col][row] = seen && col < row ? D * kk[n][2 * r + e] * (BACK ? bi : bj) : 0.0f;
-                p[e] = seen ? scale * D * qk[n][2 * r + e] : 0.0f;
+                p[e] = seen ? scale * D * qk[n][2 * r + e] * (BACK ? 1.0f : bj) : 0.0f;
             }
             c.p.put(row, n * 8 + 2 * t, p[0], p[1]);
         }
@@ -161,31 +169,79 @@ __device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, con
 }
 
 // Rows of a strided tensor into shared memory, zeros past `rows` and `cols`. Aligned rows of the same type come by
-// asynchronous copies.
+// asynchronous copies, eight neighbouring threads to a row.
 template <class E, class T>
 __device__ __forceinline__ void load_rows(E *to, int pitch, const T *from, int64_t stride, int rows, int count, int cols,
                                           int padded, bool wide, int tid, int threads) {
     if constexpr (sizeof(T) == sizeof(E)) {
         if (wide) {
             constexpr int N = 16 / sizeof(E);
-            const int per = padded / N;
-            for (int x = tid; x < count * per; x += threads) {
-                const int r = x / per, c = (x - r * per) * N;
-                E *p = to + r * pitch + c;
-                if (r < rows && c < cols) cp_async16(p, from + r * stride + c);
-                else *(uint4 *)p = make_uint4(0, 0, 0, 0);
-            }
+            for (int c = tid % 8 * N; c < padded; c += 8 * N)
+                for (int r = tid / 8; r < count; r += threads / 8) {
+                    E *p = to + r * pitch + c;
+                    if (r < rows && c < cols) cp_async16(p, from + r * stride + c);
+                    else *(uint4 *)p = make_uint4(0, 0, 0, 0);
+                }
             return;
         }
     }
-    const int per = padded / 2;
-    for (int x = tid; x < count * per; x += threads) {
-        const int r = x / per, c = (x - r * per) * 2;
-        const T *p = from + (int64_t)r * stride + c;
-        const float u = r < rows && c < cols ? to_float(p[0]) : 0.0f, v = r < rows && c + 1 < cols ? to_float(p[1]) : 0.0f;
-        if constexpr (sizeof(E) == 2) *(uint32_t *)(to + r * pitch + c) = pack(u, v);
-        else *(float2 *)(to + r * pitch + c) = make_float2(u, v);
+    for (int c = tid % 8 * 2; c < padded; c += 16)
+        for (int r = tid / 8; r < count; r += threads / 8) {
+            const T *p = from + r * stride + c;
+            const float u = r < rows && c < cols ? to_float(p[0]) : 0.0f, v = r < rows && c + 1 < cols ? to_float(p[1]) : 0.0f;
+            if constexpr (sizeof(E) == 2) *(uint32_t *)(to + r * pitch + c) = pack(u, v);
+            else *(float2 *)(to + r * pitch + c) = make_float2(u, v);
+        }
+}
+
+// A warp's MT * 16 columns of a state [K][V] as accumulators of S^T (rows v, columns k), and back.
+template <int MT, int KP>
+__device__ __forceinline__ void load_state(float (&S)[MT][KP / 8][4], const float *from, int K, int V, int v0, int lane) {
+    const int k0 = (lane & 3) * 2, v1 = v0 + (lane >> 2);
+    if (from && K == KP && v0 + 16 * MT <= V) {
+        const float *p = from + k0 * V + v1, *q = p + V;
+#pragma unroll
+        for (int j = 0; j < KP / 8; ++j, p += 8 * V, q += 8 * V)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                S[m][j][0] = p[16 * m], S[m][j][1] = q[16 * m];
+                S[m][j][2] = p[16 * m + 8], S[m][j][3] = q[16 * m + 8];
+            }
+        return;
     }
+#pragma unroll
+    for (int j = 0; j < KP / 8; ++j)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = 8 * j + k0 + (e & 1), v = v1 + 16 * m + (e >> 1) * 8;
+                S[m][j][e] = from && k < K && v < V ? from[k * V + v] : 0.0f;
+            }
+}
+template <int MT, int KP>
+__device__ __forceinline__ void store_state(float *to, const float (&S)[MT][KP / 8][4], int K, int V, int v0, int lane) {
+    const int k0 = (lane & 3) * 2, v1 = v0 + (lane >> 2);
+    if (K == KP && v0 + 16 * MT <= V) {
+        float *p = to + k0 * V + v1, *q = p + V;
+#pragma unroll
+        for (int j = 0; j < KP / 8; ++j, p += 8 * V, q += 8 * V)
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                p[16 * m] = S[m][j][0], q[16 * m] = S[m][j][1];
+                p[16 * m + 8] = S[m][j][2], q[16 * m + 8] = S[m][j][3];
+            }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < KP / 8; ++j)
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int k = 8 * j + k0 + (e & 1), v = v1 + 16 * m + (e >> 1) * 8;
+                if (k < K && v < V) to[k * V + v] = S[m][j][e];
+            }
 }
 
 // 16 x 16 values (rows v, columns tokens) of one accumulator pair, to the rows of a strided tensor; tokens: a bit each
@@ -251,16 +307,25 @@ __device__ __forceinline__ void kept_values(float (&v)[8], const void *kept, int
         *(float4 *)v = ((const float4 *)kept)[2 * x], *(float4 *)(v + 4) = ((const float4 *)kept)[2 * x + 1];
     }
 }
-// The 8 values of a thread into rows of S^T in shared memory.
-template <class E>
-__device__ __forceinline__ void put_state(E *St, int pitch, int tile_v, int tile_k, const float (&v)[8], int lane) {
-    E *p = St + (tile_v * 16 + (lane >> 2)) * pitch + tile_k * 16 + 2 * (lane & 3);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        E *q = p + (e & 1) * 8 * pitch + (e >> 1) * 8;
-        if constexpr (sizeof(E) == 2) *(uint32_t *)q = pack(v[2 * e], v[2 * e + 1]);
-        else *(float2 *)q = make_float2(v[2 * e], v[2 * e + 1]);
-    }
+// A thread's 8 kept values into rows of S^T in shared memory.
+__device__ __forceinline__ void put_state(bf16 *St, int pitch, int tile_v, int tile_k, const void *kept, int64_t x, int lane) {
+    const uint4 y = ((const uint4 *)kept)[x];
+    bf16 *p = St + (tile_v * 16 + (lane >> 2)) * pitch + tile_k * 16 + 2 * (lane & 3);
+    *(uint32_t *)p = y.x, *(uint32_t *)(p + 8 * pitch) = y.y;
+    *(uint32_t *)(p + 8) = y.z, *(uint32_t *)(p + 8 * pitch + 8) = y.w;
 }
+__device__ __forceinline__ void put_state(float *St, int pitch, int tile_v, int tile_k, const void *kept, int64_t x, int lane) {
+    const float4 y = ((const float4 *)kept)[2 * x], z = ((const float4 *)kept)[2 * x + 1];
+    float *p = St + (tile_v * 16 + (lane >> 2)) * pitch + tile_k * 16 + 2 * (lane & 3);
+    *(float2 *)p = make_float2(y.x, y.y), *(float2 *)(p + 8 * pitch) = make_float2(y.z, y.w);
+    *(float2 *)(p + 8) = make_float2(z.x, z.y), *(float2 *)(p + 8 * pitch + 8) = make_float2(z.z, z.w);
+}
+
+// Two neighbouring values.
+__device__ __forceinline__ float2 pair_at(const bf16 *p) {
+    const uint32_t x = *(const uint32_t *)p;
+    return make_float2(low(x), high(x));
+}
+__device__ __forceinline__ float2 pair_at(const float *p) { return *(const float2 *)p; }
 
 }  // namespace gb

@@ -27,8 +27,44 @@ struct Layout {
     __host__ __device__ static int bytes(int warps) { return 2 * stage(warps) + kTile / kChunk * (int)sizeof(Chunk<P>); }
 };
 
+// A chunk that holds infinities or NaN, token by token: within the products a token meets every other one, if only as 0
+// times it, which these values pass. S: the warp's accumulators, in memory.
 template <class T, class P, int KP, int MT>
-__global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_forward_kernel(const __grid_constant__ Forward f) {
+__device__ __noinline__ void odd_chunk(const Forward &f, float *S, const typename P::E *Q, const typename P::E *K,
+                                       const typename P::E *V, int vp, int64_t n, int h, int64_t at, int v0, int lane) {
+    const goib2d_delta_desc &d = f.d;
+    const int g = lane >> 2, t = lane & 3, tokens = (int)(d.n_steps - at < kChunk ? d.n_steps - at : kChunk);
+    for (int i = 0; i < tokens; ++i) {
+        const Gate gate = load_gate<T>(d, n, at + i, h);
+        const float a = gate.fresh ? 0.0f : expf(gate.g);
+        for (int m = 0; m < 2 * MT; ++m) {  // the thread's rows
+            float *s = S + (m >> 1) * (KP / 8) * 4 + (m & 1) * 2;
+            const int v = v0 + 16 * (m >> 1) + 8 * (m & 1) + g;
+            float sk = 0.0f, sq = 0.0f, kq = 0.0f;
+            for (int j = 0; j < KP / 8; ++j)
+                for (int e = 0; e < 2; ++e) {
+                    float &x = s[4 * j + e];
+                    const float k = to_float(K[i * (KP + 8) + 8 * j + 2 * t + e]), q = to_float(Q[i * (KP + 8) + 8 * j + 2 * t + e]);
+                    x = gate.fresh ? 0.0f : a * x;
+                    sk += x * k, sq += x * q, kq += k * q;
+                }
+            for (int o = 1; o < 4; o *= 2)
+                sk += __shfl_xor_sync(~0u, sk, o), sq += __shfl_xor_sync(~0u, sq, o), kq += __shfl_xor_sync(~0u, kq, o);
+            const float r = to_float(V[i * vp + v]) - sk, u = gate.b * r;
+            for (int j = 0; j < KP / 8; ++j)
+                for (int e = 0; e < 2; ++e) s[4 * j + e] += to_float(K[i * (KP + 8) + 8 * j + 2 * t + e]) * u;
+            if (t == 0 && v < d.value_dim) {
+                row<T>(d.out, d.out_stride, n, at + i, h)[v] = from_float<T>(d.scale * (sq + kq * u));
+                if (f.r)
+                    ((typename P::E *)f.r)[((n * d.heads + h) * d.n_steps + at + i) * d.value_dim + v] =
+                        from_float<typename P::E>(r);
+            }
+        }
+    }
+}
+
+template <class T, class P, int KP, int MT>
+__global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 : 1) goib2d_delta_forward_kernel(const __grid_constant__ Forward f) {
     using L = Layout<P, KP, MT>;
     using E = typename P::E;
     constexpr int KT = KP / 16;
@@ -36,22 +72,14 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_forward_kern
     extern __shared__ __align__(16) char sm[];
     const goib2d_delta_desc &d = f.d;
     const int K = d.key_dim, V = d.value_dim, threads = blockDim.x, warps = threads / 32;
-    const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, t = lane & 3;
     const int64_t nh = blockIdx.x, n = nh / d.heads, steps = d.n_steps;
     const int h = (int)(nh - n * d.heads), hk = h / (d.heads / d.key_heads);
     const int stage = L::stage(warps), vp = L::v_pitch(warps), v0 = w * 16 * MT;
     Chunk<P> *chunks = (Chunk<P> *)(sm + 2 * stage);
 
     float S[MT][KP / 8][4];  // S^T: rows v, columns k
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < KP / 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = v0 + 16 * m + g + (e >> 1) * 8, k = j * 8 + 2 * t + (e & 1);
-                S[m][j][e] = d.state_in && v < V && k < K ? d.state_in[(nh * K + k) * V + v] : 0.0f;
-            }
+    load_state<MT, KP>(S, d.state_in ? d.state_in + nh * K * V : nullptr, K, V, v0, lane);
 
     const T *q0 = row<T>(d.q, d.q_stride, n, 0, hk), *k0 = row<T>(d.k, d.k_stride, n, 0, hk);
     const T *v_0 = row<T>(d.v, d.v_stride, n, 0, h);
@@ -99,16 +127,7 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_forward_kern
             const Chunk<P> &c = chunks[s];
             const E *Qs = Q + s * kChunk * L::pitch, *Ks = Kb + s * kChunk * L::pitch;
             E *Vs = Vb + s * kChunk * vp;
-            const uint32_t whole = steps - at < kChunk ? (1u << (steps - at)) - 1 : 0xffffu;
-            // All tokens of the chunk at once (only == -1). Within the products a token meets the others as 0 times
-            // them, which infinities and NaN pass; a chunk that holds any is done again token by token, each with
-            // the tokens before it that its state has seen and nothing else.
-            int only = -1;
-        again:
-            auto in = [&](int e) {  // whether the thread's column e (tokens 2 t, 2 t + 1, and 8 on) takes part
-                const int i = (e >> 1) * 8 + 2 * t + (e & 1);
-                return i <= only && c.since[i] == c.since[only];
-            };
+            const uint32_t tokens = steps - at < kChunk ? (1u << (steps - at)) - 1 : 0xffffu;
             float Y[MT][2][4] = {}, O[MT][2][4] = {};
 #pragma unroll
             for (int j = 0; j < KT; ++j) {
@@ -121,7 +140,6 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_forward_kern
                 }
             }
             const typename P::B2 z = c.z.n_rows(lane);
-            const typename P::B1 p = c.p.n_rows1(lane);
             float bad = 0.0f;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
@@ -131,86 +149,68 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_forward_kern
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const float a = c.a[j * 8 + 2 * t + (e & 1)];
-                        x[j][e] -= a == 0.0f ? 0.0f : a * Y[m][j][e];  // nothing of the old state, not even NaN
-                        if (only >= 0 && !in(2 * j + (e & 1))) x[j][e] = 0.0f;
-                        O[m][j][e] = a == 0.0f ? 0.0f : O[m][j][e] * (d.scale * a);
+                        const int i = j * 8 + 2 * t + (e & 1);
+                        x[j][e] -= c.a[i] * Y[m][j][e];
+                        O[m][j][e] *= c.sa[i];
                         Y[m][j][e] = 0.0f;
                     }
                 P::mul(Y[m][0], Y[m][1], P::exact(x[0], x[1]), z);  // r
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) bad += 0.0f * (Y[m][j][e] * c.b[j * 8 + 2 * t + (e & 1)]);
+                    for (int e = 0; e < 4; ++e) bad = fmaf(0.0f, Y[m][j][e], bad);
             }
-            if (only < 0 && __any_sync(~0u, bad != 0.0f)) {
-                only = 0;
-                goto again;
+            if (__any_sync(~0u, c.odd || bad != 0.0f)) {
+                float s[MT * (KP / 8) * 4];
+#pragma unroll
+                for (int i = 0; i < MT * (KP / 8) * 4; ++i) s[i] = S[i / (KP / 2)][i / 4 % (KP / 8)][i % 4];
+                odd_chunk<T, P, KP, MT>(f, s, Qs, Ks, Vs, vp, n, h, at, v0, lane);
+#pragma unroll
+                for (int i = 0; i < MT * (KP / 8) * 4; ++i) S[i / (KP / 2)][i / 4 % (KP / 8)][i % 4] = s[i];
+                continue;
             }
-            const uint32_t tokens = only < 0 ? whole : whole & 1u << only;
             if (f.r) {
                 E *to = (E *)f.r + (nh * steps + at) * V;
-                if (half && only < 0)
+                if (half)
                     store_rows<MT>((bf16 *)to, V, tokens, v0, V, f.wide_r, (bf16 *)Vs, vp, Y, lane);
                 else
 #pragma unroll
                     for (int m = 0; m < MT; ++m) store_direct<E>(to, V, tokens, v0 + 16 * m, V, Y[m], lane);
             }
             typename P::A2 u[MT];
+            {
+                const typename P::B1 p = c.p.n_rows1(lane);
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
+                for (int m = 0; m < MT; ++m) {
+                    P::mul(O[m][0], O[m][1], P::rounded(Y[m][0], Y[m][1]), p);
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        Y[m][j][e] *= c.b[j * 8 + 2 * t + (e & 1)];
-                        if (only >= 0 && !in(2 * j + (e & 1))) Y[m][j][e] = 0.0f;
-                    }
-                P::mul(O[m][0], O[m][1], P::rounded(Y[m][0], Y[m][1]), p);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float dd = c.d[j * 8 + 2 * t + (e & 1)];
-                        Y[m][j][e] = dd == 0.0f ? 0.0f : dd * Y[m][j][e];
-                    }
-                u[m] = P::exact(Y[m][0], Y[m][1]);
+                        for (int e = 0; e < 4; ++e) Y[m][j][e] *= c.bd[j * 8 + 2 * t + (e & 1)];
+                    u[m] = P::exact(Y[m][0], Y[m][1]);
+                }
             }
             T *to = row<T>(d.out, d.out_stride, n, at, h);
-            if (half && only < 0)
+            if (half)
                 store_rows<MT>((bf16 *)to, d.out_stride[1], tokens, v0, V, f.wide_o, (bf16 *)Vs, vp, O, lane);
             else
 #pragma unroll
                 for (int m = 0; m < MT; ++m) store_direct<T>(to, d.out_stride[1], tokens, v0 + 16 * m, V, O[m], lane);
-            if (only >= 0 && only < kChunk - 1) {
-                ++only;
-                goto again;
-            }
             const float a_end = c.a_end;
 #pragma unroll
             for (int j = 0; j < KT; ++j) {
-                typename P::B1 kb = P::k_rows(Ks, L::pitch, 0, 16 * j, lane);
-                if (only >= 0) P::mask_k(kb, in(0) | in(1) << 1 | in(2) << 2 | in(3) << 3);
+                const typename P::B1 kb = P::k_rows(Ks, L::pitch, 0, 16 * j, lane);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
                     float(&c0)[4] = S[m][2 * j], (&c1)[4] = S[m][2 * j + 1];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        c0[e] = a_end == 0.0f ? 0.0f : a_end * c0[e], c1[e] = a_end == 0.0f ? 0.0f : a_end * c1[e];
+                    for (int e = 0; e < 4; ++e) c0[e] *= a_end, c1[e] *= a_end;
                     P::mul(c0, c1, u[m], kb);
                 }
             }
         }
     }
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int j = 0; j < KP / 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int v = v0 + 16 * m + g + (e >> 1) * 8, k = j * 8 + 2 * t + (e & 1);
-                if (v < V && k < K) d.state_out[(nh * K + k) * V + v] = S[m][j][e];
-            }
+    store_state<MT, KP>(d.state_out + nh * K * V, S, K, V, v0, lane);
 }
 
 template <class T, class P, int KP, int MT>

@@ -104,12 +104,6 @@ struct Half {
         ldsm_t(b.x, at_a(p, pitch, row, col, lane));
         return b;
     }
-    // keep the rows k of B whose bit is set: bits 0, 1 for rows 2 t, 2 t + 1, bits 2, 3 for those 8 on
-    static __device__ __forceinline__ void mask_k(B1 &b, int keep) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            b.x[e] &= (keep >> (e & 1) * 2 & 1 ? 0xffffu : 0) | (keep >> (e & 1) * 2 & 2 ? 0xffff0000u : 0);
-    }
     // a 16x16 block in float32 as an accumulator pair's rows and columns: transposed rows of shared memory
     static __device__ __forceinline__ void values_t(float (&c)[2][4], const E *p, int pitch, int row, int col, int lane) {
         uint32_t x[4];
@@ -212,11 +206,6 @@ struct Full {
                 for (int e = 0; e < 2; ++e)
                     part(q[(8 * k + e) * pitch + 8 * n], b.hi[4 * n + 2 * k + e], b.lo[4 * n + 2 * k + e]);
         return b;
-    }
-    static __device__ __forceinline__ void mask_k(B1 &b, int keep) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (!(keep >> (e & 3) & 1)) b.hi[e] = 0, b.lo[e] = 0.0f;
     }
     static __device__ __forceinline__ void values_t(float (&c)[2][4], const E *p, int pitch, int row, int col, int lane) {
         const E *q = p + (row + 2 * (lane & 3)) * pitch + col + (lane >> 2);
