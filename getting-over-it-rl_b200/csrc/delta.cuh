@@ -49,9 +49,8 @@ inline bool delta_full(const goib2d_delta_desc &d) {
     return d.dtype == GOIB2D_FLOAT32 || d.n_worlds * d.n_steps * d.heads <= 4096;
 }
 
-// What goib2d_delta_forward keeps for goib2d_delta_backward: r [n][h][t][V], and S at every keep-th token, its S^T cut
-// into 16 x 16 tiles [n][h][t / keep][V tile][K tile], a tile's values as the 32 threads of a warp hold them in
-// accumulators (8 values a thread). Both in bfloat16, or in float32 (delta_full).
+// What goib2d_delta_forward keeps for goib2d_delta_backward: r [n][h][t][V], and S at every keep-th token, as its S^T
+// [n][h][t / keep][V up to 16s][padded keys]. Both in bfloat16, or in float32 (delta_full).
 struct Saved {
     int64_t r, states, bytes;   // bytes: both
     int32_t keep, tiles_v, tiles_k, size;

@@ -36,17 +36,17 @@ template <class P, int KP, int MT>
 struct Layout {
     static constexpr int pitch = KP + 8, E = sizeof(typename P::E);
     __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (E == 2 ? 8 : 4); }
-    __host__ __device__ static int stage(int warps) { return kTile * (2 * pitch + 2 * v_pitch(warps)) * E; }
     __host__ __device__ static int bytes(int warps) {
-        return 2 * stage(warps) + kTile / kChunk * (int)sizeof(Chunk<P>) + warps * kTile * 4;
+        return kTile<P> * (4 * pitch + 2 * v_pitch(warps)) * E + kTile<P> / kChunk * (int)sizeof(Chunk<P>) +
+               warps * kTile<P> * 4;
     }
 };
 
 template <class T, class P, int KP, int MT>
-__global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_back_state_kernel(const __grid_constant__ Backward f) {
+__global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 : 1) goib2d_delta_back_state_kernel(const __grid_constant__ Backward f) {
     using L = Layout<P, KP, MT>;
     using E = typename P::E;
-    constexpr int KT = KP / 16;
+    constexpr int KT = KP / 16, TILE = kTile<P>;
     constexpr bool half = sizeof(E) == 2;
     extern __shared__ __align__(16) char sm[];
     const goib2d_delta_desc &d = f.d;
@@ -54,66 +54,74 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_back_state_k
     const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
     const int64_t nh = blockIdx.x, n = nh / d.heads, steps = d.n_steps;
     const int h = (int)(nh - n * d.heads), hk = h / (d.heads / d.key_heads);
-    const int stage = L::stage(warps), vp = L::v_pitch(warps), v0 = w * 16 * MT, cols = warps * 16 * MT;
-    Chunk<P> *chunks = (Chunk<P> *)(sm + 2 * stage);
-    float *db = (float *)(chunks + kTile / kChunk);  // [warp][token of the tile]
+    const int vp = L::v_pitch(warps), v0 = w * 16 * MT, cols = warps * 16 * MT;
+    // Q and K twice, the next tile's coming while this one is solved; dO and r once, coming while Z and P are made
+    E *const Q0 = (E *)sm, *const Ob = Q0 + 4 * TILE * L::pitch, *const Rb = Ob + TILE * vp;
+    Chunk<P> *chunks = (Chunk<P> *)(Rb + TILE * vp);
+    float *db = (float *)(chunks + TILE / kChunk);  // [warp][token of the tile]
 
     float S[MT][KP / 8][4];  // dS^T: rows v, columns k
     load_state<MT, KP>(S, f.gr.dstate_out ? f.gr.dstate_out + nh * K * V : nullptr, K, V, v0, lane);
-    const int64_t tiles = (steps + kTile - 1) / kTile;
+    const int64_t tiles = (steps + TILE - 1) / TILE;
     const T *q0 = row<T>(d.q, d.q_stride, n, 0, hk), *k0 = row<T>(d.k, d.k_stride, n, 0, hk);
     const T *o0 = f.gr.dout ? row<T>(f.gr.dout, f.gr.dout_stride, n, 0, h) : nullptr;
     const E *r0 = (const E *)f.r + nh * steps * V;
-    auto load = [&](int64_t tile) {
-        E *Q = (E *)(sm + (tile & 1) * stage), *Kb = Q + kTile * L::pitch, *Ob = Kb + kTile * L::pitch, *Rb = Ob + kTile * vp;
-        const int64_t at = tile * kTile;
-        const int left = (int)(steps - at < kTile ? steps - at : kTile);
-        load_rows(Q, L::pitch, q0 + at * d.q_stride[1], d.q_stride[1], left, kTile, K, KP, f.wide_q, tid, threads);
-        load_rows(Kb, L::pitch, k0 + at * d.k_stride[1], d.k_stride[1], left, kTile, K, KP, f.wide_k, tid, threads);
-        load_rows(Ob, vp, o0 + at * f.gr.dout_stride[1], f.gr.dout_stride[1], o0 ? left : 0, kTile, V, cols, f.wide_do, tid,
-                  threads);
-        load_rows(Rb, vp, r0 + at * V, V, left, kTile, V, cols, f.wide_r, tid, threads);
+    auto load_keys = [&](int64_t tile) {
+        E *Q = Q0 + (tile & 1) * 2 * TILE * L::pitch;
+        const int64_t at = tile * TILE;
+        const int left = (int)(steps - at < TILE ? steps - at : TILE);
+        load_rows(Q, L::pitch, q0 + at * d.q_stride[1], d.q_stride[1], left, TILE, K, KP, f.wide_q, tid, threads);
+        load_rows(Q + TILE * L::pitch, L::pitch, k0 + at * d.k_stride[1], d.k_stride[1], left, TILE, K, KP, f.wide_k, tid, threads);
         cp_commit();
     };
-    Gate gate[kTile / kChunk];
+    auto load_values = [&](int64_t tile) {
+        const int64_t at = tile * TILE;
+        const int left = (int)(steps - at < TILE ? steps - at : TILE);
+        load_rows(Ob, vp, o0 + at * f.gr.dout_stride[1], f.gr.dout_stride[1], o0 ? left : 0, TILE, V, cols, f.wide_do, tid,
+                  threads);
+        load_rows(Rb, vp, r0 + at * V, V, left, TILE, V, cols, f.wide_r, tid, threads);
+        cp_commit();
+    };
+    Gate gate[TILE / kChunk];
     auto gates = [&](int64_t tile) {
 #pragma unroll
-        for (int s = 0; s < kTile / kChunk; ++s)
-            if (s % warps == w) gate[s] = load_gate<T>(d, n, tile * kTile + s * kChunk + (lane & 15), h);
+        for (int s = 0; s < TILE / kChunk; ++s)
+            if ((tile * (TILE / kChunk) + s) % warps == w) gate[s] = load_gate<T>(d, n, tile * TILE + s * kChunk + (lane & 15), h);
     };
     // db of the tile before, from the warps' parts
     auto finish = [&](int64_t tile) {
-        const int64_t at = tile * kTile + tid;
-        if (tid < kTile && at < steps) {
+        const int64_t at = tile * TILE + tid;
+        if (tid < TILE && at < steps) {
             float x = 0.0f;
-            for (int i = 0; i < warps; ++i) x += db[i * kTile + tid];
+            for (int i = 0; i < warps; ++i) x += db[i * TILE + tid];
             *row<T>(f.gr.dbeta, f.gr.dbeta_stride, n, at, h) = from_float<T>(x);
         }
     };
-    if (tiles) load(tiles - 1), gates(tiles - 1);
+    if (tiles) load_keys(tiles - 1), gates(tiles - 1);
     for (int64_t tile = tiles - 1; tile >= 0; --tile) {
-        const E *Q = (const E *)(sm + (tile & 1) * stage), *Kb = Q + kTile * L::pitch, *Ob = Kb + kTile * L::pitch;
-        E *Rb = (E *)(Ob + kTile * vp);
+        const E *Q = Q0 + (tile & 1) * 2 * TILE * L::pitch, *Kb = Q + TILE * L::pitch;
         cp_wait<0>();
         __syncthreads();
         if (tile + 1 < tiles) finish(tile + 1);
-        if (tile > 0) load(tile - 1);
+        load_values(tile);
+        if (tile > 0) load_keys(tile - 1);
 #pragma unroll
-        for (int s = 0; s < kTile / kChunk; ++s)
-            if (s % warps == w)
+        for (int s = 0; s < TILE / kChunk; ++s)
+            if ((tile * (TILE / kChunk) + s) % warps == w)
                 prepare<P, KP, true>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
                                      d.scale, lane);
-        if (tile > 0) gates(tile - 1);
+        if (tile > 0) gates(tile - 1), cp_wait<1>();
+        else cp_wait<0>();
         __syncthreads();
-        if ((tile + 1) * kTile % f.keep == 0 || tile == tiles - 1) {
-            const int64_t at = nh * ((steps + f.keep - 1) / f.keep) + tile * kTile / f.keep;
+        if ((tile + 1) * TILE % f.keep == 0 || tile == tiles - 1) {
+            const int64_t at = nh * ((steps + f.keep - 1) / f.keep) + tile * TILE / f.keep;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                if (w * MT + m < f.tiles_v) keep_state<E, KT>(f.kept_ds, (at * f.tiles_v + w * MT + m) * KT, S[m], lane);
+                if (w * MT + m < f.tiles_v) keep_state<KT>((E *)f.kept_ds + (at * f.tiles_v + w * MT + m) * 16 * KP, S[m], lane);
         }
 #pragma unroll 1
-        for (int s = kTile / kChunk - 1; s >= 0; --s) {
-            const int64_t at = tile * kTile + s * kChunk;
+        for (int s = TILE / kChunk - 1; s >= 0; --s) {
+            const int64_t at = tile * TILE + s * kChunk;
             if (at >= steps) continue;
             const Chunk<P> &c = chunks[s];
             const E *Qs = Q + s * kChunk * L::pitch, *Ks = Kb + s * kChunk * L::pitch, *Os = Ob + s * kChunk * vp;
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_back_state_k
             typename P::A2 o[MT], y[MT];
             float sum[4] = {};
             {
-                const typename P::B2 z = c.z.k_rows(lane), p = c.p.k_rows(lane);
+                const typename P::B2 z = c.z.n_rows(lane), p = c.p.k_rows(lane);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -157,7 +165,7 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256) goib2d_delta_back_state_k
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 for (int i = 4; i < 32; i *= 2) sum[e] += __shfl_xor_sync(~0u, sum[e], i);
-                if (g == 0) db[w * kTile + s * kChunk + (e >> 1) * 8 + 2 * t + (e & 1)] = sum[e];
+                if (g == 0) db[w * TILE + s * kChunk + (e >> 1) * 8 + 2 * t + (e & 1)] = sum[e];
             }
             T *to = row<T>(f.gr.dv, f.gr.dv_stride, n, at, h);
             if (half) {
@@ -278,7 +286,7 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
 #pragma unroll 1
     for (int j = 0; j < group; ++j) {
         const int h = hk * group + j;
-        const int64_t nh = n * d.heads + h, kept = (nh * spans + span) * tv * (KP / 16) * 32;
+        const int64_t nh = n * d.heads + h, kept = (nh * spans + span) * cols * KP;
         __syncthreads();
         const bool o = f.gr.dout != nullptr;
         load_rows(s.O, vp, o ? row<T>(f.gr.dout, f.gr.dout_stride, n, at, h) : nullptr, f.gr.dout_stride[1], o ? left : 0, C, V,
@@ -286,21 +294,20 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
         load_rows(s.V, vp, row<E>((const void *)f.dv, f.dv_stride, n, at, h), f.dv_stride[1], left, C, V, cols, f.wide_dv, tid,
                   threads);
         load_rows(s.R, vp, (const E *)f.r + (nh * steps + at) * V, V, left, C, V, cols, f.wide_r, tid, threads);
+        // S0 may hold anything where the span's first token starts afresh: it is not used then
+        const E *kept_s = (const E *)f.kept_s + kept, *kept_ds = (const E *)f.kept_ds + kept;
+        load_rows(s.S, L::pitch, kept_s, KP, cols, cols, KP, KP, true, tid, threads);
         cp_commit();
-        // S0, which may hold anything where the span's first token starts afresh
         const bool anew = load_gate<T>(d, n, at, h).fresh;
         float end = 0.0f;
-        for (int i = tid; i < tv * (KP / 16) * 32; i += threads) {
-            if (!anew) {
-                float u[8], v[8];
-                kept_values<E>(u, f.kept_s, kept + i), kept_values<E>(v, f.kept_ds, kept + i);
+        for (int i = tid * 8; i < cols * KP; i += threads * 8) {
+            float u[8], v[8];
+            eight_at(u, kept_s + i), eight_at(v, kept_ds + i);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) end += u[e] * v[e];
-            }
-            put_state(s.S, L::pitch, i / 32 / (KP / 16), i / 32 % (KP / 16), f.kept_s, kept + i, i % 32);
+            for (int e = 0; e < 8; ++e) end += u[e] * v[e];
         }
         for (int i = 16; i > 0; i >>= 1) end += __shfl_xor_sync(~0u, end, i);
-        if (lane == 0) x.end[w] = end;
+        if (lane == 0) x.end[w] = anew ? 0.0f : end;
         if (part == 0) {
             const int i = lane & 15;
             const Gate gate = load_gate<T>(d, n, at + rb * 16 + i, h);
@@ -309,9 +316,9 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
             const int since = __popc(fresh & ((2u << i) - 1)), all = __popc(fresh);
             if (lane < 16) {
                 const int l = rb * 16 + i;
-                x.a[l] = since ? 0.0f : exp2f((float)G), x.d[l] = since == all ? exp2f((float)(last - G)) : 0.0f;
+                x.a[l] = since ? 0.0f : exp2_fast((float)G), x.d[l] = since == all ? exp2_fast((float)(last - G)) : 0.0f;
                 x.b[l] = gate.b, x.hi[l] = (float)G, x.lo[l] = (float)(G - (double)(float)G), x.since[l] = since;
-                if (i == 0) x.through[rb] = all ? 0.0f : exp2f((float)last);
+                if (i == 0) x.through[rb] = all ? 0.0f : exp2_fast((float)last);
             }
         }
         cp_wait<0>();
@@ -382,7 +389,7 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
                         for (int e = 0; e < 2; ++e) {
                             const int col = nt * 8 + 2 * t + e, jj = rb * 16 + col;
                             const bool seen = col <= g + 8 * r && x.since[jj] == since, past = seen && col < g + 8 * r;
-                            const float D = seen ? exp2f((hi - x.hi[jj]) + (lo - x.lo[jj])) * x.b[jj] : 0.0f;
+                            const float D = seen ? exp2_fast((hi - x.hi[jj]) + (lo - x.lo[jj])) * x.b[jj] : 0.0f;
                             float &y = A[nt][2 * r + e], &z = M[nt][2 * r + e];
                             y = seen ? d.scale * D * y : 0.0f;
                             z = past ? -D * z : 0.0f;
@@ -442,8 +449,8 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
             if (t == 0 && part == 0) x.rows[i0 + 8 * r] = rows[r];
         }
         __syncthreads();
-        for (int i = tid; i < tv * (KP / 16) * 32; i += threads)
-            put_state(s.S, L::pitch, i / 32 / (KP / 16), i / 32 % (KP / 16), f.kept_ds, kept + i, i % 32);
+        load_rows(s.S, L::pitch, kept_ds, KP, cols, cols, KP, KP, true, tid, threads);
+        cp_commit();
         // the tokens as j: A and M over the tokens from them on
         m = 1.0f;
 #pragma unroll 1
@@ -466,7 +473,7 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
                         for (int e = 0; e < 4; ++e) {
                             const int r = e >> 1, jj = i0 + 8 * r, i = ib * 16 + nt * 8 + 2 * t + (e & 1);
                             const bool seen = jj <= i && x.since[i] == x.since[jj];
-                            const float D = seen ? exp2f((x.hi[i] - x.hi[jj]) + (x.lo[i] - x.lo[jj])) * b_i[r] : 0.0f;
+                            const float D = seen ? exp2_fast((x.hi[i] - x.hi[jj]) + (x.lo[i] - x.lo[jj])) * b_i[r] : 0.0f;
                             A[nt][e] = seen ? d.scale * D * A[nt][e] : 0.0f;
                             M[nt][e] = seen && jj < i ? -D * M[nt][e] : 0.0f;
                         }
@@ -488,6 +495,7 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
                 P::mul(dk[2 * c], dk[2 * c + 1], fm, P::k_rows(s.K, L::pitch, ib * 16, k0 + c * 16, lane));
             }
         }
+        cp_wait<0>();
         __syncthreads();
         // what they leave in the last state
         {

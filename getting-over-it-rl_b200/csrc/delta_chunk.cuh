@@ -17,7 +17,16 @@
 namespace gb {
 
 constexpr int kChunk = 16;
-constexpr int kTile = 32;  // tokens that a block holds at a time
+// Tokens that a block of the forward and backward passes over rollouts holds at a time, so that six blocks of 64
+// channels fit an SM.
+template <class P>
+constexpr int kTile = sizeof(typename P::E) == 2 ? 32 : 16;
+
+__device__ __forceinline__ float exp2_fast(float x) {  // within 2^-22; below 2^-126: 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // A 16 x 16 matrix that a chunk's products use: two bfloat16 each, or float32.
 template <class P>
@@ -30,9 +39,10 @@ struct Square<Half> {
         split(x, y, h, l);
         *(uint32_t *)&hi[r][c] = h, *(uint32_t *)&lo[r][c] = l;
     }
-    __device__ __forceinline__ void put(int r, int c, float x) {
-        hi[r][c] = __float2bfloat16_rn(x);
-        lo[r][c] = __float2bfloat16_rn(x - __bfloat162float(hi[r][c]));
+    __device__ __forceinline__ void put(int r, int c, const float (&x)[8]) {  // (r, c) to (r, c + 7), c 0 or 8
+        uint4 h, l;
+        split(x[0], x[1], h.x, l.x), split(x[2], x[3], h.y, l.y), split(x[4], x[5], h.z, l.z), split(x[6], x[7], h.w, l.w);
+        *(uint4 *)&hi[r][c] = h, *(uint4 *)&lo[r][c] = l;
     }
     __device__ __forceinline__ Half::B1 n_rows1(int lane) const { return Half::n_rows(&hi[0][0], 24, 0, 0, lane); }
     __device__ __forceinline__ Half::B2 n_rows(int lane) const {
@@ -50,22 +60,27 @@ template <>
 struct Square<Full> {
     float x[kChunk][24];
     __device__ __forceinline__ void put(int r, int c, float u, float v) { *(float2 *)&x[r][c] = make_float2(u, v); }
-    __device__ __forceinline__ void put(int r, int c, float u) { x[r][c] = u; }
+    __device__ __forceinline__ void put(int r, int c, const float (&y)[8]) {
+        *(float4 *)&x[r][c] = make_float4(y[0], y[1], y[2], y[3]);
+        *(float4 *)&x[r][c + 4] = make_float4(y[4], y[5], y[6], y[7]);
+    }
     __device__ __forceinline__ Full::B1 n_rows1(int lane) const { return Full::n_rows(&x[0][0], 24, 0, 0, lane); }
     __device__ __forceinline__ Full::B1 n_rows(int lane) const { return Full::n_rows(&x[0][0], 24, 0, 0, lane); }
     __device__ __forceinline__ Full::B1 k_rows(int lane) const { return Full::k_rows(&x[0][0], 24, 0, 0, lane); }
 };
 
-// What one chunk needs besides its rows: Z (or T), P, and the tokens' factors.
+// What one chunk needs besides its rows: Z (or T) transposed, P, and the tokens' factors.
 template <class P>
 struct alignas(16) Chunk {
-    Square<P> z, p;
-    float wt[kChunk][20];   // the strictly lower matrix, transposed
+    union {
+        Square<P> z;
+        float wt[kChunk][20];   // before Z is there: the strictly lower matrix, transposed
+    };
+    Square<P> p;
+    float4 gate[kChunk];        // hi, lo (hi + lo: G / ln 2), b, and the tokens up to this one that start afresh
     float a[kChunk], sa[kChunk], d[kChunk], b[kChunk], bd[kChunk];  // sa = scale a, bd = b d
-    float hi[kChunk], lo[kChunk];  // hi + lo: G / ln 2
-    int since[kChunk];      // tokens of the chunk up to this one that start afresh
     float a_end;
-    int odd;                // whether a write strength is not finite
+    int odd;                    // whether a write strength is not finite
 };
 
 // A token's gates, held by lanes i and i + 16 of the warp that prepares the chunk.
@@ -107,11 +122,10 @@ __device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, con
     const int since = __popc(fresh & ((2u << i) - 1)), all = __popc(fresh);
     const int odd = __any_sync(~0u, 0.0f * gate.b != 0.0f);
     if (lane < 16) {
-        const float a = since ? 0.0f : exp2f((float)G), d = since == all ? exp2f((float)(end - G)) : 0.0f;
+        const float hi = (float)G, a = since ? 0.0f : exp2_fast(hi), d = since == all ? exp2_fast((float)(end - G)) : 0.0f;
         c.a[i] = a, c.sa[i] = scale * a, c.d[i] = d, c.b[i] = gate.b, c.bd[i] = gate.b * d;
-        c.hi[i] = (float)G, c.lo[i] = (float)(G - (double)(float)G);
-        c.since[i] = since;
-        if (lane == 0) c.a_end = all ? 0.0f : exp2f((float)end), c.odd = odd;
+        c.gate[i] = make_float4(hi, (float)(G - (double)hi), gate.b, (float)since);
+        if (lane == 0) c.a_end = all ? 0.0f : exp2_fast((float)end), c.odd = odd;
     }
     float kk[2][4] = {}, qk[2][4] = {};
 #pragma unroll
@@ -121,22 +135,23 @@ __device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, con
         P::mul(qk[0], qk[1], P::a_rows(Q, pitch, 0, x, lane), kb);
     }
     __syncwarp();
+    const float4 rows[2] = {c.gate[g], c.gate[g + 8]};
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-        const int row = g + 8 * r;
-        const float hi = c.hi[row], lo = c.lo[row], bi = c.b[row];
-        const int si = c.since[row];
+    for (int n = 0; n < 2; ++n) {
+        const float4 cols[2] = {c.gate[n * 8 + 2 * t], c.gate[n * 8 + 2 * t + 1]};
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int r = 0; r < 2; ++r) {
+            const int row = g + 8 * r;
             float p[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = n * 8 + 2 * t + e;
-                const float bj = c.b[col];
-                const bool seen = col <= row && c.since[col] == si;
-                const float D = seen ? exp2f((hi - c.hi[col]) + (lo - c.lo[col])) : 0.0f;
-                c.wt[col][row] = seen && col < row ? D * kk[n][2 * r + e] * (BACK ? bi : bj) : 0.0f;
-                p[e] = seen ? scale * D * qk[n][2 * r + e] * (BACK ? 1.0f : bj) : 0.0f;
+                const bool seen = col <= row && cols[e].w == rows[r].w;
+                const float D = exp2_fast((rows[r].x - cols[e].x) + (rows[r].y - cols[e].y));
+                const float w = D * kk[n][2 * r + e] * (BACK ? rows[r].z : cols[e].z);
+                c.wt[col][row] = seen && col < row ? w : 0.0f;
+                const float x = scale * D * qk[n][2 * r + e];
+                p[e] = seen ? (BACK ? x : x * cols[e].z) : 0.0f;
             }
             c.p.put(row, n * 8 + 2 * t, p[0], p[1]);
         }
@@ -162,10 +177,11 @@ __device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, con
 #pragma unroll
         for (int r = 0; r < kChunk; ++r)
             if (r < i || __popc(fresh & ((2u << r) - 1)) != since) z[r] = 0.0f;
-    if (lane < 16) {
+    __syncwarp();
+    float half[8];  // of the column, a half-warp each
 #pragma unroll
-        for (int r = 0; r < kChunk; ++r) c.z.put(r, i, z[r]);
-    }
+    for (int r = 0; r < 8; ++r) half[r] = lane < 16 ? z[r] : z[8 + r];
+    c.z.put(i, lane / 16 * 8, half);
 }
 
 // Rows of a strided tensor into shared memory, zeros past `rows` and `cols`. Aligned rows of the same type come by
@@ -280,45 +296,19 @@ __device__ __forceinline__ void store_rows(bf16 *to, int64_t stride, uint32_t to
     __syncwarp();
 }
 
-// A 16-row tile of S^T to the fragments kept for the backward pass (Saved), and a thread's 8 values back: rows v = g,
-// g + 8 and columns 2 t, 2 t + 1, 8 on, as two accumulator tiles.
-template <class E, int KT>
-__device__ __forceinline__ void keep_state(void *kept, int64_t tile, const float (&S)[2 * KT][4], int lane) {
+// 16 rows of S^T to what is kept for the backward pass (Saved): rows v of KT * 16 channels.
+template <int KT>
+__device__ __forceinline__ void keep_state(bf16 *to, const float (&S)[2 * KT][4], int lane) {
+    uint32_t *p = (uint32_t *)to + (lane >> 2) * KT * 8 + (lane & 3);
 #pragma unroll
-    for (int j = 0; j < KT; ++j) {
-        const int64_t x = (tile + j) * 32 + lane;
-        const float(&c0)[4] = S[2 * j], (&c1)[4] = S[2 * j + 1];
-        if constexpr (sizeof(E) == 2) {
-            const Half::A1 y = Half::rounded(c0, c1);
-            ((uint4 *)kept)[x] = make_uint4(y.x[0], y.x[1], y.x[2], y.x[3]);
-        } else {
-            ((float4 *)kept)[2 * x] = make_float4(c0[0], c0[1], c0[2], c0[3]);
-            ((float4 *)kept)[2 * x + 1] = make_float4(c1[0], c1[1], c1[2], c1[3]);
-        }
-    }
+    for (int j = 0; j < 2 * KT; ++j) p[4 * j] = pack(S[j][0], S[j][1]), p[KT * 64 + 4 * j] = pack(S[j][2], S[j][3]);
 }
-template <class E>
-__device__ __forceinline__ void kept_values(float (&v)[8], const void *kept, int64_t x) {
-    if constexpr (sizeof(E) == 2) {
-        const uint4 y = ((const uint4 *)kept)[x];
-        v[0] = low(y.x), v[1] = high(y.x), v[2] = low(y.y), v[3] = high(y.y);
-        v[4] = low(y.z), v[5] = high(y.z), v[6] = low(y.w), v[7] = high(y.w);
-    } else {
-        *(float4 *)v = ((const float4 *)kept)[2 * x], *(float4 *)(v + 4) = ((const float4 *)kept)[2 * x + 1];
-    }
-}
-// A thread's 8 kept values into rows of S^T in shared memory.
-__device__ __forceinline__ void put_state(bf16 *St, int pitch, int tile_v, int tile_k, const void *kept, int64_t x, int lane) {
-    const uint4 y = ((const uint4 *)kept)[x];
-    bf16 *p = St + (tile_v * 16 + (lane >> 2)) * pitch + tile_k * 16 + 2 * (lane & 3);
-    *(uint32_t *)p = y.x, *(uint32_t *)(p + 8 * pitch) = y.y;
-    *(uint32_t *)(p + 8) = y.z, *(uint32_t *)(p + 8 * pitch + 8) = y.w;
-}
-__device__ __forceinline__ void put_state(float *St, int pitch, int tile_v, int tile_k, const void *kept, int64_t x, int lane) {
-    const float4 y = ((const float4 *)kept)[2 * x], z = ((const float4 *)kept)[2 * x + 1];
-    float *p = St + (tile_v * 16 + (lane >> 2)) * pitch + tile_k * 16 + 2 * (lane & 3);
-    *(float2 *)p = make_float2(y.x, y.y), *(float2 *)(p + 8 * pitch) = make_float2(y.z, y.w);
-    *(float2 *)(p + 8) = make_float2(z.x, z.y), *(float2 *)(p + 8 * pitch + 8) = make_float2(z.z, z.w);
+template <int KT>
+__device__ __forceinline__ void keep_state(float *to, const float (&S)[2 * KT][4], int lane) {
+    float2 *p = (float2 *)to + (lane >> 2) * KT * 8 + (lane & 3);
+#pragma unroll
+    for (int j = 0; j < 2 * KT; ++j)
+        p[4 * j] = make_float2(S[j][0], S[j][1]), p[KT * 64 + 4 * j] = make_float2(S[j][2], S[j][3]);
 }
 
 // Two neighbouring values.
@@ -327,5 +317,15 @@ __device__ __forceinline__ float2 pair_at(const bf16 *p) {
     return make_float2(low(x), high(x));
 }
 __device__ __forceinline__ float2 pair_at(const float *p) { return *(const float2 *)p; }
+
+// Eight neighbouring values, 16-byte aligned.
+__device__ __forceinline__ void eight_at(float (&v)[8], const bf16 *p) {
+    const uint4 y = *(const uint4 *)p;
+    v[0] = low(y.x), v[1] = high(y.x), v[2] = low(y.y), v[3] = high(y.y);
+    v[4] = low(y.z), v[5] = high(y.z), v[6] = low(y.w), v[7] = high(y.w);
+}
+__device__ __forceinline__ void eight_at(float (&v)[8], const float *p) {
+    *(float4 *)v = *(const float4 *)p, *(float4 *)(v + 4) = *(const float4 *)(p + 4);
+}
 
 }  // namespace gb

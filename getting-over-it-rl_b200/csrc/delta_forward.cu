@@ -13,7 +13,7 @@ namespace {
 struct Forward {
     goib2d_delta_desc d;
     void *r;          // [n][h][t][V], or NULL
-    void *kept;       // S at the start of every span, in fragments (Saved), or NULL
+    void *kept;       // S at the start of every span (Saved), or NULL
     int32_t keep;     // tokens of a span
     int32_t tiles_v;  // 16-column tiles of V
     bool wide_q, wide_k, wide_v, wide_o, wide_r;
@@ -23,8 +23,8 @@ template <class P, int KP, int MT>
 struct Layout {
     static constexpr int pitch = KP + 8, E = sizeof(typename P::E);
     __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (E == 2 ? 8 : 4); }
-    __host__ __device__ static int stage(int warps) { return kTile * (2 * pitch + v_pitch(warps)) * E; }
-    __host__ __device__ static int bytes(int warps) { return 2 * stage(warps) + kTile / kChunk * (int)sizeof(Chunk<P>); }
+    __host__ __device__ static int stage(int warps) { return kTile<P> * (2 * pitch + v_pitch(warps)) * E; }
+    __host__ __device__ static int bytes(int warps) { return 2 * stage(warps) + kTile<P> / kChunk * (int)sizeof(Chunk<P>); }
 };
 
 // A chunk that holds infinities or NaN, token by token: within the products a token meets every other one, if only as 0
@@ -67,7 +67,7 @@ template <class T, class P, int KP, int MT>
 __global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 : 1) goib2d_delta_forward_kernel(const __grid_constant__ Forward f) {
     using L = Layout<P, KP, MT>;
     using E = typename P::E;
-    constexpr int KT = KP / 16;
+    constexpr int KT = KP / 16, TILE = kTile<P>;
     constexpr bool half = sizeof(E) == 2;
     extern __shared__ __align__(16) char sm[];
     const goib2d_delta_desc &d = f.d;
@@ -84,45 +84,45 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 :
     const T *q0 = row<T>(d.q, d.q_stride, n, 0, hk), *k0 = row<T>(d.k, d.k_stride, n, 0, hk);
     const T *v_0 = row<T>(d.v, d.v_stride, n, 0, h);
     auto load = [&](int64_t tile) {
-        E *Q = (E *)(sm + (tile & 1) * stage), *Kb = Q + kTile * L::pitch, *Vb = Kb + kTile * L::pitch;
-        const int64_t at = tile * kTile;
-        const int left = (int)(steps - at < kTile ? steps - at : kTile);
-        load_rows(Q, L::pitch, q0 + at * d.q_stride[1], d.q_stride[1], left, kTile, K, KP, f.wide_q, tid, threads);
-        load_rows(Kb, L::pitch, k0 + at * d.k_stride[1], d.k_stride[1], left, kTile, K, KP, f.wide_k, tid, threads);
-        load_rows(Vb, vp, v_0 + at * d.v_stride[1], d.v_stride[1], left, kTile, V, warps * 16 * MT, f.wide_v, tid, threads);
+        E *Q = (E *)(sm + (int)(tile & 1) * stage), *Kb = Q + TILE * L::pitch, *Vb = Kb + TILE * L::pitch;
+        const int64_t at = tile * TILE;
+        const int left = (int)(steps - at < TILE ? steps - at : TILE);
+        load_rows(Q, L::pitch, q0 + at * d.q_stride[1], d.q_stride[1], left, TILE, K, KP, f.wide_q, tid, threads);
+        load_rows(Kb, L::pitch, k0 + at * d.k_stride[1], d.k_stride[1], left, TILE, K, KP, f.wide_k, tid, threads);
+        load_rows(Vb, vp, v_0 + at * d.v_stride[1], d.v_stride[1], left, TILE, V, warps * 16 * MT, f.wide_v, tid, threads);
         cp_commit();
     };
-    const int64_t tiles = (steps + kTile - 1) / kTile;
+    const int64_t tiles = (steps + TILE - 1) / TILE;
     if (tiles) load(0);
-    Gate gate[kTile / kChunk];
+    Gate gate[TILE / kChunk];
     auto gates = [&](int64_t tile) {
 #pragma unroll
-        for (int s = 0; s < kTile / kChunk; ++s)
-            if (s % warps == w) gate[s] = load_gate<T>(d, n, tile * kTile + s * kChunk + (lane & 15), h);
+        for (int s = 0; s < TILE / kChunk; ++s)
+            if ((tile * (TILE / kChunk) + s) % warps == w) gate[s] = load_gate<T>(d, n, tile * TILE + s * kChunk + (lane & 15), h);
     };
     gates(0);
     for (int64_t tile = 0; tile < tiles; ++tile) {
-        const E *Q = (const E *)(sm + (tile & 1) * stage), *Kb = Q + kTile * L::pitch;
-        E *Vb = (E *)(Kb + kTile * L::pitch);
+        const E *Q = (const E *)(sm + (int)(tile & 1) * stage), *Kb = Q + TILE * L::pitch;
+        E *Vb = (E *)(Kb + TILE * L::pitch);
         cp_wait<0>();
         __syncthreads();
         if (tile + 1 < tiles) load(tile + 1);
 #pragma unroll
-        for (int s = 0; s < kTile / kChunk; ++s)
-            if (s % warps == w)
+        for (int s = 0; s < TILE / kChunk; ++s)
+            if ((tile * (TILE / kChunk) + s) % warps == w)
                 prepare<P, KP, false>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
                                       d.scale, lane);
         if (tile + 1 < tiles) gates(tile + 1);
         __syncthreads();
-        if (f.kept && tile * kTile % f.keep == 0) {
-            const int64_t at = nh * ((steps + f.keep - 1) / f.keep) + tile * kTile / f.keep;
+        if (f.kept && tile * TILE % f.keep == 0) {
+            const int64_t at = nh * ((steps + f.keep - 1) / f.keep) + tile * TILE / f.keep;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-                if (w * MT + m < f.tiles_v) keep_state<E, KT>(f.kept, (at * f.tiles_v + w * MT + m) * KT, S[m], lane);
+                if (w * MT + m < f.tiles_v) keep_state<KT>((E *)f.kept + (at * f.tiles_v + w * MT + m) * 16 * KP, S[m], lane);
         }
 #pragma unroll 1
-        for (int s = 0; s < kTile / kChunk; ++s) {
-            const int64_t at = tile * kTile + s * kChunk;
+        for (int s = 0; s < TILE / kChunk; ++s) {
+            const int64_t at = tile * TILE + s * kChunk;
             if (at >= steps) break;
             const Chunk<P> &c = chunks[s];
             const E *Qs = Q + s * kChunk * L::pitch, *Ks = Kb + s * kChunk * L::pitch;
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 :
                     P::mul(O[m][0], O[m][1], P::first(a), qb);  // Half: o is rounded to bfloat16, S once before it
                 }
             }
-            const typename P::B2 z = c.z.n_rows(lane);
+            const typename P::B2 z = c.z.k_rows(lane);
             float bad = 0.0f;
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
