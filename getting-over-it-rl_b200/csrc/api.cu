@@ -1020,6 +1020,8 @@ int goib2d_candidate_pairs(const goib2d_pair_desc *d, int32_t *pair_a, int32_t *
 
 // ---- the policy's side (delta_*.cu, clip.cu)
 namespace {
+bool far(const int64_t *stride) { return stride[1] > INT32_MAX || stride[1] < -INT32_MAX; }
+
 int delta_check(const goib2d_delta_desc *d) {
     if (!d) return fail(GOIB2D_EINVAL, "null argument");
     if (d->n_worlds < 0 || d->n_steps < 0) return fail(GOIB2D_EINVAL, "negative size");
@@ -1034,6 +1036,10 @@ int delta_check(const goib2d_delta_desc *d) {
                                                         (long long)d->n_worlds, d->heads);
     const int64_t token = (int64_t)d->heads * (d->key_dim + d->value_dim);
     if (d->n_worlds && d->n_steps > (INT64_MAX >> 6) / d->n_worlds / token) return fail(GOIB2D_ELIMIT, "size overflows");
+    if (d->n_steps > INT32_MAX - 64) return fail(GOIB2D_ELIMIT, "%lld steps (2^31 - 65 at most)", (long long)d->n_steps);
+    if (far(d->q_stride) || far(d->k_stride) || far(d->v_stride) || far(d->g_stride) || far(d->beta_stride) ||
+        far(d->out_stride) || far(d->reset_stride))
+        return fail(GOIB2D_ELIMIT, "a step's stride is 2^31 elements or more");
     const int64_t spans = (d->n_steps + 31) / 32;
     if (d->n_worlds && spans > INT32_MAX / (d->n_worlds * d->heads))
         return fail(GOIB2D_ELIMIT, "%lld steps of %lld worlds of %d heads (2^31 - 1 pieces of 32 steps in all)",
@@ -1088,6 +1094,8 @@ int goib2d_delta_backward(const goib2d_delta_desc *d, const goib2d_delta_grads *
     if (d->n_steps && (!saved || (uintptr_t)saved % 16)) return fail(GOIB2D_EINVAL, "saved is null or not 16-byte aligned");
     if (d->n_steps && (!gr->dq || !gr->dk || !gr->dv || !gr->dg || !gr->dbeta))
         return fail(GOIB2D_EINVAL, "null gradient");
+    if (far(gr->dout_stride) || far(gr->dv_stride))
+        return fail(GOIB2D_ELIMIT, "a step's stride is 2^31 elements or more");
     CUDA_TRY(gb::launch_delta_backward(*d, *gr, saved, workspace, (cudaStream_t)stream));
     return 0;
 }

@@ -55,7 +55,7 @@ struct Saved {
     int64_t r, states, bytes;   // bytes: both
     int32_t keep, tiles_v, tiles_k, size;
 };
-inline int padded_keys(int K) { return K <= 16 ? 16 : K <= 32 ? 32 : K <= 64 ? 64 : 128; }
+inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
 inline Saved delta_saved(const goib2d_delta_desc &d) {
     const int64_t nh = d.n_worlds * d.heads;
     Saved s;
@@ -68,6 +68,26 @@ inline Saved delta_saved(const goib2d_delta_desc &d) {
     s.bytes = s.r + s.states;
     return s;
 }
+
+// How the columns of V are shared out in the passes over rollouts: a block takes 64 columns of one (world, head) with
+// warps of 32 (of 16, where a state has 128 channels: 64 accumulators a thread either way); where that makes fewer
+// than two blocks for an SM, in the shape for few (ahead, delta_chunk.cuh), with warps of 16 columns, and so many in a
+// block that every SM has one, up to four.
+struct Split {
+    int MT, warps, blocks;
+    bool ahead;
+    explicit Split(const goib2d_delta_desc &d) {
+        const int64_t nh = d.n_worlds * d.heads;
+        const int tiles = (d.value_dim + 15) / 16;
+        ahead = nh * ((tiles + 3) / 4) < 2 * 148;
+        MT = ahead || tiles == 1 || d.key_dim > 64 ? 1 : 2;
+        const int all = (tiles + MT - 1) / MT;
+        warps = all < 4 / MT ? all : 4 / MT;
+        if (ahead)
+            while (warps > 1 && nh * ((all + warps - 1) / warps) < 100) warps = (warps + 1) / 2;
+        blocks = (all + warps - 1) / warps;
+    }
+};
 
 // Allow a kernel `bytes` of dynamic shared memory, and the SM's largest share of it for its blocks.
 template <class F>

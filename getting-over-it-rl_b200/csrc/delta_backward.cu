@@ -25,107 +25,101 @@ struct Backward {
     void *kept_ds;           // dS after each span, in the same layout
     void *dv;                // dv as the second kernel reads it: gr.dv, or float32 in the workspace
     int64_t dv_stride[3];
-    int32_t keep, tiles_v;
+    float *db;               // db by warps' columns: [n][h][parts][t]
+    int32_t keep, tiles_v, parts;
     bool wide_q, wide_k, wide_do, wide_dv, wide_r;
     bool wide_dqk;           // pairs of channels of dq and dk are aligned
 };
 
 // ---- dS through the rollout, dv and db
 
-template <class P, int KP, int MT>
+template <class P, int KP, int MT, bool AHEAD>
 struct Layout {
-    static constexpr int pitch = KP + 8, E = sizeof(typename P::E);
-    __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (E == 2 ? 8 : 4); }
+    using E = typename P::E;
+    static constexpr int pitch = KP + 8, chunks = AHEAD ? 2 : kTile<P> / kChunk;
+    static constexpr int rows = AHEAD ? kChunk : kTile<P>;  // of a slot
+    static constexpr int keys = AHEAD ? 4 : 2, values = AHEAD ? 4 : 1;  // slots of q and k, of dO and r
+    static constexpr int most = MT == 2 ? 2 : 4;            // warps that solve
+    static constexpr int threads = 32 * (most + (AHEAD ? 2 : 0));
+    __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (sizeof(E) == 2 ? 8 : 4); }
     __host__ __device__ static int bytes(int warps) {
-        return kTile<P> * (4 * pitch + 2 * v_pitch(warps)) * E + kTile<P> / kChunk * (int)sizeof(Chunk<P>) +
-               warps * kTile<P> * 4;
+        return 2 * rows * (keys * pitch + values * v_pitch(warps)) * (int)sizeof(E) + chunks * (int)sizeof(Chunk<P>);
     }
 };
 
-template <class T, class P, int KP, int MT>
-__global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 : 1) goib2d_delta_back_state_kernel(const __grid_constant__ Backward f) {
-    using L = Layout<P, KP, MT>;
+template <class T, class P, int KP, int MT, bool AHEAD>
+__global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 : KP == 128 ? 3 : MT == 2 ? 6 : 3)
+    goib2d_delta_back_state_kernel(const __grid_constant__ Backward f) {
+    using L = Layout<P, KP, MT, AHEAD>;
     using E = typename P::E;
-    constexpr int KT = KP / 16, TILE = kTile<P>;
+    constexpr int KT = KP / 16;
     constexpr bool half = sizeof(E) == 2;
     extern __shared__ __align__(16) char sm[];
     const goib2d_delta_desc &d = f.d;
-    const int K = d.key_dim, V = d.value_dim, threads = blockDim.x, warps = threads / 32;
-    const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
-    const int64_t nh = blockIdx.x, n = nh / d.heads, steps = d.n_steps;
+    const int K = d.key_dim, V = d.value_dim, w = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane >> 2, t = lane & 3;
+    const int warps = blockDim.x / 32 - (AHEAD ? 2 : 0), threads = blockDim.x;
+    const int64_t nh = blockIdx.x, n = nh / d.heads;
+    const int steps = (int)d.n_steps, count = (steps + kChunk - 1) / kChunk;
     const int h = (int)(nh - n * d.heads), hk = h / (d.heads / d.key_heads);
-    const int vp = L::v_pitch(warps), v0 = w * 16 * MT, cols = warps * 16 * MT;
-    // Q and K twice, the next tile's coming while this one is solved; dO and r once, coming while Z and P are made
-    E *const Q0 = (E *)sm, *const Ob = Q0 + 4 * TILE * L::pitch, *const Rb = Ob + TILE * vp;
-    Chunk<P> *chunks = (Chunk<P> *)(Rb + TILE * vp);
-    float *db = (float *)(chunks + TILE / kChunk);  // [warp][token of the tile]
+    const int vp = L::v_pitch(warps), cols = warps * 16 * MT, block0 = blockIdx.y * cols;
+    const int key_slot = 2 * L::rows * L::pitch, value_slot = 2 * L::rows * vp;
+    E *const keys = (E *)sm, *const values = keys + L::keys * key_slot;
+    Chunk<P> *chunks = (Chunk<P> *)(values + L::values * value_slot);
+    const T *const q = row<T>(d.q, d.q_stride, n, 0, hk), *const k = row<T>(d.k, d.k_stride, n, 0, hk);
+    const T *const o = f.gr.dout ? row<T>(f.gr.dout, f.gr.dout_stride, n, 0, h) + block0 : nullptr;
+    const E *const r = (const E *)f.r + nh * steps * V + block0;
+    const int qs = (int)d.q_stride[1], ks = (int)d.k_stride[1], os = (int)f.gr.dout_stride[1];
+    const Gates<T> gates(d, n, h);
 
+    if (AHEAD && w >= warps) {
+        // every second chunk, from the last down (i-th: chunk count - 1 - i); two slots and one chunk's matrices
+        const int me = w - warps;
+        auto load = [&](int i) {
+            const int at = (count - 1 - i) * kChunk, left = steps - at;
+            if (at >= 0) {
+                E *Q = keys + (i & 3) * key_slot, *Ob = values + (i & 3) * value_slot;
+                chunk_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, K, KP, f.wide_q, lane);
+                chunk_rows(Q + kChunk * L::pitch, L::pitch, k + (int64_t)at * ks, ks, left, K, KP, f.wide_k, lane);
+                chunk_rows(Ob, vp, o + (int64_t)at * os, os, o ? left : 0, V - block0, cols, f.wide_do, lane);
+                chunk_rows(Ob + kChunk * vp, vp, r + (int64_t)at * V, V, left, V - block0, cols, f.wide_r, lane);
+            }
+            cp_commit();
+        };
+        auto gate_of = [&](int i) {
+            const int at = (count - 1 - i) * kChunk;
+            return at < 0 ? Gate{0.0f, 0.0f, false} : gates.at(at + (lane & 15));
+        };
+        load(me);
+        Gate next = gate_of(me);
+        for (int i = me; i < count; i += 2) {
+            if (i >= 2) bar_wait(3 + me, 32 + 32 * warps);  // i - 2 is done: its slot and its matrices are free
+            load(i + 2);
+            const Gate gate = next;
+            next = gate_of(i + 2);
+            cp_wait<1>();
+            __syncwarp();
+            const E *Q = keys + (i & 3) * key_slot;
+            prepare<P, KP, true>(chunks[me], Q, Q + kChunk * L::pitch, L::pitch, gate, d.scale, lane);
+            __threadfence_block();
+            bar_arrive(1 + me, 32 + 32 * warps);
+        }
+        return;
+    }
+
+    const int v0 = w * 16 * MT, tile0 = block0 / 16 + w * MT;
     float S[MT][KP / 8][4];  // dS^T: rows v, columns k
-    load_state<MT, KP>(S, f.gr.dstate_out ? f.gr.dstate_out + nh * K * V : nullptr, K, V, v0, lane);
-    const int64_t tiles = (steps + TILE - 1) / TILE;
-    const T *q0 = row<T>(d.q, d.q_stride, n, 0, hk), *k0 = row<T>(d.k, d.k_stride, n, 0, hk);
-    const T *o0 = f.gr.dout ? row<T>(f.gr.dout, f.gr.dout_stride, n, 0, h) : nullptr;
-    const E *r0 = (const E *)f.r + nh * steps * V;
-    auto load_keys = [&](int64_t tile) {
-        E *Q = Q0 + (tile & 1) * 2 * TILE * L::pitch;
-        const int64_t at = tile * TILE;
-        const int left = (int)(steps - at < TILE ? steps - at : TILE);
-        load_rows(Q, L::pitch, q0 + at * d.q_stride[1], d.q_stride[1], left, TILE, K, KP, f.wide_q, tid, threads);
-        load_rows(Q + TILE * L::pitch, L::pitch, k0 + at * d.k_stride[1], d.k_stride[1], left, TILE, K, KP, f.wide_k, tid, threads);
-        cp_commit();
-    };
-    auto load_values = [&](int64_t tile) {
-        const int64_t at = tile * TILE;
-        const int left = (int)(steps - at < TILE ? steps - at : TILE);
-        load_rows(Ob, vp, o0 + at * f.gr.dout_stride[1], f.gr.dout_stride[1], o0 ? left : 0, TILE, V, cols, f.wide_do, tid,
-                  threads);
-        load_rows(Rb, vp, r0 + at * V, V, left, TILE, V, cols, f.wide_r, tid, threads);
-        cp_commit();
-    };
-    Gate gate[TILE / kChunk];
-    auto gates = [&](int64_t tile) {
+    load_state<MT, KP>(S, f.gr.dstate_out ? f.gr.dstate_out + nh * K * V : nullptr, K, V, block0 + v0, lane);
+    T *const dv = row<T>(f.gr.dv, f.gr.dv_stride, n, 0, h) + block0;
+    E *const also = !half && f.dv != f.gr.dv ? row<E>(f.dv, f.dv_stride, n, 0, h) + block0 : nullptr;
+    float *const db = tile0 < f.tiles_v ? f.db + (nh * f.parts + tile0 / MT) * steps : nullptr;
+    const int dvs = (int)f.gr.dv_stride[1];
+    auto solve = [&](int at, const E *Qs, const E *Ks, const E *Os, E *Rs, const Chunk<P> &c) {
+            if ((at + kChunk) % f.keep == 0 || at + kChunk >= steps) {
+                const int64_t x = (nh * ((steps + f.keep - 1) / f.keep) + at / f.keep) * f.tiles_v + tile0;
 #pragma unroll
-        for (int s = 0; s < TILE / kChunk; ++s)
-            if ((tile * (TILE / kChunk) + s) % warps == w) gate[s] = load_gate<T>(d, n, tile * TILE + s * kChunk + (lane & 15), h);
-    };
-    // db of the tile before, from the warps' parts
-    auto finish = [&](int64_t tile) {
-        const int64_t at = tile * TILE + tid;
-        if (tid < TILE && at < steps) {
-            float x = 0.0f;
-            for (int i = 0; i < warps; ++i) x += db[i * TILE + tid];
-            *row<T>(f.gr.dbeta, f.gr.dbeta_stride, n, at, h) = from_float<T>(x);
-        }
-    };
-    if (tiles) load_keys(tiles - 1), gates(tiles - 1);
-    for (int64_t tile = tiles - 1; tile >= 0; --tile) {
-        const E *Q = Q0 + (tile & 1) * 2 * TILE * L::pitch, *Kb = Q + TILE * L::pitch;
-        cp_wait<0>();
-        __syncthreads();
-        if (tile + 1 < tiles) finish(tile + 1);
-        load_values(tile);
-        if (tile > 0) load_keys(tile - 1);
-#pragma unroll
-        for (int s = 0; s < TILE / kChunk; ++s)
-            if ((tile * (TILE / kChunk) + s) % warps == w)
-                prepare<P, KP, true>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
-                                     d.scale, lane);
-        if (tile > 0) gates(tile - 1), cp_wait<1>();
-        else cp_wait<0>();
-        __syncthreads();
-        if ((tile + 1) * TILE % f.keep == 0 || tile == tiles - 1) {
-            const int64_t at = nh * ((steps + f.keep - 1) / f.keep) + tile * TILE / f.keep;
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-                if (w * MT + m < f.tiles_v) keep_state<KT>((E *)f.kept_ds + (at * f.tiles_v + w * MT + m) * 16 * KP, S[m], lane);
-        }
-#pragma unroll 1
-        for (int s = TILE / kChunk - 1; s >= 0; --s) {
-            const int64_t at = tile * TILE + s * kChunk;
-            if (at >= steps) continue;
-            const Chunk<P> &c = chunks[s];
-            const E *Qs = Q + s * kChunk * L::pitch, *Ks = Kb + s * kChunk * L::pitch, *Os = Ob + s * kChunk * vp;
-            E *Rs = Rb + s * kChunk * vp;
+                for (int m = 0; m < MT; ++m)
+                    if (tile0 + m < f.tiles_v) keep_state<KT>((E *)f.kept_ds + (x + m) * 16 * KP, S[m], lane);
+            }
             const uint32_t tokens = steps - at < kChunk ? (1u << (steps - at)) - 1 : 0xffffu;
             float X[MT][2][4] = {};
 #pragma unroll
@@ -165,19 +159,20 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 :
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 for (int i = 4; i < 32; i *= 2) sum[e] += __shfl_xor_sync(~0u, sum[e], i);
-                if (g == 0) db[w * TILE + s * kChunk + (e >> 1) * 8 + 2 * t + (e & 1)] = sum[e];
+                const int token = (e >> 1) * 8 + 2 * t + (e & 1);
+                if (g == 0 && db && at + token < steps) db[at + token] = sum[e];
             }
-            T *to = row<T>(f.gr.dv, f.gr.dv_stride, n, at, h);
+            T *to = dv + (int64_t)at * dvs;
             if (half) {
-                store_rows<MT>((bf16 *)to, f.gr.dv_stride[1], tokens, v0, V, f.wide_dv, (bf16 *)Rs, vp, X, lane);
+                store_rows<MT>((bf16 *)to, dvs, tokens, v0, V - block0, f.wide_dv, (bf16 *)Rs, vp, X, lane);
             } else {
 #pragma unroll
-                for (int m = 0; m < MT; ++m) store_direct<T>(to, f.gr.dv_stride[1], tokens, v0 + 16 * m, V, X[m], lane);
-                if (f.dv != f.gr.dv) {
-                    E *also = row<E>(f.dv, f.dv_stride, n, at, h);
+                for (int m = 0; m < MT; ++m) store_direct<T>(to, dvs, tokens, v0 + 16 * m, V - block0, X[m], lane);
+                if (also)
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) store_direct<E>(also, f.dv_stride[1], tokens, v0 + 16 * m, V, X[m], lane);
-                }
+                    for (int m = 0; m < MT; ++m)
+                        store_direct<E>(also + (int64_t)at * f.dv_stride[1], (int)f.dv_stride[1], tokens, v0 + 16 * m, V - block0,
+                                        X[m], lane);
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
@@ -208,11 +203,64 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 :
 #pragma unroll
                 for (int m = 0; m < MT; ++m) P::mul(S[m][2 * j], S[m][2 * j + 1], y[m], kb);
             }
+    };
+    if constexpr (AHEAD) {
+#pragma unroll 1
+        for (int i = 0; i < count; ++i) {
+            const E *Q = keys + (i & 3) * key_slot;
+            E *Ob = values + (i & 3) * value_slot;
+            bar_wait(1 + (i & 1), 32 + 32 * warps);
+            solve((count - 1 - i) * kChunk, Q, Q + kChunk * L::pitch, Ob, Ob + kChunk * vp, chunks[i & 1]);
+            if (i + 2 < count) bar_arrive(3 + (i & 1), 32 + 32 * warps);
+        }
+    } else {
+        // q and k twice, the next tile's coming while this one is solved; dO and r once, coming while the chunks are prepared
+        constexpr int TILE = kTile<P>, N = TILE / kChunk;
+        const int tiles = (steps + TILE - 1) / TILE;
+        E *const Ob = values, *const Rb = values + TILE * vp;
+        auto load_keys = [&](int tile) {
+            E *Q = keys + (tile & 1) * key_slot;
+            const int at = tile * TILE, left = steps - at < TILE ? steps - at : TILE;
+            load_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, TILE, K, KP, f.wide_q, threadIdx.x, threads);
+            load_rows(Q + TILE * L::pitch, L::pitch, k + (int64_t)at * ks, ks, left, TILE, K, KP, f.wide_k, threadIdx.x, threads);
+            cp_commit();
+        };
+        auto load_values = [&](int tile) {
+            const int at = tile * TILE, left = steps - at < TILE ? steps - at : TILE;
+            load_rows(Ob, vp, o + (int64_t)at * os, os, o ? left : 0, TILE, V - block0, cols, f.wide_do, threadIdx.x, threads);
+            load_rows(Rb, vp, r + (int64_t)at * V, V, left, TILE, V - block0, cols, f.wide_r, threadIdx.x, threads);
+            cp_commit();
+        };
+        Gate gate[N];
+        auto gates_of = [&](int tile) {
+#pragma unroll
+            for (int s = 0; s < N; ++s)
+                if ((tile * N + s) % warps == w) gate[s] = gates.at(tile * TILE + s * kChunk + (lane & 15));
+        };
+        if (tiles) load_keys(tiles - 1), gates_of(tiles - 1);
+#pragma unroll 1
+        for (int tile = tiles - 1; tile >= 0; --tile) {
+            const E *Q = keys + (tile & 1) * key_slot, *Kb = Q + TILE * L::pitch;
+            cp_wait<0>();
+            __syncthreads();
+            load_values(tile);
+            if (tile > 0) load_keys(tile - 1);
+#pragma unroll
+            for (int s = 0; s < N; ++s)
+                if ((tile * N + s) % warps == w)
+                    prepare<P, KP, true>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
+                                         d.scale, lane);
+            if (tile > 0) gates_of(tile - 1), cp_wait<1>();
+            else cp_wait<0>();
+            __syncthreads();
+#pragma unroll 1
+            for (int s = N - 1; s >= 0; --s)
+                if (tile * TILE + s * kChunk < steps)
+                    solve(tile * TILE + s * kChunk, Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, Ob + s * kChunk * vp,
+                          Rb + s * kChunk * vp, chunks[s]);
         }
     }
-    __syncthreads();
-    if (tiles) finish(0);
-    if (f.gr.dstate_in) store_state<MT, KP>(f.gr.dstate_in + nh * K * V, S, K, V, v0, lane);
+    if (f.gr.dstate_in) store_state<MT, KP>(f.gr.dstate_in + nh * K * V, S, K, V, block0 + v0, lane);
 }
 
 // ---- dq, dk and dg, span by span
@@ -319,6 +367,11 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
                 x.a[l] = since ? 0.0f : exp2_fast((float)G), x.d[l] = since == all ? exp2_fast((float)(last - G)) : 0.0f;
                 x.b[l] = gate.b, x.hi[l] = (float)G, x.lo[l] = (float)(G - (double)(float)G), x.since[l] = since;
                 if (i == 0) x.through[rb] = all ? 0.0f : exp2_fast((float)last);
+                if (l < left) {
+                    float db = 0.0f;
+                    for (int e = 0; e < f.parts; ++e) db += f.db[(nh * f.parts + e) * steps + at + l];
+                    *row<T>(f.gr.dbeta, f.gr.dbeta_stride, n, at + l, h) = from_float<T>(db);
+                }
             }
         }
         cp_wait<0>();
@@ -605,13 +658,13 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
     }
 }
 
-template <class T, class P, int KP, int MT>
-cudaError_t back_state(const Backward &f, cudaStream_t s) {
-    const int warps = (f.d.value_dim + 16 * MT - 1) / (16 * MT);
-    const size_t smem = Layout<P, KP, MT>::bytes(warps);
-    cudaError_t e = allow_smem(goib2d_delta_back_state_kernel<T, P, KP, MT>, smem);
+template <class T, class P, int KP, int MT, bool AHEAD>
+cudaError_t back_state(const Backward &f, const Split &b, cudaStream_t s) {
+    const size_t smem = Layout<P, KP, MT, AHEAD>::bytes(b.warps);
+    cudaError_t e = allow_smem(goib2d_delta_back_state_kernel<T, P, KP, MT, AHEAD>, smem);
     if (e != cudaSuccess) return e;
-    goib2d_delta_back_state_kernel<T, P, KP, MT><<<(unsigned)(f.d.n_worlds * f.d.heads), 32 * warps, smem, s>>>(f);
+    goib2d_delta_back_state_kernel<T, P, KP, MT, AHEAD>
+        <<<dim3((unsigned)(f.d.n_worlds * f.d.heads), b.blocks), 32 * (b.warps + (AHEAD ? 2 : 0)), smem, s>>>(f);
     return cudaGetLastError();
 }
 
@@ -627,13 +680,27 @@ cudaError_t back_span(const Backward &f, cudaStream_t s) {
 }
 
 template <class T, class P, int KP>
-cudaError_t backward_of(const Backward &f, cudaStream_t s) {
-    const cudaError_t e = f.d.value_dim <= 16 ? back_state<T, P, KP, 1>(f, s) : back_state<T, P, KP, 2>(f, s);
+cudaError_t back_wide(Backward &f, cudaStream_t s) {
+    const Split b(f.d);
+    f.parts = (f.tiles_v + b.MT - 1) / b.MT;
+    if (b.ahead) return back_state<T, P, KP, 1, true>(f, b, s);
+    if constexpr (KP < 128)
+        if (b.MT == 2) return back_state<T, P, KP, 2, false>(f, b, s);
+    return back_state<T, P, KP, 1, false>(f, b, s);
+}
+
+template <class T, class P, int KP>
+cudaError_t backward_of(Backward &f, cudaStream_t s) {
+    const cudaError_t e = back_wide<T, P, KP>(f, s);
     if (e != cudaSuccess) return e;
     if constexpr (sizeof(typename P::E) == 2 || KP <= 64)
         if (f.keep == 64) return back_span<T, P, KP, 64>(f, s);
     if constexpr (sizeof(typename P::E) == 4) return back_span<T, P, KP, 32>(f, s);
     return cudaErrorUnknown;
+}
+
+int64_t db_bytes(const goib2d_delta_desc &d) {  // [n][h][16-column tiles of V][t], in whole 16 bytes
+    return (d.n_worlds * d.heads * ((d.value_dim + 15) / 16) * d.n_steps * 4 + 15) / 16 * 16;
 }
 
 template <class T, class P>
@@ -645,8 +712,9 @@ cudaError_t backward_typed(const goib2d_delta_desc &d, const goib2d_delta_grads 
     const int V = d.value_dim, z = sizeof(T);
     f.dv = gr.dv;
     for (int i = 0; i < 3; ++i) f.dv_stride[i] = gr.dv_stride[i];
+    f.db = (float *)((char *)workspace + at.states);
     if (sizeof(T) != sizeof(typename P::E)) {
-        f.dv = (char *)workspace + at.states;
+        f.dv = (char *)workspace + at.states + db_bytes(d);
         f.dv_stride[0] = d.n_steps * d.heads * V, f.dv_stride[1] = (int64_t)d.heads * V, f.dv_stride[2] = V;
     }
     f.wide_q = rows_aligned(d.q, d.q_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
@@ -657,7 +725,6 @@ cudaError_t backward_typed(const goib2d_delta_desc &d, const goib2d_delta_grads 
     f.wide_dqk = (uintptr_t)gr.dq % (2 * z) == 0 && (uintptr_t)gr.dk % (2 * z) == 0;
     for (int i = 0; i < 3; ++i) f.wide_dqk = f.wide_dqk && gr.dq_stride[i] % 2 == 0 && gr.dk_stride[i] % 2 == 0;
     switch (padded_keys(d.key_dim)) {
-        case 16: return backward_of<T, P, 16>(f, s);
         case 32: return backward_of<T, P, 32>(f, s);
         case 64: return backward_of<T, P, 64>(f, s);
         default: return backward_of<T, P, 128>(f, s);
@@ -668,7 +735,7 @@ cudaError_t backward_typed(const goib2d_delta_desc &d, const goib2d_delta_grads 
 
 int64_t delta_workspace_bytes(const goib2d_delta_desc &d) {
     const Saved s = delta_saved(d);
-    return s.states + (d.dtype == GOIB2D_BFLOAT16 && s.size == 4 ? s.r : 0);
+    return s.states + db_bytes(d) + (d.dtype == GOIB2D_BFLOAT16 && s.size == 4 ? s.r : 0);
 }
 
 cudaError_t launch_delta_backward(const goib2d_delta_desc &d, const goib2d_delta_grads &gr, const void *saved,

@@ -17,11 +17,17 @@
 namespace gb {
 
 constexpr int kChunk = 16;
-// Tokens that a block of the forward and backward passes over rollouts holds at a time, so that six blocks of 64
-// channels fit an SM.
-template <class P>
-constexpr int kTile = sizeof(typename P::E) == 2 ? 32 : 16;
 
+// The passes over rollouts come in two shapes. With blocks for every SM, all warps of a block load a tile of chunks,
+// prepare one each and solve them in turn: nothing waits idle, as others have the SM meanwhile. With few (worlds, heads)
+// a chunk's latency is the rollout's: then two warps more run ahead of the others and prepare every second chunk each
+// (AHEAD), and the columns are spread over more warps.
+template <class P>
+constexpr int kTile = sizeof(typename P::E) == 2 ? 32 : 16;  // tokens of a tile, so that six blocks of 64 channels fit
+
+// One warp that prepares and the ones that solve, by the hardware's named barriers: `threads` counts both.
+__device__ __forceinline__ void bar_wait(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ float exp2_fast(float x) {  // within 2^-22; below 2^-126: 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -98,6 +104,23 @@ __device__ __forceinline__ Gate load_gate(const goib2d_delta_desc &d, int64_t n,
     r.fresh = (d.reset && d.reset[n * d.reset_stride[0] + t * d.reset_stride[1]]) || expf(r.g) == 0.0f;
     return r;
 }
+
+// The gates of one (world, head), chunk by chunk.
+template <class T>
+struct Gates {
+    const T *g, *b;
+    const uint8_t *reset;
+    int gs, bs, rs, steps;
+    __device__ __forceinline__ Gates(const goib2d_delta_desc &d, int64_t n, int h)
+        : g(row<T>(d.g, d.g_stride, n, 0, h)), b(row<T>(d.beta, d.beta_stride, n, 0, h)),
+          reset(d.reset ? d.reset + n * d.reset_stride[0] : nullptr), gs((int)d.g_stride[1]), bs((int)d.beta_stride[1]),
+          rs((int)d.reset_stride[1]), steps((int)d.n_steps) {}
+    __device__ __forceinline__ Gate at(int t) const {  // lane's token
+        if (t >= steps) return {0.0f, 0.0f, false};
+        const float x = to_float(g[(int64_t)t * gs]), y = to_float(b[(int64_t)t * bs]);
+        return {x, y, (reset && reset[(int64_t)t * rs]) || expf(x) == 0.0f};
+    }
+};
 
 // The running sums of 16 tokens' g / ln 2, in float64: differences of sums over a chunk of strong decays keep
 // float32's precision. Lanes i and i + 16 hold token i.
@@ -260,9 +283,32 @@ __device__ __forceinline__ void store_state(float *to, const float (&S)[MT][KP /
             }
 }
 
+// The same for 16 rows by one warp.
+template <class E, class T>
+__device__ __forceinline__ void chunk_rows(E *to, int pitch, const T *from, int stride, int rows, int cols, int padded,
+                                           bool wide, int lane) {
+    if constexpr (sizeof(T) == sizeof(E)) {
+        if (wide) {
+            constexpr int N = 16 / sizeof(E);
+            for (int c = lane % 8 * N; c < padded; c += 8 * N) {
+                const T *p = from + (int64_t)(lane / 8) * stride + c;
+                E *q = to + lane / 8 * pitch + c;
+                const int left = c < cols ? rows - lane / 8 : 0;
+#pragma unroll
+                for (int r = 0; r < kChunk; r += 4, p += (int64_t)4 * stride, q += 4 * pitch) {
+                    if (r < left) cp_async16(q, p);
+                    else *(uint4 *)q = make_uint4(0, 0, 0, 0);
+                }
+            }
+            return;
+        }
+    }
+    load_rows(to, pitch, from, stride, rows, kChunk, cols, padded, false, lane, 32);
+}
+
 // 16 x 16 values (rows v, columns tokens) of one accumulator pair, to the rows of a strided tensor; tokens: a bit each
 template <class T>
-__device__ __forceinline__ void store_direct(T *to, int64_t stride, uint32_t tokens, int v0, int V, const float (&c)[2][4],
+__device__ __forceinline__ void store_direct(T *to, int stride, uint32_t tokens, int v0, int V, const float (&c)[2][4],
                                              int lane) {
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -270,13 +316,13 @@ __device__ __forceinline__ void store_direct(T *to, int64_t stride, uint32_t tok
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int token = n * 8 + 2 * t + (e & 1), v = v0 + g + (e >> 1) * 8;
-            if (tokens >> token & 1 && v < V) to[token * stride + v] = from_float<T>(c[n][e]);
+            if (tokens >> token & 1 && v < V) to[(int64_t)token * stride + v] = from_float<T>(c[n][e]);
         }
 }
 
 // The same for MT tiles by way of the warp's own columns of a [token][v] buffer, for rows of 16-byte pieces.
 template <int MT>
-__device__ __forceinline__ void store_rows(bf16 *to, int64_t stride, uint32_t tokens, int v0, int V, bool wide, bf16 *buf,
+__device__ __forceinline__ void store_rows(bf16 *to, int stride, uint32_t tokens, int v0, int V, bool wide, bf16 *buf,
                                            int pitch, const float (&c)[MT][2][4], int lane) {
     __syncwarp();
 #pragma unroll
@@ -288,7 +334,7 @@ __device__ __forceinline__ void store_rows(bf16 *to, int64_t stride, uint32_t to
         const int x = lane + 32 * m, token = x / (2 * MT), v = v0 + x % (2 * MT) * 8;
         if (!(tokens >> token & 1) || v >= V) continue;
         const bf16 *p = buf + token * pitch + v;
-        bf16 *q = to + token * stride + v;
+        bf16 *q = to + (int64_t)token * stride + v;
         if (wide) *(uint4 *)q = *(const uint4 *)p;
         else
             for (int e = 0; e < 8 && v + e < V; ++e) q[e] = p[e];

@@ -1,10 +1,9 @@
 // The gated delta rule over rollouts (goib2d_delta_forward), in chunks of 16 tokens (delta_chunk.cuh).
 //
-// One block per (world, head); each warp owns MT * 16 columns of S, as the transposed accumulators S^T [V][K] of its
-// matrix products, for the whole rollout: q, k, v are read once, o written once, and the state never leaves the
-// registers. A chunk's products chain without shared memory: S^T is the A operand of S^T K^T and S^T Q^T, their
-// result (V - a Y)^T that of (..) Z^T, its result u^T that of u^T P^T and of the update u^T K. Tiles of two chunks are
-// loaded ahead by asynchronous copies while the warps solve the current one; the warps share out the chunks' Z and P.
+// A block takes some columns of V of one (world, head); a warp owns MT * 16 of them, as the transposed accumulators S^T
+// [V][K] of its matrix products, for the whole rollout: v is read once, o written once, and the state never leaves the
+// registers. A chunk's products chain without shared memory: S^T is the A operand of S^T K^T and S^T Q^T, their result
+// (V - a Y)^T that of (..) Z^T, its result r^T that of r^T P^T and of the update u^T K.
 #include "delta_chunk.cuh"
 
 namespace gb {
@@ -19,12 +18,16 @@ struct Forward {
     bool wide_q, wide_k, wide_v, wide_o, wide_r;
 };
 
-template <class P, int KP, int MT>
+template <class P, int KP, int MT, bool AHEAD>
 struct Layout {
-    static constexpr int pitch = KP + 8, E = sizeof(typename P::E);
-    __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (E == 2 ? 8 : 4); }
-    __host__ __device__ static int stage(int warps) { return kTile<P> * (2 * pitch + v_pitch(warps)) * E; }
-    __host__ __device__ static int bytes(int warps) { return 2 * stage(warps) + kTile<P> / kChunk * (int)sizeof(Chunk<P>); }
+    using E = typename P::E;
+    static constexpr int pitch = KP + 8, slots = AHEAD ? 4 : 2, chunks = AHEAD ? 2 : kTile<P> / kChunk;
+    static constexpr int rows = AHEAD ? kChunk : kTile<P>;  // of a slot
+    static constexpr int most = MT == 2 ? 2 : 4;            // warps that solve
+    static constexpr int threads = 32 * (most + (AHEAD ? 2 : 0));
+    __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (sizeof(E) == 2 ? 8 : 4); }
+    __host__ __device__ static int slot(int warps) { return rows * (2 * pitch + v_pitch(warps)) * (int)sizeof(E); }
+    __host__ __device__ static int bytes(int warps) { return slots * slot(warps) + chunks * (int)sizeof(Chunk<P>); }
 };
 
 // A chunk that holds infinities or NaN, token by token: within the products a token meets every other one, if only as 0
@@ -50,7 +53,7 @@ __device__ __noinline__ void odd_chunk(const Forward &f, float *S, const typenam
                 }
             for (int o = 1; o < 4; o *= 2)
                 sk += __shfl_xor_sync(~0u, sk, o), sq += __shfl_xor_sync(~0u, sq, o), kq += __shfl_xor_sync(~0u, kq, o);
-            const float r = to_float(V[i * vp + v]) - sk, u = gate.b * r;
+            const float r = to_float(V[i * vp + v - v0]) - sk, u = gate.b * r;
             for (int j = 0; j < KP / 8; ++j)
                 for (int e = 0; e < 2; ++e) s[4 * j + e] += to_float(K[i * (KP + 8) + 8 * j + 2 * t + e]) * u;
             if (t == 0 && v < d.value_dim) {
@@ -63,70 +66,70 @@ __device__ __noinline__ void odd_chunk(const Forward &f, float *S, const typenam
     }
 }
 
-template <class T, class P, int KP, int MT>
-__global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 : 1) goib2d_delta_forward_kernel(const __grid_constant__ Forward f) {
-    using L = Layout<P, KP, MT>;
+template <class T, class P, int KP, int MT, bool AHEAD>
+__global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 : KP == 128 ? 3 : MT == 2 ? 6 : 3)
+    goib2d_delta_forward_kernel(const __grid_constant__ Forward f) {
+    using L = Layout<P, KP, MT, AHEAD>;
     using E = typename P::E;
-    constexpr int KT = KP / 16, TILE = kTile<P>;
+    constexpr int KT = KP / 16;
     constexpr bool half = sizeof(E) == 2;
     extern __shared__ __align__(16) char sm[];
     const goib2d_delta_desc &d = f.d;
-    const int K = d.key_dim, V = d.value_dim, threads = blockDim.x, warps = threads / 32;
-    const int tid = threadIdx.x, w = tid / 32, lane = tid % 32, t = lane & 3;
-    const int64_t nh = blockIdx.x, n = nh / d.heads, steps = d.n_steps;
+    const int K = d.key_dim, V = d.value_dim, w = threadIdx.x / 32, lane = threadIdx.x % 32, t = lane & 3;
+    const int warps = blockDim.x / 32 - (AHEAD ? 2 : 0), threads = blockDim.x;
+    const int64_t nh = blockIdx.x, n = nh / d.heads;
+    const int steps = (int)d.n_steps, count = (steps + kChunk - 1) / kChunk;
     const int h = (int)(nh - n * d.heads), hk = h / (d.heads / d.key_heads);
-    const int stage = L::stage(warps), vp = L::v_pitch(warps), v0 = w * 16 * MT;
-    Chunk<P> *chunks = (Chunk<P> *)(sm + 2 * stage);
+    const int slot = L::slot(warps), vp = L::v_pitch(warps), block0 = blockIdx.y * warps * 16 * MT;
+    Chunk<P> *chunks = (Chunk<P> *)(sm + L::slots * slot);
+    const T *const q = row<T>(d.q, d.q_stride, n, 0, hk), *const k = row<T>(d.k, d.k_stride, n, 0, hk);
+    const T *const v = row<T>(d.v, d.v_stride, n, 0, h) + block0;
+    const int qs = (int)d.q_stride[1], ks = (int)d.k_stride[1], vs = (int)d.v_stride[1];
+    const Gates<T> gates(d, n, h);
 
-    float S[MT][KP / 8][4];  // S^T: rows v, columns k
-    load_state<MT, KP>(S, d.state_in ? d.state_in + nh * K * V : nullptr, K, V, v0, lane);
-
-    const T *q0 = row<T>(d.q, d.q_stride, n, 0, hk), *k0 = row<T>(d.k, d.k_stride, n, 0, hk);
-    const T *v_0 = row<T>(d.v, d.v_stride, n, 0, h);
-    auto load = [&](int64_t tile) {
-        E *Q = (E *)(sm + (int)(tile & 1) * stage), *Kb = Q + TILE * L::pitch, *Vb = Kb + TILE * L::pitch;
-        const int64_t at = tile * TILE;
-        const int left = (int)(steps - at < TILE ? steps - at : TILE);
-        load_rows(Q, L::pitch, q0 + at * d.q_stride[1], d.q_stride[1], left, TILE, K, KP, f.wide_q, tid, threads);
-        load_rows(Kb, L::pitch, k0 + at * d.k_stride[1], d.k_stride[1], left, TILE, K, KP, f.wide_k, tid, threads);
-        load_rows(Vb, vp, v_0 + at * d.v_stride[1], d.v_stride[1], left, TILE, V, warps * 16 * MT, f.wide_v, tid, threads);
-        cp_commit();
-    };
-    const int64_t tiles = (steps + TILE - 1) / TILE;
-    if (tiles) load(0);
-    Gate gate[TILE / kChunk];
-    auto gates = [&](int64_t tile) {
-#pragma unroll
-        for (int s = 0; s < TILE / kChunk; ++s)
-            if ((tile * (TILE / kChunk) + s) % warps == w) gate[s] = load_gate<T>(d, n, tile * TILE + s * kChunk + (lane & 15), h);
-    };
-    gates(0);
-    for (int64_t tile = 0; tile < tiles; ++tile) {
-        const E *Q = (const E *)(sm + (int)(tile & 1) * stage), *Kb = Q + TILE * L::pitch;
-        E *Vb = (E *)(Kb + TILE * L::pitch);
-        cp_wait<0>();
-        __syncthreads();
-        if (tile + 1 < tiles) load(tile + 1);
-#pragma unroll
-        for (int s = 0; s < TILE / kChunk; ++s)
-            if ((tile * (TILE / kChunk) + s) % warps == w)
-                prepare<P, KP, false>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
-                                      d.scale, lane);
-        if (tile + 1 < tiles) gates(tile + 1);
-        __syncthreads();
-        if (f.kept && tile * TILE % f.keep == 0) {
-            const int64_t at = nh * ((steps + f.keep - 1) / f.keep) + tile * TILE / f.keep;
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-                if (w * MT + m < f.tiles_v) keep_state<KT>((E *)f.kept + (at * f.tiles_v + w * MT + m) * 16 * KP, S[m], lane);
+    if (AHEAD && w >= warps) {
+        // every second chunk; two slots of rows and one chunk's matrices are this warp's
+        const int me = w - warps;
+        auto load = [&](int i) {
+            const int at = i * kChunk, left = steps - at;
+            if (left > 0) {
+                E *Q = (E *)(sm + (i & 3) * slot), *Kb = Q + kChunk * L::pitch, *Vb = Kb + kChunk * L::pitch;
+                chunk_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, K, KP, f.wide_q, lane);
+                chunk_rows(Kb, L::pitch, k + (int64_t)at * ks, ks, left, K, KP, f.wide_k, lane);
+                chunk_rows(Vb, vp, v + (int64_t)at * vs, vs, left, V - block0, warps * 16 * MT, f.wide_v, lane);
+            }
+            cp_commit();
+        };
+        load(me);
+        Gate next = gates.at(me * kChunk + (lane & 15));
+        for (int i = me; i < count; i += 2) {
+            if (i >= 2) bar_wait(3 + me, 32 + 32 * warps);  // chunk i - 2 is solved: its slot and its matrices are free
+            load(i + 2);
+            const Gate gate = next;
+            next = gates.at((i + 2) * kChunk + (lane & 15));
+            cp_wait<1>();
+            __syncwarp();
+            const E *Q = (const E *)(sm + (i & 3) * slot);
+            prepare<P, KP, false>(chunks[me], Q, Q + kChunk * L::pitch, L::pitch, gate, d.scale, lane);
+            __threadfence_block();
+            bar_arrive(1 + me, 32 + 32 * warps);
         }
-#pragma unroll 1
-        for (int s = 0; s < TILE / kChunk; ++s) {
-            const int64_t at = tile * TILE + s * kChunk;
-            if (at >= steps) break;
-            const Chunk<P> &c = chunks[s];
-            const E *Qs = Q + s * kChunk * L::pitch, *Ks = Kb + s * kChunk * L::pitch;
-            E *Vs = Vb + s * kChunk * vp;
+        return;
+    }
+
+    const int v0 = w * 16 * MT, tile0 = block0 / 16 + w * MT;  // columns within the block; the first tile of V
+    float S[MT][KP / 8][4];  // S^T: rows v, columns k
+    load_state<MT, KP>(S, d.state_in ? d.state_in + nh * K * V : nullptr, K, V, block0 + v0, lane);
+    T *const out = row<T>(d.out, d.out_stride, n, 0, h) + block0;
+    E *const r = f.r ? (E *)f.r + nh * steps * V + block0 : nullptr;
+    const int os = (int)d.out_stride[1];
+    auto solve = [&](int at, const E *Qs, const E *Ks, E *Vs, const Chunk<P> &c) {
+            if (f.kept && at % f.keep == 0) {
+                const int64_t x = (nh * ((steps + f.keep - 1) / f.keep) + at / f.keep) * f.tiles_v + tile0;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+                    if (tile0 + m < f.tiles_v) keep_state<KT>((E *)f.kept + (x + m) * 16 * KP, S[m], lane);
+            }
             const uint32_t tokens = steps - at < kChunk ? (1u << (steps - at)) - 1 : 0xffffu;
             float Y[MT][2][4] = {}, O[MT][2][4] = {};
 #pragma unroll
@@ -164,18 +167,18 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 :
                 float s[MT * (KP / 8) * 4];
 #pragma unroll
                 for (int i = 0; i < MT * (KP / 8) * 4; ++i) s[i] = S[i / (KP / 2)][i / 4 % (KP / 8)][i % 4];
-                odd_chunk<T, P, KP, MT>(f, s, Qs, Ks, Vs, vp, n, h, at, v0, lane);
+                odd_chunk<T, P, KP, MT>(f, s, Qs, Ks, Vs + v0, vp, n, h, at, block0 + v0, lane);
 #pragma unroll
                 for (int i = 0; i < MT * (KP / 8) * 4; ++i) S[i / (KP / 2)][i / 4 % (KP / 8)][i % 4] = s[i];
-                continue;
+                return;
             }
-            if (f.r) {
-                E *to = (E *)f.r + (nh * steps + at) * V;
+            if (r) {
+                E *to = r + (int64_t)at * V;
                 if (half)
-                    store_rows<MT>((bf16 *)to, V, tokens, v0, V, f.wide_r, (bf16 *)Vs, vp, Y, lane);
+                    store_rows<MT>((bf16 *)to, V, tokens, v0, V - block0, f.wide_r, (bf16 *)Vs, vp, Y, lane);
                 else
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) store_direct<E>(to, V, tokens, v0 + 16 * m, V, Y[m], lane);
+                    for (int m = 0; m < MT; ++m) store_direct<E>(to, V, tokens, v0 + 16 * m, V - block0, Y[m], lane);
             }
             typename P::A2 u[MT];
             {
@@ -190,12 +193,12 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 :
                     u[m] = P::exact(Y[m][0], Y[m][1]);
                 }
             }
-            T *to = row<T>(d.out, d.out_stride, n, at, h);
+            T *to = out + (int64_t)at * os;
             if (half)
-                store_rows<MT>((bf16 *)to, d.out_stride[1], tokens, v0, V, f.wide_o, (bf16 *)Vs, vp, O, lane);
+                store_rows<MT>((bf16 *)to, os, tokens, v0, V - block0, f.wide_o, (bf16 *)Vs, vp, O, lane);
             else
 #pragma unroll
-                for (int m = 0; m < MT; ++m) store_direct<T>(to, d.out_stride[1], tokens, v0 + 16 * m, V, O[m], lane);
+                for (int m = 0; m < MT; ++m) store_direct<T>(to, os, tokens, v0 + 16 * m, V - block0, O[m], lane);
             const float a_end = c.a_end;
 #pragma unroll
             for (int j = 0; j < KT; ++j) {
@@ -208,24 +211,72 @@ __global__ void __launch_bounds__(MT == 2 ? 128 : 256, MT == 2 && KP <= 64 ? 3 :
                     P::mul(c0, c1, u[m], kb);
                 }
             }
+    };
+    if constexpr (AHEAD) {
+#pragma unroll 1
+        for (int i = 0; i < count; ++i) {
+            E *Q = (E *)(sm + (i & 3) * slot);
+            bar_wait(1 + (i & 1), 32 + 32 * warps);
+            solve(i * kChunk, Q, Q + kChunk * L::pitch, Q + 2 * kChunk * L::pitch, chunks[i & 1]);
+            if (i + 2 < count) bar_arrive(3 + (i & 1), 32 + 32 * warps);
+        }
+    } else {
+        constexpr int TILE = kTile<P>, N = TILE / kChunk;
+        const int tiles = (steps + TILE - 1) / TILE;
+        auto load = [&](int tile) {
+            E *Q = (E *)(sm + (tile & 1) * slot), *Kb = Q + TILE * L::pitch, *Vb = Kb + TILE * L::pitch;
+            const int at = tile * TILE, left = steps - at < TILE ? steps - at : TILE;
+            load_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, TILE, K, KP, f.wide_q, threadIdx.x, threads);
+            load_rows(Kb, L::pitch, k + (int64_t)at * ks, ks, left, TILE, K, KP, f.wide_k, threadIdx.x, threads);
+            load_rows(Vb, vp, v + (int64_t)at * vs, vs, left, TILE, V - block0, warps * 16 * MT, f.wide_v, threadIdx.x, threads);
+            cp_commit();
+        };
+        Gate gate[N];
+        auto gates_of = [&](int tile) {
+#pragma unroll
+            for (int s = 0; s < N; ++s)
+                if ((tile * N + s) % warps == w) gate[s] = gates.at(tile * TILE + s * kChunk + (lane & 15));
+        };
+        if (tiles) load(0), gates_of(0);
+#pragma unroll 1
+        for (int tile = 0; tile < tiles; ++tile) {
+            E *Q = (E *)(sm + (tile & 1) * slot), *Kb = Q + TILE * L::pitch, *Vb = Kb + TILE * L::pitch;
+            cp_wait<0>();
+            __syncthreads();
+            if (tile + 1 < tiles) load(tile + 1);
+#pragma unroll
+            for (int s = 0; s < N; ++s)
+                if ((tile * N + s) % warps == w)
+                    prepare<P, KP, false>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
+                                          d.scale, lane);
+            if (tile + 1 < tiles) gates_of(tile + 1);
+            __syncthreads();
+#pragma unroll 1
+            for (int s = 0; s < N && tile * TILE + s * kChunk < steps; ++s)
+                solve(tile * TILE + s * kChunk, Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, Vb + s * kChunk * vp,
+                      chunks[s]);
         }
     }
-    store_state<MT, KP>(d.state_out + nh * K * V, S, K, V, v0, lane);
+    store_state<MT, KP>(d.state_out + nh * K * V, S, K, V, block0 + v0, lane);
 }
 
-template <class T, class P, int KP, int MT>
-cudaError_t forward_of(const Forward &f, cudaStream_t s) {
-    const int warps = (f.d.value_dim + 16 * MT - 1) / (16 * MT);
-    const size_t smem = Layout<P, KP, MT>::bytes(warps);
-    cudaError_t e = allow_smem(goib2d_delta_forward_kernel<T, P, KP, MT>, smem);
+template <class T, class P, int KP, int MT, bool AHEAD>
+cudaError_t forward_of(const Forward &f, const Split &b, cudaStream_t s) {
+    const size_t smem = Layout<P, KP, MT, AHEAD>::bytes(b.warps);
+    cudaError_t e = allow_smem(goib2d_delta_forward_kernel<T, P, KP, MT, AHEAD>, smem);
     if (e != cudaSuccess) return e;
-    goib2d_delta_forward_kernel<T, P, KP, MT><<<(unsigned)(f.d.n_worlds * f.d.heads), 32 * warps, smem, s>>>(f);
+    goib2d_delta_forward_kernel<T, P, KP, MT, AHEAD>
+        <<<dim3((unsigned)(f.d.n_worlds * f.d.heads), b.blocks), 32 * (b.warps + (AHEAD ? 2 : 0)), smem, s>>>(f);
     return cudaGetLastError();
 }
 
 template <class T, class P, int KP>
 cudaError_t forward_wide(const Forward &f, cudaStream_t s) {
-    return f.d.value_dim <= 16 ? forward_of<T, P, KP, 1>(f, s) : forward_of<T, P, KP, 2>(f, s);
+    const Split b(f.d);
+    if (b.ahead) return forward_of<T, P, KP, 1, true>(f, b, s);
+    if constexpr (KP < 128)
+        if (b.MT == 2) return forward_of<T, P, KP, 2, false>(f, b, s);
+    return forward_of<T, P, KP, 1, false>(f, b, s);
 }
 
 template <class T, class P>
@@ -240,7 +291,6 @@ cudaError_t forward_typed(const goib2d_delta_desc &d, void *saved, cudaStream_t 
     f.wide_o = rows_aligned(d.out, d.out_stride, d.n_worlds, d.n_steps, d.heads, V, z);
     f.wide_r = V % 8 == 0;
     switch (padded_keys(d.key_dim)) {
-        case 16: return forward_wide<T, P, 16>(f, s);
         case 32: return forward_wide<T, P, 32>(f, s);
         case 64: return forward_wide<T, P, 64>(f, s);
         default: return forward_wide<T, P, 128>(f, s);

@@ -74,7 +74,10 @@ def off(got, want):
 SIZES = [(1, 1, 1, 1, 1, 1), (2, 1, 2, 1, 3, 5), (3, 2, 2, 2, 16, 16), (2, 15, 2, 2, 32, 32), (3, 16, 3, 1, 64, 64),
          (2, 17, 4, 2, 64, 32), (1, 31, 1, 1, 32, 64), (5, 33, 6, 3, 40, 71), (2, 64, 2, 1, 128, 128),
          (1, 65, 2, 2, 100, 128), (2, 130, 1, 1, 8, 128), (1, 129, 2, 1, 128, 8), (1, 600, 1, 1, 48, 24),
-         (40, 20, 4, 4, 64, 64)]
+         (40, 20, 4, 4, 64, 64),
+         # as many (worlds, heads) as fill the GPU
+         (300, 17, 1, 1, 20, 10), (110, 50, 3, 3, 32, 64), (80, 70, 4, 2, 64, 64), (301, 35, 1, 1, 100, 65),
+         (150, 33, 2, 1, 128, 128)]
 
 
 @pytest.mark.gpu
@@ -219,12 +222,13 @@ def test_broadcast_inputs_and_gradients():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [4, 160])  # few and many worlds
 @pytest.mark.parametrize("K,V", [(16, 16), (64, 64), (40, 71), (128, 128)])
-def test_states_that_start_afresh(K, V, dtype):
+def test_states_that_start_afresh(K, V, n, dtype):
     """A reset, a decay of -inf, of the type's lowest value and of -200 all empty the memory, whatever it held:
     infinities and NaN in the old state are not read. Every token of world 0 is a reset (its own write is all that
     its query sees)."""
-    n, t, h = 4, 40, 2
+    t, h = 40, 2
     a = rollout(n, t, h, h, K, V, dtype, seed=1, resets=False)
     reset = torch.zeros(n, t, dtype=torch.bool, device="cuda")
     reset[0] = True
@@ -256,11 +260,12 @@ def test_states_that_start_afresh(K, V, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("n", [6, 300])  # few and many worlds
 @pytest.mark.parametrize("V", [16, 40, 64])
-def test_a_world_recovers_from_values_that_are_not_finite(V, dtype, bad):
+def test_a_world_recovers_from_values_that_are_not_finite(V, n, dtype, bad):
     """A world whose simulation blew up sends NaN or infinities until it is reset: what comes after the reset, in the
     same chunk of tokens or later, is as if the memory had been empty, and other worlds do not notice."""
-    n, t, h, K = 6, 70, 2, 32
+    t, h, K = 70, 2, 32
     a = rollout(n, t, h, 1, K, V, dtype, seed=13, resets=False)
     reset = torch.zeros(n, t, dtype=torch.bool, device="cuda")
     spoilt = torch.zeros(n, t, dtype=torch.bool, device="cuda")
