@@ -1111,13 +1111,16 @@ int goib2d_clip_grads(const goib2d_grad *grads, int32_t n, float max_norm, float
     if (n < 0 || (n && !grads)) return fail(GOIB2D_EINVAL, "bad gradient table");
     if (!(max_norm >= 0.0f)) return fail(GOIB2D_EINVAL, "max_norm %g", (double)max_norm);
     if (!workspace || (uintptr_t)workspace % 16) return fail(GOIB2D_EINVAL, "workspace is null or not 16-byte aligned");
+    int64_t pieces = 0;  // of 16 KB
     for (int32_t i = 0; i < n; ++i) {
         const goib2d_grad &g = grads[i];
         if (g.dtype != GOIB2D_FLOAT32 && g.dtype != GOIB2D_BFLOAT16) return fail(GOIB2D_EINVAL, "tensor %d: dtype %d", i, g.dtype);
         if (g.numel < 0 || g.numel >> 48) return fail(GOIB2D_EINVAL, "tensor %d: %lld elements", i, (long long)g.numel);
+        pieces += g.numel / 4096 + 1;
         if (g.numel && (!g.data || (uintptr_t)g.data % (g.dtype == GOIB2D_BFLOAT16 ? 2 : 4)))
             return fail(GOIB2D_EINVAL, "tensor %d: null or misaligned data", i);
     }
+    if (pieces > INT32_MAX / 4) return fail(GOIB2D_ELIMIT, "too many elements");
     CUDA_TRY(gb::launch_clip(grads, n, max_norm, norm, workspace, (cudaStream_t)stream));
     return 0;
 }

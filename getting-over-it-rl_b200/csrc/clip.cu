@@ -1,137 +1,262 @@
 // Gradient clipping by the global norm over many tensors (goib2d_clip_grads): norm = sqrt(sum of squares of every
 // element of every tensor), then every element times min(1, max_norm / (norm + 1e-6)).
 //
-// The tensor table travels in the launch's parameters, so a call makes no copy and keeps nothing. Squares are summed
-// in float64: no overflow or underflow of a square in float32's range, and 5.8 conversions and multiply-adds per clock and SM at the
-// full HBM rate are far below what the SM does. Every block's sum goes to its own place and every block adds all of them in
-// one order: the same inputs give the same bits.
+// Bound by the bytes: each element read and written once where the SMs can hold it in between. One launch: a block of
+// an SM sums the squares of its tiles of 16 KB and keeps the first kKept of them in shared memory (28 MB on all SMs), the
+// grid meets, and every block scales what it kept and then its other tiles, the last read first, which the L2 cache still
+// holds some 100 MB of. The tensor table travels in the launch's parameters: a call makes no copy and keeps nothing.
+// Squares are summed in float32 over a thread's 16 bytes, and from there on in float64; where such a sum leaves the
+// range in which float32 carries it, in float64 from the squares on. Every block's sum goes to its own place and every
+// block adds all of them in one order: the same inputs give the same bits.
+#include <cooperative_groups.h>
+
 #include "policy.cuh"
 
 namespace gb {
 namespace {
 
-constexpr int kTable = 1024;        // tensors per launch: 24 KB of the 32 KB of launch parameters
-constexpr int kTile = 4096;         // elements of one block's turn
-constexpr int kThreads = 256;
-constexpr int kBlocks = 148 * 4;    // partial sums per launch
+constexpr int kThreads = 1024;
+constexpr int kBytes = kThreads * 16;  // of a tile
+constexpr int kKept = 12;              // tiles of a block that stay in shared memory
+constexpr int kBatch = 4;              // tiles whose loads are in flight together
+constexpr int kSms = 148;
+constexpr int kMost = 1024;            // tensors of a launch: 20 KB of its 32 KB of parameters
 
+enum { kSum = 1, kScale = 2 };
+
+template <int N>
 struct Table {
-    int32_t n;                      // tensors
-    int32_t first;                  // where this launch's partial sums go
-    int32_t sums;                   // partial sums of all launches (clip)
+    int32_t n, mode;
+    int32_t first, sums;               // where this launch's partial sums go; how many there are in all
     float max_norm;
     float *norm;
     double *part;
-    void *ptr[kTable];
-    int64_t end[kTable];            // (tiles up to and with this tensor) << 1 | bfloat16
-    int64_t numel[kTable];
+    void *ptr[N];
+    int32_t end[N];                    // (tiles up to and with this tensor) << 1 | bfloat16
+    int64_t numel[N];
 };
 
-// The tensor of tile t, and the tile's place in it.
-__device__ __forceinline__ int find(const Table &T, int64_t t, int64_t &at) {
-    int lo = 0, hi = T.n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (t < (T.end[mid] >> 1)) hi = mid;
-        else lo = mid + 1;
+// A thread's 16 bytes of a tile. Aligned tensors: neighbouring elements; others: elements kThreads apart. `left`: elements
+// of the tensor from its first one on (many, where the tile is whole).
+struct Piece {
+    char *p;
+    int64_t left;
+    bool half, wide;
+};
+
+// The tensor that the last tile asked for is of: tiles lo to hi - 1.
+template <int N>
+struct Cursor {
+    const Table<N> &T;
+    int i = 0, lo = 0, hi;
+    char *base;
+    bool half, wide;
+    __device__ __forceinline__ void tensor() {
+        lo = i ? T.end[i - 1] >> 1 : 0, hi = T.end[i] >> 1, half = T.end[i] & 1, wide = (uintptr_t)T.ptr[i] % 16 == 0;
+        base = (char *)T.ptr[i] + threadIdx.x * (wide ? 16 : half ? 2 : 4);
     }
-    at = (t - (lo ? T.end[lo - 1] >> 1 : 0)) * kTile;
-    return lo;
+    __device__ __forceinline__ explicit Cursor(const Table<N> &T) : T(T) { tensor(); }
+    __device__ __forceinline__ Piece at(int t) {
+        if (t < lo || t >= hi) {
+            while (t >= T.end[i] >> 1) ++i;
+            while (i > 0 && t < T.end[i - 1] >> 1) --i;
+            tensor();
+        }
+        Piece x{base + (int64_t)(t - lo) * kBytes, 1 << 30, half, wide};
+        if (t + 1 == hi) {
+            const int size = half ? 2 : 4;
+            x.left = T.numel[i] - (int64_t)(t - lo) * (kBytes / size) - threadIdx.x * (wide ? 16 / size : 1);
+        }
+        return x;
+    }
+};
+
+__device__ __forceinline__ uint4 load(const Piece &x) {
+    const int n = x.half ? 8 : 4;
+    if (x.wide && x.left >= n) return *(const uint4 *)x.p;
+    uint32_t v[4] = {};
+    const int64_t step = x.wide ? 1 : kThreads;
+    if (x.half) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e * step < x.left) v[e / 2] |= (uint32_t)((const uint16_t *)x.p)[e * step] << e % 2 * 16;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e * step < x.left) v[e] = ((const uint32_t *)x.p)[e * step];
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+__device__ __forceinline__ void store(const Piece &x, uint4 y) {
+    const int n = x.half ? 8 : 4;
+    if (x.wide && x.left >= n) {
+        __stcs((uint4 *)x.p, y);
+        return;
+    }
+    const uint32_t v[4] = {y.x, y.y, y.z, y.w};
+    const int64_t step = x.wide ? 1 : kThreads;
+    if (x.half) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e * step < x.left) ((uint16_t *)x.p)[e * step] = (uint16_t)(v[e / 2] >> e % 2 * 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (e * step < x.left) ((uint32_t *)x.p)[e * step] = v[e];
+    }
+}
+
+__device__ __forceinline__ void values(float (&f)[8], uint4 y, bool half) {
+    const uint32_t v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        f[e] = __uint_as_float(half ? v[e] << 16 : v[e]);
+        f[4 + e] = half ? __uint_as_float(v[e] & 0xffff0000u) : 0.0f;
+    }
+}
+
+__device__ __forceinline__ double squares(uint4 y, bool half) {
+    float f[8], s = 0.0f;
+    values(f, y, half);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(f[e], f[e], s);
+    if (s >= 1e-20f && s <= 1e30f) return s;
+    double d = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d += (double)f[e] * f[e];
+    return d;
+}
+
+__device__ __forceinline__ uint4 scaled(uint4 y, bool half, float c) {
+    float f[8];
+    values(f, y, half);
+    uint32_t v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (half) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(f[e] * c, f[4 + e] * c);
+            v[e] = *(const uint32_t *)&b;
+        } else {
+            v[e] = __float_as_uint(f[e] * c);
+        }
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 __device__ __forceinline__ double block_sum(double x) {
     __shared__ double warp[kThreads / 32];
+    __syncthreads();
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
     if (threadIdx.x % 32 == 0) warp[threadIdx.x / 32] = x;
     __syncthreads();
-    x = 0.0;
-    for (int i = 0; i < kThreads / 32; ++i) x += warp[i];
+    x = warp[threadIdx.x % 32];
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(~0u, x, o);
     return x;
 }
 
-__global__ void __launch_bounds__(kThreads) goib2d_grad_norm_kernel(const __grid_constant__ Table T) {
-    const int64_t tiles = T.end[T.n - 1] >> 1;
-    double sum = 0.0;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        int64_t at;
-        const int i = find(T, t, at);
-        const int64_t stop = at + kTile < T.numel[i] ? at + kTile : T.numel[i];
-        if (T.end[i] & 1) {
-            const __nv_bfloat16 *x = (const __nv_bfloat16 *)T.ptr[i];
-            for (int64_t j = at + threadIdx.x; j < stop; j += kThreads) {
-                const double y = __bfloat162float(x[j]);
-                sum += y * y;
+template <int N>
+__global__ void __launch_bounds__(kThreads) goib2d_clip_kernel(const __grid_constant__ Table<N> T) {
+    extern __shared__ uint4 kept[];
+    const int tiles = T.n ? T.end[T.n - 1] >> 1 : 0, grid = gridDim.x;
+    Cursor<N> cursor(T);
+    if (T.mode & kSum) {
+        double sum = 0.0;
+        for (int k = 0, t0 = blockIdx.x; t0 < tiles; k += kBatch, t0 += kBatch * grid) {
+            uint4 y[kBatch];
+            bool half[kBatch];
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                const int t = t0 + e * grid;
+                y[e] = make_uint4(0, 0, 0, 0), half[e] = false;
+                if (t < tiles) {
+                    const Piece x = cursor.at(t);
+                    y[e] = load(x), half[e] = x.half;
+                }
             }
-        } else {
-            const float *x = (const float *)T.ptr[i];
-            for (int64_t j = at + threadIdx.x; j < stop; j += kThreads) {
-                const double y = x[j];
-                sum += y * y;
+#pragma unroll
+            for (int e = 0; e < kBatch; ++e) {
+                if (k + e < kKept) kept[(k + e) * kThreads + threadIdx.x] = y[e];
+                sum += squares(y[e], half[e]);
             }
         }
+        sum = block_sum(sum);
+        if (threadIdx.x == 0) T.part[T.first + blockIdx.x] = sum;
+        if (!(T.mode & kScale)) return;
+        cooperative_groups::this_grid().sync();
     }
-    sum = block_sum(sum);
-    if (threadIdx.x == 0) T.part[T.first + blockIdx.x] = sum;
-}
-
-__global__ void __launch_bounds__(kThreads) goib2d_grad_clip_kernel(const __grid_constant__ Table T) {
     double sum = 0.0;
-    for (int i = threadIdx.x; i < T.sums; i += kThreads) sum += T.part[i];
+    for (int j = threadIdx.x; j < T.sums; j += kThreads) sum += T.part[j];
     const float norm = (float)sqrt(block_sum(sum));
     if (T.norm && blockIdx.x == 0 && threadIdx.x == 0) *T.norm = norm;
     const float c = T.max_norm / (norm + 1e-6f);
-    if (c >= 1.0f || T.n == 0) return;  // NaN goes on: every element becomes NaN
-    const int64_t tiles = T.end[T.n - 1] >> 1;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        int64_t at;
-        const int i = find(T, t, at);
-        const int64_t stop = at + kTile < T.numel[i] ? at + kTile : T.numel[i];
-        if (T.end[i] & 1) {
-            __nv_bfloat16 *x = (__nv_bfloat16 *)T.ptr[i];
-            for (int64_t j = at + threadIdx.x; j < stop; j += kThreads)
-                x[j] = __float2bfloat16_rn(__bfloat162float(x[j]) * c);
-        } else {
-            float *x = (float *)T.ptr[i];
-            for (int64_t j = at + threadIdx.x; j < stop; j += kThreads) x[j] *= c;
-        }
+    if (c >= 1.0f) return;  // NaN goes on: every element becomes NaN
+    const int mine = (tiles - (int)blockIdx.x + grid - 1) / grid;  // tiles of this block
+    const int held = T.mode & kSum ? (mine < kKept ? mine : kKept) : 0;
+    for (int k = mine - 1; k >= held; k -= kBatch) {
+        uint4 y[kBatch];
+        Piece x[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+            if (k - e >= held) x[e] = cursor.at(blockIdx.x + (k - e) * grid), y[e] = load(x[e]);
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+            if (k - e >= held) store(x[e], scaled(y[e], x[e].half, c));
+    }
+    for (int k = held - 1; k >= 0; --k) {
+        const Piece x = cursor.at(blockIdx.x + k * grid);
+        store(x, scaled(kept[k * kThreads + threadIdx.x], x.half, c));
     }
 }
 
-int launches(int32_t n) { return n ? (n + kTable - 1) / kTable : 1; }
+int launches(int32_t n) { return n ? (n + kMost - 1) / kMost : 1; }
 
-}  // namespace
-
-int64_t clip_workspace_bytes(const goib2d_grad *, int32_t n) { return (int64_t)sizeof(double) * kBlocks * launches(n); }
-
-cudaError_t launch_clip(const goib2d_grad *grads, int32_t n, float max_norm, float *norm, void *workspace,
-                        cudaStream_t s) {
-    Table T;
-    T.max_norm = max_norm, T.part = (double *)workspace;
-    for (int pass = 0; pass < 2; ++pass) {
-        T.sums = pass ? T.first : 0;
-        T.first = 0, T.norm = pass ? norm : nullptr;
-        for (int32_t from = 0; from == 0 || from < n; from += kTable) {
-            T.n = n - from < kTable ? n - from : kTable;
+template <int N>
+cudaError_t clip_tables(const goib2d_grad *grads, int32_t n, float max_norm, float *norm, double *part, cudaStream_t s) {
+    const size_t smem = (size_t)kKept * kBytes;
+    cudaError_t e = cudaFuncSetAttribute(goib2d_clip_kernel<N>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    int sms = 0, dev = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    sms = sms < kSms ? sms : kSms;
+    Table<N> T;
+    T.max_norm = max_norm, T.part = part, T.first = 0;
+    const bool one = n <= N;
+    for (int mode = one ? kSum | kScale : kSum; mode <= (kSum | kScale); mode = mode == kSum ? kScale : 4) {
+        if (mode == kScale) T.sums = T.first;
+        T.mode = mode, T.norm = mode & kScale ? norm : nullptr;
+        for (int32_t from = 0; from == 0 || from < n; from += N) {
+            T.n = n - from < N ? n - from : N;
             int64_t tiles = 0;
             for (int i = 0; i < T.n; ++i) {
                 const goib2d_grad &g = grads[from + i];
-                tiles += (g.numel + kTile - 1) / kTile;
+                const int64_t elements = kBytes / (g.dtype == GOIB2D_BFLOAT16 ? 2 : 4);
+                tiles += (g.numel + elements - 1) / elements;
                 T.ptr[i] = g.data, T.numel[i] = g.numel;
-                T.end[i] = tiles << 1 | (g.dtype == GOIB2D_BFLOAT16);
+                T.end[i] = (int32_t)(tiles << 1) | (g.dtype == GOIB2D_BFLOAT16);
             }
-            const int blocks = tiles < kBlocks ? (tiles ? (int)tiles : 1) : kBlocks;
-            if (!pass) {
-                if (tiles) goib2d_grad_norm_kernel<<<blocks, kThreads, 0, s>>>(T);
-                T.first += tiles ? blocks : 0;
-            } else {
-                if (tiles || T.norm) goib2d_grad_clip_kernel<<<blocks, kThreads, 0, s>>>(T);
-                T.norm = nullptr;
-            }
-            const cudaError_t e = cudaGetLastError();
+            const int blocks = tiles < sms ? (tiles ? (int)tiles : 1) : sms;
+            if (one) T.sums = blocks;
+            void *args[] = {&T};
+            e = cudaLaunchCooperativeKernel((const void *)goib2d_clip_kernel<N>, dim3(blocks), dim3(kThreads), args, smem, s);
             if (e != cudaSuccess) return e;
+            if (mode == kSum) T.first += blocks;
+            T.norm = nullptr;
         }
     }
     return cudaSuccess;
+}
+
+}  // namespace
+
+int64_t clip_workspace_bytes(const goib2d_grad *, int32_t n) { return (int64_t)sizeof(double) * kSms * launches(n); }
+
+cudaError_t launch_clip(const goib2d_grad *grads, int32_t n, float max_norm, float *norm, void *workspace,
+                        cudaStream_t s) {
+    // the table is copied with the launch: a small one for few tensors
+    return n <= 64 ? clip_tables<64>(grads, n, max_norm, norm, (double *)workspace, s)
+                   : clip_tables<kMost>(grads, n, max_norm, norm, (double *)workspace, s);
 }
 
 }  // namespace gb

@@ -239,19 +239,24 @@ def clip_grads_(grads, max_norm):
     device = grads[0].device
     if device.type != "cuda":
         raise TypeError("gradients must be CUDA tensors")
-    table = array("q")
-    for x in grads:
-        dt = _DTYPE.get(x.dtype)
-        if dt is None or x.device != device or x.layout is not torch.strided:
-            raise ValueError(f"gradients must be dense float32 or bfloat16 tensors on {device}, got {x.dtype} on {x.device}")
-        if not (x.is_contiguous() or _dense(x)):
-            raise ValueError(f"a gradient of shape {tuple(x.shape)} and strides {x.stride()} is not dense in memory")
-        n = x.numel()
-        if n:
-            table.extend((x.data_ptr(), n, dt))
-    count = len(table) // 3
-    if len(set(table[::3])) != count:
+    index = device.index
+    if not (all(x.get_device() == index and x.layout is torch.strided and x.dtype in _DTYPE for x in grads) and
+            all(x.is_contiguous() or _dense(x) for x in grads)):
+        for x in grads:
+            if x.get_device() != index or x.layout is not torch.strided or x.dtype not in _DTYPE:
+                raise ValueError(f"gradients must be dense float32 or bfloat16 tensors on {device}, got {x.dtype} on "
+                                 f"{x.device} ({x.layout})")
+            if not (x.is_contiguous() or _dense(x)):
+                raise ValueError(f"a gradient of shape {tuple(x.shape)} and strides {x.stride()} is not dense in memory")
+    grads = [x for x in grads if x.numel()]
+    count = len(grads)
+    where = [x.data_ptr() for x in grads]
+    if len(set(where)) != count:
         raise ValueError("the same gradient twice")
+    table = array("q", bytes(_GRAD.size * count))
+    table[0::3] = array("q", where)
+    table[1::3] = array("q", [x.numel() for x in grads])
+    table[2::3] = array("q", [_DTYPE[x.dtype] for x in grads])
     packed = table.buffer_info()[0]
     lib = native.load()
     with _on(device):
