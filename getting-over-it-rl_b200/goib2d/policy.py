@@ -18,7 +18,6 @@ path. Calls run on the current stream of the tensors' device and return without 
 """
 import struct
 from array import array
-from contextlib import nullcontext
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -76,11 +75,6 @@ def _sizes(q, v, steps):
     return v.shape[0], v.shape[1] if steps else 1, h, hk, K, V
 
 
-def _on(device):
-    """The device's guard, where it is not the current one (the C calls run on the current device)."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -97,39 +91,61 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     returned. q, k (N, Hk, K), v (N, H, V), g (log decay) and beta (N, H), reset (N,) bool or None; scale defaults
     to K ** -0.5. Inputs may have any strides with contiguous channels. Not differentiable: rollouts train through
     delta_rule."""
-    n, _, h, hk, K, V = _sizes(q, v, False)
+    # everything in one expression first: an acting loop calls this once per world step
     device, dt = v.device, v.dtype
+    vs, qs, ks, gs, bs = v.stride(), q.stride(), k.stride(), g.stride(), beta.stride()
+    if out is None:
+        out = torch.empty_like(v)
+    shape, heads = v.shape, g.shape
+    os_ = out.stride()
+    if not (len(vs) == len(qs) == len(os_) == 3 and q.shape == k.shape and heads == beta.shape and heads == shape[:2] and
+            out.shape == shape and q.shape[0] == shape[0] and state.shape == (*heads, q.shape[2], shape[2]) and
+            vs[2] == qs[2] == ks[2] == os_[2] == 1 and dt in _DTYPE and _alike(dt, device, q, k, g, beta, out) and
+            v.is_cuda and state.dtype is torch.float32 and state.device == device and state.is_contiguous()):
+        _check_step(state, q, k, v, g, beta, out)
+    n, h, V = shape
+    hk, K = q.shape[1:]
+    if not (0 < K <= MAX_DIM and 0 < V <= MAX_DIM and hk > 0 and h > 0 and h % hk == 0):
+        _sizes(q, v, False)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
                                     beta.requires_grad or state.requires_grad):
         raise ValueError("delta_step_ is not differentiable: use delta_rule, or torch.no_grad()")
-    if out is None:
-        out = torch.empty((n, h, V), dtype=dt, device=device)
-    qs, ks, vs, gs, bs, os_ = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride(), out.stride()
-    # all of it in one expression first: an acting loop calls this once per world step
-    if not (_alike(dt, device, q, k, v, g, beta, out) and q.shape == k.shape and q.shape[0] == n and
-            out.shape == v.shape and g.shape == beta.shape == (n, h) and state.shape == (n, h, K, V) and
-            qs[2] == ks[2] == vs[2] == os_[2] == 1 and state.is_contiguous() and
-            _alike(torch.float32, device, state)):
-        _state("state", state, (n, h, K, V), device)
-        for name, x, shape in (("q", q, (n, hk, K)), ("k", k, (n, hk, K)), ("v", v, (n, h, V)), ("out", out, (n, h, V))):
-            _rows(name, x, shape, dt, device)
-        for name, x in (("g", g), ("beta", beta)):
-            _rows(name, x, (n, h), dt, device, False)
-    rp, rs = _reset(reset, (n,), device)
+    rp, rs = (0, (0,)) if reset is None else _reset(reset, (n,), device)
     sp = state.data_ptr()
     desc = _DESC.pack(n, 1, h, hk, K, V, _DTYPE[dt], K ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
                       v.data_ptr(), g.data_ptr(), beta.data_ptr(), rp, sp, sp, out.data_ptr(),
                       qs[0], 0, qs[1], ks[0], 0, ks[1], vs[0], 0, vs[1], gs[0], 0, gs[1], bs[0], 0, bs[1],
                       os_[0], 0, os_[1], rs[0], 0)
-    lib = native.load()
-    with _on(device):
-        native.check(lib.goib2d_delta_step(desc, _raw_stream(device.index)))
+    _call(device, native.load().goib2d_delta_step, desc)
     return out
 
 
-def _describe(q, k, v, g, beta, state, reset, scale, last, out):
+def _check_step(state, q, k, v, g, beta, out):
+    """delta_step_'s refusals, one by one (a channel axis of size 1 may have any stride)."""
+    n, _, h, hk, K, V = _sizes(q, v, False)
+    device, dt = v.device, v.dtype
+    _state("state", state, (n, h, K, V), device)
+    for name, x, shape in (("q", q, (n, hk, K)), ("k", k, (n, hk, K)), ("v", v, (n, h, V)), ("out", out, (n, h, V))):
+        _rows(name, x, shape, dt, device)
+    for name, x in (("g", g), ("beta", beta)):
+        _rows(name, x, (n, h), dt, device, False)
+
+
+def _call(device, function, *args):
+    """A C call on the tensors' device and its current stream (the last argument)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = function(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(device):
+            rc = function(*args, _raw_stream(index))
+    if rc:
+        native.check(rc)
+
+
+def _describe(sizes, q, k, v, g, beta, state, reset, scale, last, out):
     """goib2d_delta_desc of a rollout call."""
-    n, t, h, hk, K, V = _sizes(q, v, True)
+    n, t, h, hk, K, V = sizes
     device, dt = v.device, v.dtype
     qp, qs = _rows("q", q, (n, t, hk, K), dt, device)
     kp, ks = _rows("k", k, (n, t, hk, K), dt, device)
@@ -144,20 +160,18 @@ def _describe(q, k, v, g, beta, state, reset, scale, last, out):
 
 def _forward(q, k, v, g, beta, state, reset, scale, train):
     """(o, last state, what the backward pass keeps or None)."""
-    n, t, h, hk, K, V = _sizes(q, v, True)
+    sizes = n, t, h, hk, K, V = _sizes(q, v, True)
     device = v.device
     lib = native.load()
-    with _on(device):
-        out = torch.empty((n, t, h, V), dtype=v.dtype, device=device)
-        last = torch.empty((n, h, K, V), dtype=torch.float32, device=device)
-        desc = _describe(q, k, v, g, beta, state, reset, scale, last, out)
-        saved = None
-        if train:
-            size = lib.goib2d_delta_saved_bytes(desc)
-            native.check(min(size, 0))
-            saved = torch.empty(size, dtype=torch.uint8, device=device)
-        native.check(lib.goib2d_delta_forward(desc, saved.data_ptr() if train else None,
-                                              _raw_stream(device.index)))
+    out = torch.empty((n, t, h, V), dtype=v.dtype, device=device)
+    last = torch.empty((n, h, K, V), dtype=torch.float32, device=device)
+    desc = _describe(sizes, q, k, v, g, beta, state, reset, scale, last, out)
+    saved = None
+    if train:
+        size = lib.goib2d_delta_saved_bytes(desc)
+        native.check(min(size, 0))
+        saved = torch.empty(size, dtype=torch.uint8, device=device)
+    _call(device, lib.goib2d_delta_forward, desc, saved.data_ptr() if train else None)
     return out, last, saved
 
 
@@ -176,30 +190,28 @@ class _DeltaRule(torch.autograd.Function):
         q, k, v, g, beta, state, reset, last, saved = ctx.saved_tensors
         if dout is None and dlast is None:
             return (None,) * 8
-        n, t, h, hk, K, V = _sizes(q, v, True)
+        sizes = n, t, h, hk, K, V = _sizes(q, v, True)
         device, dt = v.device, v.dtype
         lib = native.load()
-        with _on(device):
-            desc = _describe(q, k, v, g, beta, state, reset, ctx.scale, last, last)
-            dop, dos = 0, (0, 0, 0)
-            if dout is not None:
-                dout = dout if dout.stride(-1) == 1 else dout.contiguous()
-                dop, dos = dout.data_ptr(), dout.stride()[:3]
-            dlast = None if dlast is None else dlast.contiguous()
-            dq, dk = (torch.empty((n, t, hk, K), dtype=dt, device=device) for _ in range(2))
-            dv = torch.empty((n, t, h, V), dtype=dt, device=device)
-            dg, dbeta = (torch.empty((n, t, h), dtype=dt, device=device) for _ in range(2))
-            first = None
-            if state is not None and ctx.needs_input_grad[5]:
-                first = torch.empty((n, h, K, V), dtype=torch.float32, device=device)
-            grads = _GRADS.pack(dop, 0 if dlast is None else dlast.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                                dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), 0 if first is None else first.data_ptr(),
-                                *dos, *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *dg.stride(), *dbeta.stride())
-            size = lib.goib2d_delta_workspace_bytes(desc)
-            native.check(min(size, 0))
-            work = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
-            native.check(lib.goib2d_delta_backward(desc, grads, saved.data_ptr(), work.data_ptr(),
-                                                   _raw_stream(device.index)))
+        desc = _describe(sizes, q, k, v, g, beta, state, reset, ctx.scale, last, last)
+        dop, dos = 0, (0, 0, 0)
+        if dout is not None:
+            dout = dout if dout.stride(-1) == 1 else dout.contiguous()
+            dop, dos = dout.data_ptr(), dout.stride()[:3]
+        dlast = None if dlast is None else dlast.contiguous()
+        dq, dk = (torch.empty((n, t, hk, K), dtype=dt, device=device) for _ in range(2))
+        dv = torch.empty((n, t, h, V), dtype=dt, device=device)
+        dg, dbeta = (torch.empty((n, t, h), dtype=dt, device=device) for _ in range(2))
+        first = None
+        if state is not None and ctx.needs_input_grad[5]:
+            first = torch.empty((n, h, K, V), dtype=torch.float32, device=device)
+        grads = _GRADS.pack(dop, 0 if dlast is None else dlast.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                            dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), 0 if first is None else first.data_ptr(),
+                            *dos, *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *dg.stride(), *dbeta.stride())
+        size = lib.goib2d_delta_workspace_bytes(desc)
+        native.check(min(size, 0))
+        work = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
+        _call(device, lib.goib2d_delta_backward, desc, grads, saved.data_ptr(), work.data_ptr())
         return dq, dk, dv, dg, dbeta, first, None, None
 
 
@@ -259,11 +271,9 @@ def clip_grads_(grads, max_norm):
     table[2::3] = array("q", [_DTYPE[x.dtype] for x in grads])
     packed = table.buffer_info()[0]
     lib = native.load()
-    with _on(device):
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        size = lib.goib2d_clip_workspace_bytes(packed, count)
-        native.check(min(size, 0))
-        work = torch.empty(size, dtype=torch.uint8, device=device)
-        native.check(lib.goib2d_clip_grads(packed, count, max_norm, norm.data_ptr(), work.data_ptr(),
-                                           _raw_stream(device.index)))
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    size = lib.goib2d_clip_workspace_bytes(packed, count)
+    native.check(min(size, 0))
+    work = torch.empty(size, dtype=torch.uint8, device=device)
+    _call(device, lib.goib2d_clip_grads, packed, count, max_norm, norm.data_ptr(), work.data_ptr())
     return norm
