@@ -39,8 +39,6 @@ struct Layout {
     static constexpr int pitch = KP + 8, chunks = AHEAD ? 2 : kTile<P> / kChunk;
     static constexpr int rows = AHEAD ? kChunk : kTile<P>;  // of a slot
     static constexpr int keys = AHEAD ? 4 : 2, values = AHEAD ? 4 : 1;  // slots of q and k, of dO and r
-    static constexpr int most = MT == 2 ? 2 : 4;            // warps that solve
-    static constexpr int threads = 32 * (most + (AHEAD ? 2 : 0));
     __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (sizeof(E) == 2 ? 8 : 4); }
     __host__ __device__ static int bytes(int warps) {
         return 2 * rows * (keys * pitch + values * v_pitch(warps)) * (int)sizeof(E) + chunks * (int)sizeof(Chunk<P>);
@@ -48,7 +46,7 @@ struct Layout {
 };
 
 template <class T, class P, int KP, int MT, bool AHEAD>
-__global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 : KP == 128 ? 3 : MT == 2 ? 6 : 3)
+__global__ void __maxnreg__(AHEAD ? 232 : 168)  // 168: 12 warps an SM
     goib2d_delta_back_state_kernel(const __grid_constant__ Backward f) {
     using L = Layout<P, KP, MT, AHEAD>;
     using E = typename P::E;
@@ -85,21 +83,18 @@ __global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 :
             }
             cp_commit();
         };
-        auto gate_of = [&](int i) {
-            const int at = (count - 1 - i) * kChunk;
-            return at < 0 ? Gate{0.0f, 0.0f, false} : gates.at(at + (lane & 15));
-        };
+        auto gate_of = [&](int i) { return gates.at((int64_t)(count - 1 - i) * kChunk + (lane & 15)); };
         load(me);
-        Gate next = gate_of(me);
+        RawGate<T> next = gate_of(me);
         for (int i = me; i < count; i += 2) {
             if (i >= 2) bar_wait(3 + me, 32 + 32 * warps);  // i - 2 is done: its slot and its matrices are free
             load(i + 2);
-            const Gate gate = next;
+            const RawGate<T> gate = next;
             next = gate_of(i + 2);
             cp_wait<1>();
             __syncwarp();
             const E *Q = keys + (i & 3) * key_slot;
-            prepare<P, KP, true>(chunks[me], Q, Q + kChunk * L::pitch, L::pitch, gate, d.scale, lane);
+            prepare<P, KP, true>(chunks[me], Q, Q + kChunk * L::pitch, L::pitch, gate.get(), d.scale, lane);
             __threadfence_block();
             bar_arrive(1 + me, 32 + 32 * warps);
         }
@@ -231,13 +226,19 @@ __global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 :
             load_rows(Rb, vp, r + (int64_t)at * V, V, left, TILE, V - block0, cols, f.wide_r, threadIdx.x, threads);
             cp_commit();
         };
-        Gate gate[N];
-        auto gates_of = [&](int tile) {
+        RawGate<T> gate[N];
+        // the tiles' chunks are prepared by the warps in turn; `first`: the warp of the tile's first one
+        auto turn_of = [&](int first, int s) { 
+            const int x = first + s;  // at most three over
+            return x < warps ? x : x - warps < warps ? x - warps : x - 2 * warps < warps ? x - 2 * warps : 0;
+        };
+        auto gates_of = [&](int tile, int first) {
 #pragma unroll
             for (int s = 0; s < N; ++s)
-                if ((tile * N + s) % warps == w) gate[s] = gates.at(tile * TILE + s * kChunk + (lane & 15));
+                if (turn_of(first, s) == w) gate[s] = gates.at(tile * TILE + s * kChunk + (lane & 15));
         };
-        if (tiles) load_keys(tiles - 1), gates_of(tiles - 1);
+        if (tiles) load_keys(tiles - 1), gates_of(tiles - 1, 0);
+        int turn = 0;
 #pragma unroll 1
         for (int tile = tiles - 1; tile >= 0; --tile) {
             const E *Q = keys + (tile & 1) * key_slot, *Kb = Q + TILE * L::pitch;
@@ -247,10 +248,11 @@ __global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 :
             if (tile > 0) load_keys(tile - 1);
 #pragma unroll
             for (int s = 0; s < N; ++s)
-                if ((tile * N + s) % warps == w)
-                    prepare<P, KP, true>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
+                if (turn_of(turn, s) == w)
+                    prepare<P, KP, true>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s].get(),
                                          d.scale, lane);
-            if (tile > 0) gates_of(tile - 1), cp_wait<1>();
+            turn = turn_of(turn, N);
+            if (tile > 0) gates_of(tile - 1, turn), cp_wait<1>();
             else cp_wait<0>();
             __syncthreads();
 #pragma unroll 1
@@ -315,6 +317,7 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
     using L = Span<P, KP, C>;
     using E = typename P::E;
     constexpr int RB = L::RB, KH = L::KH, threads = L::warps * 32, PL = C / 32;
+    constexpr int N = 16 / sizeof(E), B = 4;
     extern __shared__ __align__(16) char sm[];
     const goib2d_delta_desc &d = f.d;
     const int K = d.key_dim, V = d.value_dim, tv = f.tiles_v, vp = L::v_pitch(tv), cols = tv * 16;
@@ -328,37 +331,44 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
     const L s(sm, tv);
     auto &x = *s.x;
 
-    load_rows(s.Q, L::pitch, row<T>(d.q, d.q_stride, n, at, hk), d.q_stride[1], left, C, K, KP, f.wide_q, tid, threads);
-    load_rows(s.K, L::pitch, row<T>(d.k, d.k_stride, n, at, hk), d.k_stride[1], left, C, K, KP, f.wide_k, tid, threads);
+    load_rows(s.Q, L::pitch, row<T>(d.q, d.q_stride, n, at, hk), (int)d.q_stride[1], left, C, K, KP, f.wide_q, tid, threads);
+    load_rows(s.K, L::pitch, row<T>(d.k, d.k_stride, n, at, hk), (int)d.k_stride[1], left, C, K, KP, f.wide_k, tid, threads);
     float dq[KH / 8][4] = {}, dk[KH / 8][4] = {};
 #pragma unroll 1
     for (int j = 0; j < group; ++j) {
         const int h = hk * group + j;
         const int64_t nh = n * d.heads + h, kept = (nh * spans + span) * cols * KP;
+        const Gates<T> gates(d, n, h);
+        const RawGate<T> raw = gates.at(at + rb * 16 + (lane & 15)), first = gates.at(at);
         __syncthreads();
         const bool o = f.gr.dout != nullptr;
-        load_rows(s.O, vp, o ? row<T>(f.gr.dout, f.gr.dout_stride, n, at, h) : nullptr, f.gr.dout_stride[1], o ? left : 0, C, V,
+        load_rows(s.O, vp, o ? row<T>(f.gr.dout, f.gr.dout_stride, n, at, h) : nullptr, (int)f.gr.dout_stride[1], o ? left : 0, C, V,
                   cols, f.wide_do, tid, threads);
-        load_rows(s.V, vp, row<E>((const void *)f.dv, f.dv_stride, n, at, h), f.dv_stride[1], left, C, V, cols, f.wide_dv, tid,
+        load_rows(s.V, vp, row<E>((const void *)f.dv, f.dv_stride, n, at, h), (int)f.dv_stride[1], left, C, V, cols, f.wide_dv, tid,
                   threads);
         load_rows(s.R, vp, (const E *)f.r + (nh * steps + at) * V, V, left, C, V, cols, f.wide_r, tid, threads);
         // S0 may hold anything where the span's first token starts afresh: it is not used then
         const E *kept_s = (const E *)f.kept_s + kept, *kept_ds = (const E *)f.kept_ds + kept;
         load_rows(s.S, L::pitch, kept_s, KP, cols, cols, KP, KP, true, tid, threads);
         cp_commit();
-        const bool anew = load_gate<T>(d, n, at, h).fresh;
+        const bool anew = first.get().fresh;
         float end = 0.0f;
-        for (int i = tid * 8; i < cols * KP; i += threads * 8) {
-            float u[8], v[8];
-            eight_at(u, kept_s + i), eight_at(v, kept_ds + i);
+        for (int i = tid * N; i < cols * KP; i += threads * N * B) {  // B pairs of loads in flight
+            uint4 u[B], v[B];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) end += u[e] * v[e];
+            for (int e = 0; e < B; ++e) {
+                const bool in = i + e * threads * N < cols * KP;
+                u[e] = in ? *(const uint4 *)(kept_s + i + e * threads * N) : make_uint4(0, 0, 0, 0);
+                v[e] = in ? *(const uint4 *)(kept_ds + i + e * threads * N) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < B; ++e) end += dot16<E>(u[e], v[e]);
         }
         for (int i = 16; i > 0; i >>= 1) end += __shfl_xor_sync(~0u, end, i);
         if (lane == 0) x.end[w] = anew ? 0.0f : end;
         if (part == 0) {
             const int i = lane & 15;
-            const Gate gate = load_gate<T>(d, n, at + rb * 16 + i, h);
+            const Gate gate = raw.get();
             const double G = running_sum(gate, lane), last = __shfl_sync(~0u, G, 15);
             const uint32_t fresh = __ballot_sync(~0u, gate.fresh) & 0xffffu;
             const int since = __popc(fresh & ((2u << i) - 1)), all = __popc(fresh);

@@ -95,17 +95,21 @@ struct Gate {
     bool fresh;
 };
 
+// The same as loaded: nothing is done with the values until they are asked for, so that a load for the next chunk is
+// not waited for.
 template <class T>
-__device__ __forceinline__ Gate load_gate(const goib2d_delta_desc &d, int64_t n, int64_t t, int h) {
-    if (t < 0 || t >= d.n_steps) return {0.0f, 0.0f, false};
-    Gate r;
-    r.g = to_float(*row<T>(d.g, d.g_stride, n, t, h));
-    r.b = to_float(*row<T>(d.beta, d.beta_stride, n, t, h));
-    r.fresh = (d.reset && d.reset[n * d.reset_stride[0] + t * d.reset_stride[1]]) || expf(r.g) == 0.0f;
-    return r;
-}
+struct RawGate {
+    T g, b;
+    uint8_t reset;
+    bool live;
+    __device__ __forceinline__ Gate get() const {
+        if (!live) return {0.0f, 0.0f, false};
+        const float x = to_float(g);
+        return {x, to_float(b), reset || expf(x) == 0.0f};
+    }
+};
 
-// The gates of one (world, head), chunk by chunk.
+// The gates of one (world, head).
 template <class T>
 struct Gates {
     const T *g, *b;
@@ -115,10 +119,15 @@ struct Gates {
         : g(row<T>(d.g, d.g_stride, n, 0, h)), b(row<T>(d.beta, d.beta_stride, n, 0, h)),
           reset(d.reset ? d.reset + n * d.reset_stride[0] : nullptr), gs((int)d.g_stride[1]), bs((int)d.beta_stride[1]),
           rs((int)d.reset_stride[1]), steps((int)d.n_steps) {}
-    __device__ __forceinline__ Gate at(int t) const {  // lane's token
-        if (t >= steps) return {0.0f, 0.0f, false};
-        const float x = to_float(g[(int64_t)t * gs]), y = to_float(b[(int64_t)t * bs]);
-        return {x, y, (reset && reset[(int64_t)t * rs]) || expf(x) == 0.0f};
+    __device__ __forceinline__ RawGate<T> at(int64_t t) const {
+        RawGate<T> r;
+        r.live = t >= 0 && t < steps;
+        r.reset = 0, r.g = r.b = T(0.0f);
+        if (r.live) {
+            r.g = g[t * gs], r.b = b[t * bs];
+            if (reset) r.reset = reset[t * rs];
+        }
+        return r;
     }
 };
 
@@ -210,27 +219,35 @@ __device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, con
 // Rows of a strided tensor into shared memory, zeros past `rows` and `cols`. Aligned rows of the same type come by
 // asynchronous copies, eight neighbouring threads to a row.
 template <class E, class T>
-__device__ __forceinline__ void load_rows(E *to, int pitch, const T *from, int64_t stride, int rows, int count, int cols,
+__device__ __forceinline__ void load_rows(E *to, int pitch, const T *from, int stride, int rows, int count, int cols,
                                           int padded, bool wide, int tid, int threads) {
+    const int r0 = tid / 8, dr = threads / 8;
+    const int64_t step = (int64_t)dr * stride;
+    from += (int64_t)r0 * stride, to += r0 * pitch;
     if constexpr (sizeof(T) == sizeof(E)) {
         if (wide) {
             constexpr int N = 16 / sizeof(E);
-            for (int c = tid % 8 * N; c < padded; c += 8 * N)
-                for (int r = tid / 8; r < count; r += threads / 8) {
-                    E *p = to + r * pitch + c;
-                    if (r < rows && c < cols) cp_async16(p, from + r * stride + c);
-                    else *(uint4 *)p = make_uint4(0, 0, 0, 0);
+            for (int c = tid % 8 * N; c < padded; c += 8 * N) {
+                const T *p = from + c;
+                E *q = to + c;
+                const int live = c < cols ? rows : 0;
+                for (int r = r0; r < count; r += dr, p += step, q += dr * pitch) {
+                    if (r < live) cp_async16(q, p);
+                    else *(uint4 *)q = make_uint4(0, 0, 0, 0);
                 }
+            }
             return;
         }
     }
-    for (int c = tid % 8 * 2; c < padded; c += 16)
-        for (int r = tid / 8; r < count; r += threads / 8) {
-            const T *p = from + r * stride + c;
+    for (int c = tid % 8 * 2; c < padded; c += 16) {
+        const T *p = from + c;
+        E *q = to + c;
+        for (int r = r0; r < count; r += dr, p += step, q += dr * pitch) {
             const float u = r < rows && c < cols ? to_float(p[0]) : 0.0f, v = r < rows && c + 1 < cols ? to_float(p[1]) : 0.0f;
-            if constexpr (sizeof(E) == 2) *(uint32_t *)(to + r * pitch + c) = pack(u, v);
-            else *(float2 *)(to + r * pitch + c) = make_float2(u, v);
+            if constexpr (sizeof(E) == 2) *(uint32_t *)q = pack(u, v);
+            else *(float2 *)q = make_float2(u, v);
         }
+    }
 }
 
 // A warp's MT * 16 columns of a state [K][V] as accumulators of S^T (rows v, columns k), and back.
@@ -364,14 +381,17 @@ __device__ __forceinline__ float2 pair_at(const bf16 *p) {
 }
 __device__ __forceinline__ float2 pair_at(const float *p) { return *(const float2 *)p; }
 
-// Eight neighbouring values, 16-byte aligned.
-__device__ __forceinline__ void eight_at(float (&v)[8], const bf16 *p) {
-    const uint4 y = *(const uint4 *)p;
-    v[0] = low(y.x), v[1] = high(y.x), v[2] = low(y.y), v[3] = high(y.y);
-    v[4] = low(y.z), v[5] = high(y.z), v[6] = low(y.w), v[7] = high(y.w);
-}
-__device__ __forceinline__ void eight_at(float (&v)[8], const float *p) {
-    *(float4 *)v = *(const float4 *)p, *(float4 *)(v + 4) = *(const float4 *)(p + 4);
+// The sum of the products of 16 bytes of values.
+template <class E>
+__device__ __forceinline__ float dot16(const uint4 &x, const uint4 &y) {
+    const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(E) == 2) s += low(u[e]) * low(v[e]) + high(u[e]) * high(v[e]);
+        else s += __uint_as_float(u[e]) * __uint_as_float(v[e]);
+    }
+    return s;
 }
 
 }  // namespace gb

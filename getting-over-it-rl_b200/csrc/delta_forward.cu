@@ -23,8 +23,6 @@ struct Layout {
     using E = typename P::E;
     static constexpr int pitch = KP + 8, slots = AHEAD ? 4 : 2, chunks = AHEAD ? 2 : kTile<P> / kChunk;
     static constexpr int rows = AHEAD ? kChunk : kTile<P>;  // of a slot
-    static constexpr int most = MT == 2 ? 2 : 4;            // warps that solve
-    static constexpr int threads = 32 * (most + (AHEAD ? 2 : 0));
     __host__ __device__ static int v_pitch(int warps) { return warps * 16 * MT + (sizeof(E) == 2 ? 8 : 4); }
     __host__ __device__ static int slot(int warps) { return rows * (2 * pitch + v_pitch(warps)) * (int)sizeof(E); }
     __host__ __device__ static int bytes(int warps) { return slots * slot(warps) + chunks * (int)sizeof(Chunk<P>); }
@@ -38,7 +36,7 @@ __device__ __noinline__ void odd_chunk(const Forward &f, float *S, const typenam
     const goib2d_delta_desc &d = f.d;
     const int g = lane >> 2, t = lane & 3, tokens = (int)(d.n_steps - at < kChunk ? d.n_steps - at : kChunk);
     for (int i = 0; i < tokens; ++i) {
-        const Gate gate = load_gate<T>(d, n, at + i, h);
+        const Gate gate = Gates<T>(d, n, h).at(at + i).get();
         const float a = gate.fresh ? 0.0f : expf(gate.g);
         for (int m = 0; m < 2 * MT; ++m) {  // the thread's rows
             float *s = S + (m >> 1) * (KP / 8) * 4 + (m & 1) * 2;
@@ -67,7 +65,7 @@ __device__ __noinline__ void odd_chunk(const Forward &f, float *S, const typenam
 }
 
 template <class T, class P, int KP, int MT, bool AHEAD>
-__global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 : KP == 128 ? 3 : MT == 2 ? 6 : 3)
+__global__ void __maxnreg__(AHEAD ? 232 : 168)  // 168: 12 warps an SM
     goib2d_delta_forward_kernel(const __grid_constant__ Forward f) {
     using L = Layout<P, KP, MT, AHEAD>;
     using E = typename P::E;
@@ -101,16 +99,16 @@ __global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 :
             cp_commit();
         };
         load(me);
-        Gate next = gates.at(me * kChunk + (lane & 15));
+        RawGate<T> next = gates.at(me * kChunk + (lane & 15));
         for (int i = me; i < count; i += 2) {
             if (i >= 2) bar_wait(3 + me, 32 + 32 * warps);  // chunk i - 2 is solved: its slot and its matrices are free
             load(i + 2);
-            const Gate gate = next;
+            const RawGate<T> gate = next;
             next = gates.at((i + 2) * kChunk + (lane & 15));
             cp_wait<1>();
             __syncwarp();
             const E *Q = (const E *)(sm + (i & 3) * slot);
-            prepare<P, KP, false>(chunks[me], Q, Q + kChunk * L::pitch, L::pitch, gate, d.scale, lane);
+            prepare<P, KP, false>(chunks[me], Q, Q + kChunk * L::pitch, L::pitch, gate.get(), d.scale, lane);
             __threadfence_block();
             bar_arrive(1 + me, 32 + 32 * warps);
         }
@@ -231,13 +229,19 @@ __global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 :
             load_rows(Vb, vp, v + (int64_t)at * vs, vs, left, TILE, V - block0, warps * 16 * MT, f.wide_v, threadIdx.x, threads);
             cp_commit();
         };
-        Gate gate[N];
-        auto gates_of = [&](int tile) {
+        RawGate<T> gate[N];
+        // the tiles' chunks are prepared by the warps in turn; `first`: the warp of the tile's first one
+        auto turn_of = [&](int first, int s) { 
+            const int x = first + s;  // at most three over
+            return x < warps ? x : x - warps < warps ? x - warps : x - 2 * warps < warps ? x - 2 * warps : 0;
+        };
+        auto gates_of = [&](int tile, int first) {
 #pragma unroll
             for (int s = 0; s < N; ++s)
-                if ((tile * N + s) % warps == w) gate[s] = gates.at(tile * TILE + s * kChunk + (lane & 15));
+                if (turn_of(first, s) == w) gate[s] = gates.at(tile * TILE + s * kChunk + (lane & 15));
         };
-        if (tiles) load(0), gates_of(0);
+        if (tiles) load(0), gates_of(0, 0);
+        int turn = 0;
 #pragma unroll 1
         for (int tile = 0; tile < tiles; ++tile) {
             E *Q = (E *)(sm + (tile & 1) * slot), *Kb = Q + TILE * L::pitch, *Vb = Kb + TILE * L::pitch;
@@ -246,10 +250,11 @@ __global__ void __launch_bounds__(Layout<P, KP, MT, AHEAD>::threads, AHEAD ? 1 :
             if (tile + 1 < tiles) load(tile + 1);
 #pragma unroll
             for (int s = 0; s < N; ++s)
-                if ((tile * N + s) % warps == w)
-                    prepare<P, KP, false>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s],
+                if (turn_of(turn, s) == w)
+                    prepare<P, KP, false>(chunks[s], Q + s * kChunk * L::pitch, Kb + s * kChunk * L::pitch, L::pitch, gate[s].get(),
                                           d.scale, lane);
-            if (tile + 1 < tiles) gates_of(tile + 1);
+            turn = turn_of(turn, N);
+            if (tile + 1 < tiles) gates_of(tile + 1, turn);
             __syncthreads();
 #pragma unroll 1
             for (int s = 0; s < N && tile * TILE + s * kChunk < steps; ++s)
