@@ -557,3 +557,24 @@ def test_struct_layouts():
     """The packed structures are the header's (sizes as a C compiler lays them out)."""
     assert (policy._DESC.size, policy._GRADS.size, policy._GRAD.size) == (272, 208, 24)
     assert C.sizeof(C.c_void_p) == 8
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_example_acts_and_trains(dtype):
+    """examples/memory_policy.py: the rollout replayed for training gives the actions that the acting pass gave, and
+    the update's clipped gradient moves the weights."""
+    import sys
+    from pathlib import Path
+    sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
+    import memory_policy
+    torch.manual_seed(0)
+    fresh = memory_policy.MemoryPolicy().cuda().to(dtype)
+    policy, results = memory_policy.train(worlds=64, steps=24, updates=2, dtype=dtype, log=lambda line: None)
+    for r in results:
+        assert all(math.isfinite(x) for x in r.values())
+        assert r["norm"] > 0
+        # the linear layers run on other shapes in the two passes: their rounding differs too
+        assert r["replayed"] <= 4 * TOL[dtype]
+    assert all(torch.isfinite(p).all() for p in policy.parameters())
+    assert any(not torch.equal(p, q) for p, q in zip(policy.parameters(), fresh.parameters()))
