@@ -1047,6 +1047,10 @@ int delta_check(const goib2d_delta_desc *d) {
     if (d->n_worlds && !d->state_out) return fail(GOIB2D_EINVAL, "null state");
     if (d->n_worlds && d->n_steps && (!d->q || !d->k || !d->v || !d->g || !d->beta))
         return fail(GOIB2D_EINVAL, "null input");
+    const uintptr_t size = d->dtype == GOIB2D_BFLOAT16 ? 2 : 4;
+    if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->g | (uintptr_t)d->beta | (uintptr_t)d->out) % size ||
+        ((uintptr_t)d->state_in | (uintptr_t)d->state_out) % 4)
+        return fail(GOIB2D_EINVAL, "a pointer is not aligned to its elements");
     return 0;
 }
 }  // namespace
@@ -1094,6 +1098,10 @@ int goib2d_delta_backward(const goib2d_delta_desc *d, const goib2d_delta_grads *
     if (d->n_steps && (!saved || (uintptr_t)saved % 16)) return fail(GOIB2D_EINVAL, "saved is null or not 16-byte aligned");
     if (d->n_steps && (!gr->dq || !gr->dk || !gr->dv || !gr->dg || !gr->dbeta))
         return fail(GOIB2D_EINVAL, "null gradient");
+    const uintptr_t size = d->dtype == GOIB2D_BFLOAT16 ? 2 : 4;
+    if (((uintptr_t)gr->dout | (uintptr_t)gr->dq | (uintptr_t)gr->dk | (uintptr_t)gr->dv | (uintptr_t)gr->dg |
+         (uintptr_t)gr->dbeta) % size || ((uintptr_t)gr->dstate_out | (uintptr_t)gr->dstate_in) % 4)
+        return fail(GOIB2D_EINVAL, "a gradient's pointer is not aligned to its elements");
     if (far(gr->dout_stride) || far(gr->dv_stride))
         return fail(GOIB2D_ELIMIT, "a step's stride is 2^31 elements or more");
     CUDA_TRY(gb::launch_delta_backward(*d, *gr, saved, workspace, (cudaStream_t)stream));

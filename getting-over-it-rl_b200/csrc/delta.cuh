@@ -34,11 +34,19 @@ __device__ __forceinline__ float decay_at(const goib2d_delta_desc &d, int64_t n,
     return expf(to_float(*row<T>(d.g, d.g_stride, n, t, h)));
 }
 
-// Whether 16-byte accesses to the rows of a strided tensor are aligned.
-inline bool rows_aligned(const void *p, const int64_t (&s)[3], int64_t n0, int64_t n1, int64_t n2, int cols, int size) {
-    const int64_t e = 16 / size;
-    return (uintptr_t)p % 16 == 0 && cols % e == 0 && (n0 == 1 || s[0] % e == 0) && (n1 == 1 || s[1] % e == 0) &&
-           (n2 == 1 || s[2] % e == 0);
+// The largest piece, of 16, 8 or 4 bytes, that the rows of a strided tensor and their starts are whole multiples of; 0:
+// none (bfloat16 rows of odd places). n0, n1, n2: how many worlds, steps and heads there are.
+inline int rows_grain(const void *p, const int64_t (&s)[3], int64_t n0, int64_t n1, int64_t n2, int cols, int size) {
+    for (int bytes = 16; bytes >= 4; bytes /= 2) {
+        const int64_t e = bytes / size;
+        if ((uintptr_t)p % bytes == 0 && cols % e == 0 && (n0 == 1 || s[0] % e == 0) && (n1 == 1 || s[1] % e == 0) &&
+            (n2 == 1 || s[2] % e == 0))
+            return bytes;
+    }
+    return 0;
+}
+inline int dense_grain(int cols, int size) {  // of dense rows from an aligned start on
+    return cols * size % 16 == 0 ? 16 : cols * size % 8 == 0 ? 8 : cols * size % 4 == 0 ? 4 : 0;
 }
 
 // Gradients whose products run in full precision (mma.cuh, Full): those of float32 inputs, and those of few tokens in

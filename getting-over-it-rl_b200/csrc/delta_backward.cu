@@ -27,7 +27,8 @@ struct Backward {
     int64_t dv_stride[3];
     float *db;               // db by warps' columns: [n][h][parts][t]
     int32_t keep, tiles_v, parts;
-    bool wide_q, wide_k, wide_do, wide_dv, wide_r;
+    int grain_q, grain_k, grain_do, grain_dv, grain_r;  // rows_grain
+    bool wide_dv;            // rows of dv are 16-byte pieces
     bool wide_dqk;           // pairs of channels of dq and dk are aligned
 };
 
@@ -76,10 +77,10 @@ __global__ void __maxnreg__(AHEAD ? 232 : 168)  // 168: 12 warps an SM
             const int at = (count - 1 - i) * kChunk, left = steps - at;
             if (at >= 0) {
                 E *Q = keys + (i & 3) * key_slot, *Ob = values + (i & 3) * value_slot;
-                chunk_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, K, KP, f.wide_q, lane);
-                chunk_rows(Q + kChunk * L::pitch, L::pitch, k + (int64_t)at * ks, ks, left, K, KP, f.wide_k, lane);
-                chunk_rows(Ob, vp, o + (int64_t)at * os, os, o ? left : 0, V - block0, cols, f.wide_do, lane);
-                chunk_rows(Ob + kChunk * vp, vp, r + (int64_t)at * V, V, left, V - block0, cols, f.wide_r, lane);
+                chunk_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, K, KP, f.grain_q, lane);
+                chunk_rows(Q + kChunk * L::pitch, L::pitch, k + (int64_t)at * ks, ks, left, K, KP, f.grain_k, lane);
+                chunk_rows(Ob, vp, o + (int64_t)at * os, os, o ? left : 0, V - block0, cols, f.grain_do, lane);
+                chunk_rows(Ob + kChunk * vp, vp, r + (int64_t)at * V, V, left, V - block0, cols, f.grain_r, lane);
             }
             cp_commit();
         };
@@ -216,14 +217,14 @@ __global__ void __maxnreg__(AHEAD ? 232 : 168)  // 168: 12 warps an SM
         auto load_keys = [&](int tile) {
             E *Q = keys + (tile & 1) * key_slot;
             const int at = tile * TILE, left = steps - at < TILE ? steps - at : TILE;
-            load_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, TILE, K, KP, f.wide_q, threadIdx.x, threads);
-            load_rows(Q + TILE * L::pitch, L::pitch, k + (int64_t)at * ks, ks, left, TILE, K, KP, f.wide_k, threadIdx.x, threads);
+            load_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, TILE, K, KP, f.grain_q, threadIdx.x, threads);
+            load_rows(Q + TILE * L::pitch, L::pitch, k + (int64_t)at * ks, ks, left, TILE, K, KP, f.grain_k, threadIdx.x, threads);
             cp_commit();
         };
         auto load_values = [&](int tile) {
             const int at = tile * TILE, left = steps - at < TILE ? steps - at : TILE;
-            load_rows(Ob, vp, o + (int64_t)at * os, os, o ? left : 0, TILE, V - block0, cols, f.wide_do, threadIdx.x, threads);
-            load_rows(Rb, vp, r + (int64_t)at * V, V, left, TILE, V - block0, cols, f.wide_r, threadIdx.x, threads);
+            load_rows(Ob, vp, o + (int64_t)at * os, os, o ? left : 0, TILE, V - block0, cols, f.grain_do, threadIdx.x, threads);
+            load_rows(Rb, vp, r + (int64_t)at * V, V, left, TILE, V - block0, cols, f.grain_r, threadIdx.x, threads);
             cp_commit();
         };
         RawGate<T> gate[N];
@@ -331,8 +332,8 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
     const L s(sm, tv);
     auto &x = *s.x;
 
-    load_rows(s.Q, L::pitch, row<T>(d.q, d.q_stride, n, at, hk), (int)d.q_stride[1], left, C, K, KP, f.wide_q, tid, threads);
-    load_rows(s.K, L::pitch, row<T>(d.k, d.k_stride, n, at, hk), (int)d.k_stride[1], left, C, K, KP, f.wide_k, tid, threads);
+    load_rows(s.Q, L::pitch, row<T>(d.q, d.q_stride, n, at, hk), (int)d.q_stride[1], left, C, K, KP, f.grain_q, tid, threads);
+    load_rows(s.K, L::pitch, row<T>(d.k, d.k_stride, n, at, hk), (int)d.k_stride[1], left, C, K, KP, f.grain_k, tid, threads);
     float dq[KH / 8][4] = {}, dk[KH / 8][4] = {};
 #pragma unroll 1
     for (int j = 0; j < group; ++j) {
@@ -343,13 +344,13 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
         __syncthreads();
         const bool o = f.gr.dout != nullptr;
         load_rows(s.O, vp, o ? row<T>(f.gr.dout, f.gr.dout_stride, n, at, h) : nullptr, (int)f.gr.dout_stride[1], o ? left : 0, C, V,
-                  cols, f.wide_do, tid, threads);
-        load_rows(s.V, vp, row<E>((const void *)f.dv, f.dv_stride, n, at, h), (int)f.dv_stride[1], left, C, V, cols, f.wide_dv, tid,
+                  cols, f.grain_do, tid, threads);
+        load_rows(s.V, vp, row<E>((const void *)f.dv, f.dv_stride, n, at, h), (int)f.dv_stride[1], left, C, V, cols, f.grain_dv, tid,
                   threads);
-        load_rows(s.R, vp, (const E *)f.r + (nh * steps + at) * V, V, left, C, V, cols, f.wide_r, tid, threads);
+        load_rows(s.R, vp, (const E *)f.r + (nh * steps + at) * V, V, left, C, V, cols, f.grain_r, tid, threads);
         // S0 may hold anything where the span's first token starts afresh: it is not used then
         const E *kept_s = (const E *)f.kept_s + kept, *kept_ds = (const E *)f.kept_ds + kept;
-        load_rows(s.S, L::pitch, kept_s, KP, cols, cols, KP, KP, true, tid, threads);
+        load_rows(s.S, L::pitch, kept_s, KP, cols, cols, KP, KP, 16, tid, threads);
         cp_commit();
         const bool anew = first.get().fresh;
         float end = 0.0f;
@@ -512,7 +513,7 @@ __global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof
             if (t == 0 && part == 0) x.rows[i0 + 8 * r] = rows[r];
         }
         __syncthreads();
-        load_rows(s.S, L::pitch, kept_ds, KP, cols, cols, KP, KP, true, tid, threads);
+        load_rows(s.S, L::pitch, kept_ds, KP, cols, cols, KP, KP, 16, tid, threads);
         cp_commit();
         // the tokens as j: A and M over the tokens from them on
         m = 1.0f;
@@ -727,11 +728,12 @@ cudaError_t backward_typed(const goib2d_delta_desc &d, const goib2d_delta_grads 
         f.dv = (char *)workspace + at.states + db_bytes(d);
         f.dv_stride[0] = d.n_steps * d.heads * V, f.dv_stride[1] = (int64_t)d.heads * V, f.dv_stride[2] = V;
     }
-    f.wide_q = rows_aligned(d.q, d.q_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
-    f.wide_k = rows_aligned(d.k, d.k_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
-    f.wide_do = rows_aligned(gr.dout, gr.dout_stride, d.n_worlds, d.n_steps, d.heads, V, z);
-    f.wide_dv = rows_aligned(f.dv, f.dv_stride, d.n_worlds, d.n_steps, d.heads, V, sizeof(typename P::E));
-    f.wide_r = V % 8 == 0;
+    f.grain_q = rows_grain(d.q, d.q_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
+    f.grain_k = rows_grain(d.k, d.k_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
+    f.grain_do = rows_grain(gr.dout, gr.dout_stride, d.n_worlds, d.n_steps, d.heads, V, z);
+    f.grain_dv = rows_grain(f.dv, f.dv_stride, d.n_worlds, d.n_steps, d.heads, V, sizeof(typename P::E));
+    f.wide_dv = f.grain_dv == 16;
+    f.grain_r = dense_grain(V, sizeof(typename P::E));
     f.wide_dqk = (uintptr_t)gr.dq % (2 * z) == 0 && (uintptr_t)gr.dk % (2 * z) == 0;
     for (int i = 0; i < 3; ++i) f.wide_dqk = f.wide_dqk && gr.dq_stride[i] % 2 == 0 && gr.dk_stride[i] % 2 == 0;
     switch (padded_keys(d.key_dim)) {

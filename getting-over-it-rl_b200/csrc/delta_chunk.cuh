@@ -216,38 +216,89 @@ __device__ __forceinline__ void prepare(Chunk<P> &c, const typename P::E *Q, con
     c.z.put(i, lane / 16 * 8, half);
 }
 
-// Rows of a strided tensor into shared memory, zeros past `rows` and `cols`. Aligned rows of the same type come by
-// asynchronous copies, eight neighbouring threads to a row.
+// Rows of a strided tensor into shared memory, zeros past `rows` and `cols`: by asynchronous copies of `grain` bytes
+// (rows_grain) where the types are the same, eight neighbouring threads to a row.
+template <int BYTES, class E>
+__device__ __forceinline__ void copy_rows(E *to, int pitch, const E *from, int64_t step, int r0, int dr, int rows, int count,
+                                          int cols, int padded, int tid) {
+    constexpr int N = BYTES / sizeof(E);
+    for (int c = tid % 8 * N; c < padded; c += 8 * N) {
+        const E *p = from + c;
+        E *q = to + c;
+        const int live = c < cols ? rows : 0;
+        for (int r = r0; r < count; r += dr, p += step, q += dr * pitch) {
+            if (r < live) {
+                cp_async<BYTES>(q, p);
+            } else {
+#pragma unroll
+                for (int e = 0; e < BYTES / 4; ++e) ((uint32_t *)q)[e] = 0;
+            }
+        }
+    }
+}
 template <class E, class T>
-__device__ __forceinline__ void load_rows(E *to, int pitch, const T *from, int stride, int rows, int count, int cols,
-                                          int padded, bool wide, int tid, int threads) {
+__device__ __noinline__ void load_rows_odd(E *to, int pitch, const T *from, int stride, int rows, int count, int cols,
+                                          int padded, int grain, int tid, int threads) {
     const int r0 = tid / 8, dr = threads / 8;
     const int64_t step = (int64_t)dr * stride;
     from += (int64_t)r0 * stride, to += r0 * pitch;
     if constexpr (sizeof(T) == sizeof(E)) {
-        if (wide) {
+        if (grain == 8) return copy_rows<8>(to, pitch, from, step, r0, dr, rows, count, cols, padded, tid);
+        if (sizeof(T) == 4 || grain == 4) return copy_rows<4>(to, pitch, from, step, r0, dr, rows, count, cols, padded, tid);
+    }
+    constexpr int U = 4;  // rows whose loads are in flight together
+    for (int c = tid % 8 * 2; c < padded; c += 16) {
+        const T *p = from + c;
+        E *q = to + c;
+        for (int r = r0; r < count; r += U * dr, p += U * step, q += U * dr * pitch) {
+            T u[U], v[U];
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                u[e] = r + e * dr < rows && c < cols ? p[e * step] : T(0.0f);
+                v[e] = r + e * dr < rows && c + 1 < cols ? p[e * step + 1] : T(0.0f);
+            }
+#pragma unroll
+            for (int e = 0; e < U; ++e) {
+                if (r + e * dr >= count) break;
+                if constexpr (sizeof(E) == 2) *(uint32_t *)(q + e * dr * pitch) = pack(to_float(u[e]), to_float(v[e]));
+                else *(float2 *)(q + e * dr * pitch) = make_float2(to_float(u[e]), to_float(v[e]));
+            }
+        }
+    }
+}
+template <class E, class T>
+__device__ __forceinline__ void load_rows(E *to, int pitch, const T *from, int stride, int rows, int count, int cols,
+                                          int padded, int grain, int tid, int threads) {
+    if constexpr (sizeof(T) == sizeof(E)) {
+        if (grain == 16) {
+            const int r0 = tid / 8, dr = threads / 8;
+            return copy_rows<16>(to + r0 * pitch, pitch, from + (int64_t)r0 * stride, (int64_t)dr * stride, r0, dr, rows, count,
+                                 cols, padded, tid);
+        }
+    }
+    load_rows_odd(to, pitch, from, stride, rows, count, cols, padded, grain, tid, threads);
+}
+// The same for 16 rows by one warp.
+template <class E, class T>
+__device__ __forceinline__ void chunk_rows(E *to, int pitch, const T *from, int stride, int rows, int cols, int padded,
+                                           int grain, int lane) {
+    if constexpr (sizeof(T) == sizeof(E)) {
+        if (grain == 16) {
             constexpr int N = 16 / sizeof(E);
-            for (int c = tid % 8 * N; c < padded; c += 8 * N) {
-                const T *p = from + c;
-                E *q = to + c;
-                const int live = c < cols ? rows : 0;
-                for (int r = r0; r < count; r += dr, p += step, q += dr * pitch) {
-                    if (r < live) cp_async16(q, p);
+            for (int c = lane % 8 * N; c < padded; c += 8 * N) {
+                const T *p = from + (int64_t)(lane / 8) * stride + c;
+                E *q = to + lane / 8 * pitch + c;
+                const int left = c < cols ? rows - lane / 8 : 0;
+#pragma unroll
+                for (int r = 0; r < kChunk; r += 4, p += (int64_t)4 * stride, q += 4 * pitch) {
+                    if (r < left) cp_async<16>(q, p);
                     else *(uint4 *)q = make_uint4(0, 0, 0, 0);
                 }
             }
             return;
         }
     }
-    for (int c = tid % 8 * 2; c < padded; c += 16) {
-        const T *p = from + c;
-        E *q = to + c;
-        for (int r = r0; r < count; r += dr, p += step, q += dr * pitch) {
-            const float u = r < rows && c < cols ? to_float(p[0]) : 0.0f, v = r < rows && c + 1 < cols ? to_float(p[1]) : 0.0f;
-            if constexpr (sizeof(E) == 2) *(uint32_t *)q = pack(u, v);
-            else *(float2 *)q = make_float2(u, v);
-        }
-    }
+    load_rows_odd(to, pitch, from, stride, rows, kChunk, cols, padded, grain, lane, 32);
 }
 
 // A warp's MT * 16 columns of a state [K][V] as accumulators of S^T (rows v, columns k), and back.
@@ -298,29 +349,6 @@ __device__ __forceinline__ void store_state(float *to, const float (&S)[MT][KP /
                 const int k = 8 * j + k0 + (e & 1), v = v1 + 16 * m + (e >> 1) * 8;
                 if (k < K && v < V) to[k * V + v] = S[m][j][e];
             }
-}
-
-// The same for 16 rows by one warp.
-template <class E, class T>
-__device__ __forceinline__ void chunk_rows(E *to, int pitch, const T *from, int stride, int rows, int cols, int padded,
-                                           bool wide, int lane) {
-    if constexpr (sizeof(T) == sizeof(E)) {
-        if (wide) {
-            constexpr int N = 16 / sizeof(E);
-            for (int c = lane % 8 * N; c < padded; c += 8 * N) {
-                const T *p = from + (int64_t)(lane / 8) * stride + c;
-                E *q = to + lane / 8 * pitch + c;
-                const int left = c < cols ? rows - lane / 8 : 0;
-#pragma unroll
-                for (int r = 0; r < kChunk; r += 4, p += (int64_t)4 * stride, q += 4 * pitch) {
-                    if (r < left) cp_async16(q, p);
-                    else *(uint4 *)q = make_uint4(0, 0, 0, 0);
-                }
-            }
-            return;
-        }
-    }
-    load_rows(to, pitch, from, stride, rows, kChunk, cols, padded, false, lane, 32);
 }
 
 // 16 x 16 values (rows v, columns tokens) of one accumulator pair, to the rows of a strided tensor; tokens: a bit each

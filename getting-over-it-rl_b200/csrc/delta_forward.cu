@@ -15,7 +15,8 @@ struct Forward {
     void *kept;       // S at the start of every span (Saved), or NULL
     int32_t keep;     // tokens of a span
     int32_t tiles_v;  // 16-column tiles of V
-    bool wide_q, wide_k, wide_v, wide_o, wide_r;
+    int grain_q, grain_k, grain_v;  // rows_grain
+    bool wide_o, wide_r;                     // rows of 16-byte pieces
 };
 
 template <class P, int KP, int MT, bool AHEAD>
@@ -92,9 +93,9 @@ __global__ void __maxnreg__(AHEAD ? 232 : 168)  // 168: 12 warps an SM
             const int at = i * kChunk, left = steps - at;
             if (left > 0) {
                 E *Q = (E *)(sm + (i & 3) * slot), *Kb = Q + kChunk * L::pitch, *Vb = Kb + kChunk * L::pitch;
-                chunk_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, K, KP, f.wide_q, lane);
-                chunk_rows(Kb, L::pitch, k + (int64_t)at * ks, ks, left, K, KP, f.wide_k, lane);
-                chunk_rows(Vb, vp, v + (int64_t)at * vs, vs, left, V - block0, warps * 16 * MT, f.wide_v, lane);
+                chunk_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, K, KP, f.grain_q, lane);
+                chunk_rows(Kb, L::pitch, k + (int64_t)at * ks, ks, left, K, KP, f.grain_k, lane);
+                chunk_rows(Vb, vp, v + (int64_t)at * vs, vs, left, V - block0, warps * 16 * MT, f.grain_v, lane);
             }
             cp_commit();
         };
@@ -224,9 +225,9 @@ __global__ void __maxnreg__(AHEAD ? 232 : 168)  // 168: 12 warps an SM
         auto load = [&](int tile) {
             E *Q = (E *)(sm + (tile & 1) * slot), *Kb = Q + TILE * L::pitch, *Vb = Kb + TILE * L::pitch;
             const int at = tile * TILE, left = steps - at < TILE ? steps - at : TILE;
-            load_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, TILE, K, KP, f.wide_q, threadIdx.x, threads);
-            load_rows(Kb, L::pitch, k + (int64_t)at * ks, ks, left, TILE, K, KP, f.wide_k, threadIdx.x, threads);
-            load_rows(Vb, vp, v + (int64_t)at * vs, vs, left, TILE, V - block0, warps * 16 * MT, f.wide_v, threadIdx.x, threads);
+            load_rows(Q, L::pitch, q + (int64_t)at * qs, qs, left, TILE, K, KP, f.grain_q, threadIdx.x, threads);
+            load_rows(Kb, L::pitch, k + (int64_t)at * ks, ks, left, TILE, K, KP, f.grain_k, threadIdx.x, threads);
+            load_rows(Vb, vp, v + (int64_t)at * vs, vs, left, TILE, V - block0, warps * 16 * MT, f.grain_v, threadIdx.x, threads);
             cp_commit();
         };
         RawGate<T> gate[N];
@@ -290,10 +291,10 @@ cudaError_t forward_typed(const goib2d_delta_desc &d, void *saved, cudaStream_t 
     const Saved at = delta_saved(d);
     f.r = saved, f.kept = saved ? (char *)saved + at.r : nullptr, f.keep = at.keep, f.tiles_v = at.tiles_v;
     const int V = d.value_dim, z = sizeof(T);
-    f.wide_q = rows_aligned(d.q, d.q_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
-    f.wide_k = rows_aligned(d.k, d.k_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
-    f.wide_v = rows_aligned(d.v, d.v_stride, d.n_worlds, d.n_steps, d.heads, V, z);
-    f.wide_o = rows_aligned(d.out, d.out_stride, d.n_worlds, d.n_steps, d.heads, V, z);
+    f.grain_q = rows_grain(d.q, d.q_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
+    f.grain_k = rows_grain(d.k, d.k_stride, d.n_worlds, d.n_steps, d.key_heads, d.key_dim, z);
+    f.grain_v = rows_grain(d.v, d.v_stride, d.n_worlds, d.n_steps, d.heads, V, z);
+    f.wide_o = rows_grain(d.out, d.out_stride, d.n_worlds, d.n_steps, d.heads, V, z) == 16;
     f.wide_r = V % 8 == 0;
     switch (padded_keys(d.key_dim)) {
         case 32: return forward_wide<T, P, 32>(f, s);

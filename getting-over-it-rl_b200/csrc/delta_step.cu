@@ -113,9 +113,9 @@ __global__ void __launch_bounds__(1024) goib2d_delta_step_flat_kernel(const __gr
     const int tid = (z * RY + y) * X + x, threads = X * RY * Z;
     const float *in = d.state_in + (int64_t)first * K * V;
     if constexpr (WIDE)
-        for (int i = tid * 4; i < held; i += threads * 4) cp_async16(sm + i, in + i);
+        for (int i = tid * 4; i < held; i += threads * 4) cp_async<16>(sm + i, in + i);
     else
-        for (int i = tid; i < held; i += threads) cp_async4(sm + i, in + i);
+        for (int i = tid; i < held; i += threads) cp_async<4>(sm + i, in + i);
     cp_commit();
     const T *k = row<T>(d.k, d.k_stride, n, 0, hk), *q = row<T>(d.q, d.q_stride, n, 0, hk);
     for (int i = y * X + x; i < K; i += X * RY)

@@ -529,6 +529,7 @@ def test_c_entries_refuse_bad_arguments():
         assert call(desc(hk=0)) == einval and call(desc(h=3, hk=2)) == einval and call(desc(K=0)) == einval
         assert call(desc(K=129)) == elimit and call(desc(V=129)) == elimit
         assert call(desc(n=1 << 31)) == elimit and call(desc(n=1 << 20, t=1 << 50)) == elimit
+        assert call(desc(v=18)) == einval and call(desc(k=17, dtype=1)) == einval and call(desc(s_out=18)) == einval
         assert call(desc(q=0)) == einval and call(desc(beta=0)) == einval and call(desc(s_out=0)) == einval
         assert call(desc(n=0, q=0, s_out=0)) >= 0
     assert lib.goib2d_delta_step(desc(t=2), None) == einval and lib.goib2d_delta_step(desc(s_in=0), None) == einval
