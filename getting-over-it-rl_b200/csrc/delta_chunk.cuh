@@ -50,7 +50,6 @@ struct Square<Half> {
         split(x[0], x[1], h.x, l.x), split(x[2], x[3], h.y, l.y), split(x[4], x[5], h.z, l.z), split(x[6], x[7], h.w, l.w);
         *(uint4 *)&hi[r][c] = h, *(uint4 *)&lo[r][c] = l;
     }
-    __device__ __forceinline__ Half::B1 n_rows1(int lane) const { return Half::n_rows(&hi[0][0], 24, 0, 0, lane); }
     __device__ __forceinline__ Half::B2 n_rows(int lane) const {
         Half::B2 b;
         ldsm(b.hi, at_b(&hi[0][0], 24, 0, 0, lane)), ldsm(b.lo, at_b(&lo[0][0], 24, 0, 0, lane));
@@ -70,7 +69,6 @@ struct Square<Full> {
         *(float4 *)&x[r][c] = make_float4(y[0], y[1], y[2], y[3]);
         *(float4 *)&x[r][c + 4] = make_float4(y[4], y[5], y[6], y[7]);
     }
-    __device__ __forceinline__ Full::B1 n_rows1(int lane) const { return Full::n_rows(&x[0][0], 24, 0, 0, lane); }
     __device__ __forceinline__ Full::B1 n_rows(int lane) const { return Full::n_rows(&x[0][0], 24, 0, 0, lane); }
     __device__ __forceinline__ Full::B1 k_rows(int lane) const { return Full::k_rows(&x[0][0], 24, 0, 0, lane); }
 };

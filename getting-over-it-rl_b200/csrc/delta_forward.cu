@@ -138,7 +138,7 @@ __global__ void __maxnreg__(AHEAD ? 232 : 168)  // 168: 12 warps an SM
                 for (int m = 0; m < MT; ++m) {
                     const typename P::A2 a = P::exact(S[m][2 * j], S[m][2 * j + 1]);
                     P::mul(Y[m][0], Y[m][1], a, kb);
-                    P::mul(O[m][0], O[m][1], P::first(a), qb);  // Half: o is rounded to bfloat16, S once before it
+                    P::mul(O[m][0], O[m][1], P::first(a), qb);  // Half: S is rounded once, as o is: 2.0e-3 off, 1.7e-3 without
                 }
             }
             const typename P::B2 z = c.z.k_rows(lane);
@@ -181,10 +181,10 @@ __global__ void __maxnreg__(AHEAD ? 232 : 168)  // 168: 12 warps an SM
             }
             typename P::A2 u[MT];
             {
-                const typename P::B1 p = c.p.n_rows1(lane);
+                const typename P::B2 p = c.p.n_rows(lane);
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                    P::mul(O[m][0], O[m][1], P::rounded(Y[m][0], Y[m][1]), p);
+                    P::mul(O[m][0], O[m][1], P::exact(Y[m][0], Y[m][1]), p);
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
