@@ -313,7 +313,7 @@ __device__ __forceinline__ void put_block(bf16 *p, const Half::A1 &a, int lane) 
 }
 
 template <class T, class P, int KP, int C>
-__global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, KP <= 64 && sizeof(typename P::E) == 2 ? 3 : 1)
+__global__ void __launch_bounds__(Span<P, KP, C>::warps * 32, sizeof(typename P::E) == 4 ? 1 : KP == 128 ? 1 : KP == 64 ? 3 : 4)
     goib2d_delta_back_span_kernel(const __grid_constant__ Backward f) {
     using L = Span<P, KP, C>;
     using E = typename P::E;

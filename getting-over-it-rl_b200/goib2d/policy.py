@@ -61,29 +61,25 @@ def _reset(x, shape, device):
 def _sizes(q, v, steps):
     """(worlds, steps, heads, key heads, K, V) of q (N, [T,] key heads, K) and v (N, [T,] heads, V)."""
     dims = 4 if steps else 3
-    for name, x in (("q", q), ("v", v)):
-        if not isinstance(x, torch.Tensor) or not x.is_cuda:
-            raise TypeError(f"{name} must be a CUDA tensor")
-        if x.dim() != dims or x.dtype not in _DTYPE:
-            raise ValueError(f"{name} must be a float32 or bfloat16 tensor of {dims} axes, got {tuple(x.shape)} {x.dtype}")
+    if not (isinstance(q, torch.Tensor) and isinstance(v, torch.Tensor) and q.is_cuda and v.is_cuda):
+        raise TypeError("q and v must be CUDA tensors")
+    if q.dim() != dims or v.dim() != dims or v.dtype not in _DTYPE:
+        raise ValueError(f"q and v must be float32 or bfloat16 tensors of {dims} axes, got {tuple(q.shape)} {q.dtype} and "
+                         f"{tuple(v.shape)} {v.dtype}")
     hk, K = q.shape[-2:]
-    h, V = v.shape[-2:]
+    if steps:
+        n, t, h, V = v.shape
+    else:
+        (n, h, V), t = v.shape, 1
     if h < 1 or hk < 1 or h % hk:
         raise ValueError(f"{h} value heads over {hk} key heads")
     if not (1 <= K <= MAX_DIM and 1 <= V <= MAX_DIM):
         raise ValueError(f"key and value channels must be 1..{MAX_DIM}, got {K} and {V}")
-    return v.shape[0], v.shape[1] if steps else 1, h, hk, K, V
+    return n, t, h, hk, K, V
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _alike(dt, device, *tensors):
-    for x in tensors:
-        if x.dtype is not dt or x.device != device:
-            return False
-    return True
 
 
 def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
@@ -100,8 +96,10 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     os_ = out.stride()
     if not (len(vs) == len(qs) == len(os_) == 3 and q.shape == k.shape and heads == beta.shape and heads == shape[:2] and
             out.shape == shape and q.shape[0] == shape[0] and state.shape == (*heads, q.shape[2], shape[2]) and
-            vs[2] == qs[2] == ks[2] == os_[2] == 1 and dt in _DTYPE and _alike(dt, device, q, k, g, beta, out) and
-            v.is_cuda and state.dtype is torch.float32 and state.device == device and state.is_contiguous()):
+            vs[2] == qs[2] == ks[2] == os_[2] == 1 and dt in _DTYPE and
+            dt is q.dtype is k.dtype is g.dtype is beta.dtype is out.dtype and state.dtype is torch.float32 and
+            0 <= v.get_device() == q.get_device() == k.get_device() == g.get_device() == beta.get_device() ==
+            out.get_device() == state.get_device() and state.is_contiguous()):
         _check_step(state, q, k, v, g, beta, out)
     n, h, V = shape
     hk, K = q.shape[1:]
@@ -147,24 +145,28 @@ def _describe(sizes, q, k, v, g, beta, state, reset, scale, last, out):
     """goib2d_delta_desc of a rollout call."""
     n, t, h, hk, K, V = sizes
     device, dt = v.device, v.dtype
-    qp, qs = _rows("q", q, (n, t, hk, K), dt, device)
-    kp, ks = _rows("k", k, (n, t, hk, K), dt, device)
-    vp, vs = _rows("v", v, (n, t, h, V), dt, device)
-    gp, gs = _rows("g", g, (n, t, h), dt, device, False)
-    bp, bs = _rows("beta", beta, (n, t, h), dt, device, False)
-    rp, rs = _reset(reset, (n, t), device)
+    qs, ks, vs, gs, bs, os_ = q.stride(), k.stride(), v.stride(), g.stride(), beta.stride(), out.stride()
+    if not (q.shape == k.shape == (n, t, hk, K) and g.shape == beta.shape == (n, t, h) and
+            qs[3] == ks[3] == vs[3] == 1 and dt is q.dtype is k.dtype is g.dtype is beta.dtype and
+            v.get_device() == q.get_device() == k.get_device() == g.get_device() == beta.get_device()):
+        for name, x, shape in (("q", q, (n, t, hk, K)), ("k", k, (n, t, hk, K)), ("v", v, (n, t, h, V))):
+            _rows(name, x, shape, dt, device)
+        for name, x in (("g", g), ("beta", beta)):
+            _rows(name, x, (n, t, h), dt, device, False)
+    rp, rs = (0, (0, 0)) if reset is None else _reset(reset, (n, t), device)
     sp = 0 if state is None else _state("state", state, (n, h, K, V), device)
-    return _DESC.pack(n, t, h, hk, K, V, _DTYPE[dt], scale, qp, kp, vp, gp, bp, rp, sp, last.data_ptr(),
-                      out.data_ptr(), *qs, *ks, *vs, *gs, *bs, *out.stride()[:3], *rs)
+    return _DESC.pack(n, t, h, hk, K, V, _DTYPE[dt], scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
+                      beta.data_ptr(), rp, sp, last.data_ptr(), out.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
+                      vs[0], vs[1], vs[2], *gs, *bs, os_[0], os_[1], os_[2], *rs)
 
 
 def _forward(q, k, v, g, beta, state, reset, scale, train):
-    """(o, last state, what the backward pass keeps or None)."""
-    sizes = n, t, h, hk, K, V = _sizes(q, v, True)
+    """(o, last state, what the backward pass keeps or None). o has v's order of axes in memory where v is dense."""
+    sizes = n, _, h, _, K, V = _sizes(q, v, True)
     device = v.device
     lib = native.load()
-    out = torch.empty((n, t, h, V), dtype=v.dtype, device=device)
-    last = torch.empty((n, h, K, V), dtype=torch.float32, device=device)
+    out = torch.empty_like(v) if v.stride(3) == 1 else torch.empty(v.shape, dtype=v.dtype, device=device)
+    last = torch.empty((n, h, K, V), dtype=torch.float32, device=device) if state is None else torch.empty_like(state)
     desc = _describe(sizes, q, k, v, g, beta, state, reset, scale, last, out)
     saved = None
     if train:
@@ -222,7 +224,8 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
     rollout recorded step by step goes in as x.transpose(0, 1). Differentiable in q, k, v, g, beta and state."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
+                                    beta.requires_grad or (state is not None and state.requires_grad)):
         return _DeltaRule.apply(q, k, v, g, beta, state, reset, float(scale))
     return _forward(q, k, v, g, beta, state, reset, float(scale), False)[:2]
 
@@ -245,35 +248,36 @@ def clip_grads_(grads, max_norm):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
-    grads = [x for x in grads if x is not None]
-    if not grads:
+    where, numel, types = [], [], []
+    index = None
+    for x in grads:
+        if x is None:
+            continue
+        if index is None:
+            device, index = x.device, x.get_device()
+            if index < 0:
+                raise TypeError("gradients must be CUDA tensors")
+        dt = _DTYPE.get(x.dtype)
+        if dt is None or x.get_device() != index or x.layout is not torch.strided:
+            raise ValueError(f"gradients must be dense float32 or bfloat16 tensors on {device}, got {x.dtype} on {x.device} "
+                             f"({x.layout})")
+        if not (x.is_contiguous() or _dense(x)):
+            raise ValueError(f"a gradient of shape {tuple(x.shape)} and strides {x.stride()} is not dense in memory")
+        n = x.numel()
+        if n:
+            where.append(x.data_ptr()), numel.append(n), types.append(dt)
+    if index is None:
         raise ValueError("no gradients")
-    device = grads[0].device
-    if device.type != "cuda":
-        raise TypeError("gradients must be CUDA tensors")
-    index = device.index
-    if not (all(x.get_device() == index and x.layout is torch.strided and x.dtype in _DTYPE for x in grads) and
-            all(x.is_contiguous() or _dense(x) for x in grads)):
-        for x in grads:
-            if x.get_device() != index or x.layout is not torch.strided or x.dtype not in _DTYPE:
-                raise ValueError(f"gradients must be dense float32 or bfloat16 tensors on {device}, got {x.dtype} on "
-                                 f"{x.device} ({x.layout})")
-            if not (x.is_contiguous() or _dense(x)):
-                raise ValueError(f"a gradient of shape {tuple(x.shape)} and strides {x.stride()} is not dense in memory")
-    grads = [x for x in grads if x.numel()]
-    count = len(grads)
-    where = [x.data_ptr() for x in grads]
+    count = len(where)
     if len(set(where)) != count:
         raise ValueError("the same gradient twice")
     table = array("q", bytes(_GRAD.size * count))
-    table[0::3] = array("q", where)
-    table[1::3] = array("q", [x.numel() for x in grads])
-    table[2::3] = array("q", [_DTYPE[x.dtype] for x in grads])
+    table[0::3], table[1::3], table[2::3] = array("q", where), array("q", numel), array("q", types)
     packed = table.buffer_info()[0]
     lib = native.load()
-    norm = torch.empty((), dtype=torch.float32, device=device)
     size = lib.goib2d_clip_workspace_bytes(packed, count)
     native.check(min(size, 0))
-    work = torch.empty(size, dtype=torch.uint8, device=device)
-    _call(device, lib.goib2d_clip_grads, packed, count, max_norm, norm.data_ptr(), work.data_ptr())
-    return norm
+    result = torch.empty(size // 4 + 4, dtype=torch.float32, device=device)  # the norm, and the workspace 16 bytes on
+    at = result.data_ptr()
+    _call(device, lib.goib2d_clip_grads, packed, count, max_norm, at, at + 16)
+    return result[0]
