@@ -335,7 +335,8 @@ enum { GOIB2D_FLOAT32 = 0, GOIB2D_BFLOAT16 = 1 };
  * sum and the state are float32. Strides are in elements, for worlds, steps and heads; channels are contiguous.
  * state_in / state_out: contiguous [n_worlds][heads][key_dim][value_dim]; state_in NULL = zeros; they may be the
  * same buffer, and may not overlap otherwise. reset: one byte per world and step, or NULL. key_dim and value_dim
- * 1..128, heads a multiple of key_heads. */
+ * 1..128, heads a multiple of key_heads; a step's stride below 2^31 elements; pointers aligned to their elements. A value
+ * that is not finite spoils the tokens that see it, up to the next one that starts from S' = 0, and no others. */
 typedef struct goib2d_delta_desc {
     int64_t n_worlds, n_steps;
     int32_t heads, key_heads, key_dim, value_dim, dtype;
@@ -352,7 +353,9 @@ typedef struct goib2d_delta_desc {
 
 /* Gradients of the rollout's inputs, in their types, from those of its outputs: dout (as out; NULL = zeros) and
  * dstate_out (of the last state; NULL = zeros). dstate_in may be NULL (not wanted). dq and dk are summed over the
- * value heads that share a key head; dg is 0 where the state starts afresh. */
+ * value heads that share a key head; dg is 0 where the state starts afresh. Inputs that are not finite make the
+ * gradients of the tokens about them (64 steps at most, and those before them in their episode) not finite, except
+ * what state_in held where a world's first token starts from S' = 0. */
 typedef struct goib2d_delta_grads {
     const void *dout;
     const float *dstate_out;
