@@ -287,6 +287,46 @@ def test_a_world_recovers_from_values_that_are_not_finite(V, n, dtype, bad):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+# few and many worlds; bfloat16 in full products (at most 4096 tokens) and not; all heads, or one of the key head's two
+@pytest.mark.parametrize("n,h,hk,K,V,heads", [(12, 2, 1, 32, 40, 2), (12, 1, 1, 128, 71, 1), (80, 2, 1, 64, 64, 1),
+                                              (40, 2, 2, 128, 128, 2), (150, 1, 1, 20, 16, 1)])
+def test_gradients_of_a_world_that_recovers(n, h, hk, K, V, heads, dtype, bad):
+    """What is not finite in one episode does not reach the gradients of the episodes before it and after it, in the
+    same chunk of tokens or elsewhere, nor other worlds and heads."""
+    t = 150
+    a = rollout(n, t, h, hk, K, V, dtype, seed=21, resets=False)
+    r = np.random.default_rng(5)
+    dout = torch.from_numpy(r.standard_normal((n, t, h, V))).to(dtype).cuda()
+    dlast = torch.from_numpy(r.standard_normal((n, h, K, V))).float().cuda()
+    reset = torch.zeros(n, t, dtype=torch.bool, device="cuda")
+    spoilt = torch.zeros(n, t, h, dtype=torch.bool, device="cuda")  # the episodes
+    dirty, dirty_dout = {x: y.clone() if y is not None else y for x, y in a.items()}, dout.clone()
+    places = [("v", 3, 5), ("k", 4, 8), ("q", 7, 8), ("k", 14, 15), ("v", 15, 73), ("g", 70, 70), ("beta", 63, 64),
+              ("dout", 40, 41), ("q", 100, 149), ("k", 2, 2), ("g", 130, 149)]
+    for world, (name, first, last) in enumerate(places):
+        x = dirty_dout if name == "dout" else dirty[name]
+        x[world, first:last + 1, :heads if name not in ("q", "k") else None] = bad
+        hit = slice(None) if name in ("q", "k") else slice(heads)
+        reset[world, first - 2] = True
+        spoilt[world, first - 2:last + 1, hit] = True
+        for i in (last + 1, last + 4):
+            if i < t:
+                reset[world, i] = True
+    dirty["reset"] = a["reset"] = reset
+    _, _, got = backward(dirty, dirty_dout, dlast)
+    _, _, want = backward(wide(a), dout.double().cpu(), dlast.double().cpu(), recurrence)
+    key_spoilt = spoilt.view(n, t, hk, h // hk).any(-1)
+    for x in ("q", "k", "v", "g", "beta"):
+        clean = ~(key_spoilt if x in ("q", "k") else spoilt)
+        assert off(got[x][clean], want[x][clean.cpu()]) <= 2 * TOL[dtype], x
+        assert not got[x][~clean].float().isfinite().all(), x
+    first_clean = ~spoilt[:, 0]
+    assert off(got["state"][first_clean], want["state"][first_clean.cpu()]) <= 2 * TOL[F32]
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("g", [0.0, -1e-6, -30.0, -90.0, 0.05])
 def test_decays_from_none_to_all(g):
     """No decay at all, a chunk whose decays multiply to less than float32 holds, and growth."""
