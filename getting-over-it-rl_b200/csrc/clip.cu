@@ -7,7 +7,8 @@
 // holds some 100 MB of. The tensor table travels in the launch's parameters: a call makes no copy and keeps nothing.
 // Squares are summed in float32 over a thread's 16 bytes, and from there on in float64; where such a sum leaves the
 // range in which float32 carries it, in float64 from the squares on. Every block's sum goes to its own place and every
-// block adds all of them in one order: the same inputs give the same bits.
+// block adds all of them in one order: the same inputs give the same bits. 63 M weights in bfloat16 and float32: 45 to 54
+// us, 4.7 to 5.6 TB/s of one read and one write; 205 k: 6.4 us, the launch and the meeting.
 #include <cooperative_groups.h>
 
 #include "policy.cuh"

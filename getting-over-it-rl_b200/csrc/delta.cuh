@@ -77,23 +77,31 @@ inline Saved delta_saved(const goib2d_delta_desc &d) {
     return s;
 }
 
-// How the columns of V are shared out in the passes over rollouts: a block takes 64 columns of one (world, head) with
-// warps of 32 (of 16, where a state has 128 channels: 64 accumulators a thread either way); where that makes fewer
-// than two blocks for an SM, in the shape for few (ahead, delta_chunk.cuh), with warps of 16 columns, and so many in a
-// block that every SM has one, up to four.
+// How the columns of V are shared out in the passes over rollouts: a block takes 64 columns of one (world, head). With
+// many, by warps of 32 columns that do everything in turn. Ahead (delta_chunk.cuh), by warps of 16 and two more that
+// prepare: where all blocks run at once that way, at 168 registers a thread, and at more than 64 key channels (64
+// accumulators a thread with 16 columns). With fewer blocks than SMs, blocks of fewer warps, down to one, for up to
+// 100 of them, and 232 registers, which leave an SM one block. Measured, many / ahead, us:
+//   rollouts of 256 steps, 64 x 64 bfloat16: 148 (world, head)s 46 / 23, 296: 46 / 27, 444: 57 / 50 (16 steps: 8.4 / 8.8),
+//   4096 worlds x 4: 404 / 458; float32: 296 of 256 steps 92 / 59, 444 of 16: 10.5 / 13.1;
+//   32 x 32 float32 (three blocks an SM): 444 of 16 steps 6.2 / 5.8, 512: 6.4 / 9.3;
+//   128 x 128, training, 64 steps: 1024 x 4 bfloat16 1311 / 1261, 512 x 4 float32 1931 / 1817;
+//   128 x 128 bfloat16, training, 37 (world, head)s of 512 steps: 206 at 168 registers, 173 at 232.
 struct Split {
     int MT, warps, blocks;
-    bool ahead;
+    int ahead;  // 0: no; 1: one block to an SM; 2: more
     explicit Split(const goib2d_delta_desc &d) {
         const int64_t nh = d.n_worlds * d.heads;
-        const int tiles = (d.value_dim + 15) / 16;
-        ahead = nh * ((tiles + 3) / 4) < 2 * 148;
-        MT = ahead || tiles == 1 || d.key_dim > 64 ? 1 : 2;
+        const int tiles = (d.value_dim + 15) / 16, most = tiles < 4 ? tiles : 4;
+        const int at_once = 148 * (65536 / (168 * 32 * (most + 2)));
+        ahead = d.key_dim > 64 || nh * ((tiles + 3) / 4) <= at_once ? 2 : 0;
+        MT = ahead || tiles == 1 ? 1 : 2;
         const int all = (tiles + MT - 1) / MT;
         warps = all < 4 / MT ? all : 4 / MT;
         if (ahead)
             while (warps > 1 && nh * ((all + warps - 1) / warps) < 100) warps = (warps + 1) / 2;
         blocks = (all + warps - 1) / warps;
+        if (ahead && nh * blocks <= 148) ahead = 1;
     }
 };
 

@@ -19,9 +19,9 @@ namespace gb {
 constexpr int kChunk = 16;
 
 // The passes over rollouts come in two shapes. With blocks for every SM, all warps of a block load a tile of chunks,
-// prepare one each and solve them in turn: nothing waits idle, as others have the SM meanwhile. With few (worlds, heads)
-// a chunk's latency is the rollout's: then two warps more run ahead of the others and prepare every second chunk each
-// (AHEAD), and the columns are spread over more warps.
+// prepare one each and solve them in turn: nothing waits idle, as others have the SM meanwhile. Where all blocks run at
+// once a chunk's latency is the rollout's: then two warps more run ahead of the others and prepare every second chunk
+// each (AHEAD), and the columns are spread over more warps. Split (delta.cuh) chooses, with both measured.
 template <class P>
 constexpr int kTile = sizeof(typename P::E) == 2 ? 32 : 16;  // tokens of a tile, so that six blocks of 64 channels fit
 
