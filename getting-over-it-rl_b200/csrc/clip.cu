@@ -7,8 +7,10 @@
 // holds some 100 MB of. The tensor table travels in the launch's parameters: a call makes no copy and keeps nothing.
 // Squares are summed in float32 over a thread's 16 bytes, and from there on in float64; where such a sum leaves the
 // range in which float32 carries it, in float64 from the squares on. Every block's sum goes to its own place and every
-// block adds all of them in one order: the same inputs give the same bits. 63 M weights in bfloat16 and float32: 45 to 54
-// us, 4.7 to 5.6 TB/s of one read and one write; 205 k: 6.4 us, the launch and the meeting.
+// block adds all of them in one order: the same inputs give the same bits. 63 M weights in
+// bfloat16 and float32 (253 MB read and written once): 64 us from a cold L2, 54 from a warm one, 4.0 and 4.7 TB/s; where there is nothing
+// to scale 37 and 31. 205 k: 6.4 us, the launch and the meeting. A block's tiles are neighbours, so that most batches of them
+// lie in one tensor and need one branch and no bookkeeping a piece: with tiles a grid apart, 72 and 70 us, at 2.4 times the instructions.
 #include <cooperative_groups.h>
 
 #include "policy.cuh"
@@ -18,7 +20,7 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kBytes = kThreads * 16;  // of a tile
-constexpr int kKept = 12;              // tiles of a block that stay in shared memory
+constexpr int kKept = 12;              // tiles of a block that stay in shared memory, whole batches
 constexpr int kBatch = 4;              // tiles whose loads are in flight together
 constexpr int kSms = 148;
 constexpr int kMost = 1024;            // tensors of a launch: 20 KB of its 32 KB of parameters
@@ -57,12 +59,20 @@ struct Cursor {
         base = (char *)T.ptr[i] + threadIdx.x * (wide ? 16 : half ? 2 : 4);
     }
     __device__ __forceinline__ explicit Cursor(const Table<N> &T) : T(T) { tensor(); }
-    __device__ __forceinline__ Piece at(int t) {
+    __device__ __forceinline__ void to(int t) {
         if (t < lo || t >= hi) {
             while (t >= T.end[i] >> 1) ++i;
             while (i > 0 && t < T.end[i - 1] >> 1) --i;
             tensor();
         }
+    }
+    // The thread's 16 bytes of tile t where it and the kBatch - 1 behind it are whole tiles of one aligned tensor, else NULL.
+    __device__ __forceinline__ uint4 *batch(int t) {
+        to(t);
+        return wide && t + kBatch < hi ? (uint4 *)(base + (int64_t)(t - lo) * kBytes) : nullptr;
+    }
+    __device__ __forceinline__ Piece at(int t) {
+        to(t);
         Piece x{base + (int64_t)(t - lo) * kBytes, 1 << 30, half, wide};
         if (t + 1 == hi) {
             const int size = half ? 2 : 4;
@@ -159,27 +169,44 @@ __device__ __forceinline__ double block_sum(double x) {
 template <int N>
 __global__ void __launch_bounds__(kThreads) goib2d_clip_kernel(const __grid_constant__ Table<N> T) {
     extern __shared__ uint4 kept[];
-    const int tiles = T.n ? T.end[T.n - 1] >> 1 : 0, grid = gridDim.x;
+    const int tiles = T.n ? T.end[T.n - 1] >> 1 : 0;
+    const int first = (int)((int64_t)blockIdx.x * tiles / gridDim.x);  // the block's tiles, neighbours
+    const int mine = (int)((int64_t)(blockIdx.x + 1) * tiles / gridDim.x) - first;
     Cursor<N> cursor(T);
     if (T.mode & kSum) {
         double sum = 0.0;
-        for (int k = 0, t0 = blockIdx.x; t0 < tiles; k += kBatch, t0 += kBatch * grid) {
+        for (int k = 0; k < mine; k += kBatch) {
             uint4 y[kBatch];
-            bool half[kBatch];
+            const uint4 *p = k + kBatch <= mine ? cursor.batch(first + k) : nullptr;
+            if (p) {
+                if (k < kKept)
 #pragma unroll
-            for (int e = 0; e < kBatch; ++e) {
-                const int t = t0 + e * grid;
-                y[e] = make_uint4(0, 0, 0, 0), half[e] = false;
-                if (t < tiles) {
-                    const Piece x = cursor.at(t);
-                    y[e] = load(x), half[e] = x.half;
+                    for (int e = 0; e < kBatch; ++e) y[e] = __ldcs(p + e * kThreads);
+                else
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) y[e] = p[e * kThreads];
+                if (cursor.half)
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) sum += squares(y[e], true);
+                else
+#pragma unroll
+                    for (int e = 0; e < kBatch; ++e) sum += squares(y[e], false);
+            } else {
+                bool half[kBatch];
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e) {
+                    y[e] = make_uint4(0, 0, 0, 0), half[e] = false;
+                    if (k + e < mine) {
+                        const Piece x = cursor.at(first + k + e);
+                        y[e] = load(x), half[e] = x.half;
+                    }
                 }
-            }
 #pragma unroll
-            for (int e = 0; e < kBatch; ++e) {
-                if (k + e < kKept) kept[(k + e) * kThreads + threadIdx.x] = y[e];
-                sum += squares(y[e], half[e]);
+                for (int e = 0; e < kBatch; ++e) sum += squares(y[e], half[e]);
             }
+            if (k < kKept)
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e) kept[(k + e) * kThreads + threadIdx.x] = y[e];
         }
         sum = block_sum(sum);
         if (threadIdx.x == 0) T.part[T.first + blockIdx.x] = sum;
@@ -192,21 +219,28 @@ __global__ void __launch_bounds__(kThreads) goib2d_clip_kernel(const __grid_cons
     if (T.norm && blockIdx.x == 0 && threadIdx.x == 0) *T.norm = norm;
     const float c = T.max_norm / (norm + 1e-6f);
     if (c >= 1.0f) return;  // NaN goes on: every element becomes NaN
-    const int mine = (tiles - (int)blockIdx.x + grid - 1) / grid;  // tiles of this block
     const int held = T.mode & kSum ? (mine < kKept ? mine : kKept) : 0;
-    for (int k = mine - 1; k >= held; k -= kBatch) {
+    for (int k = mine; k > 0;) {
+        const bool here = k <= held;
+        const int n = k - (here ? 0 : held) < kBatch ? k - (here ? 0 : held) : kBatch;
+        k -= n;
+        uint4 *const p = n == kBatch ? cursor.batch(first + k) : nullptr;
         uint4 y[kBatch];
-        Piece x[kBatch];
+        if (p) {
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-            if (k - e >= held) x[e] = cursor.at(blockIdx.x + (k - e) * grid), y[e] = load(x[e]);
+            for (int e = 0; e < kBatch; ++e) y[e] = here ? kept[(k + e) * kThreads + threadIdx.x] : p[e * kThreads];
+            if (cursor.half)
 #pragma unroll
-        for (int e = 0; e < kBatch; ++e)
-            if (k - e >= held) store(x[e], scaled(y[e], x[e].half, c));
-    }
-    for (int k = held - 1; k >= 0; --k) {
-        const Piece x = cursor.at(blockIdx.x + k * grid);
-        store(x, scaled(kept[k * kThreads + threadIdx.x], x.half, c));
+                for (int e = 0; e < kBatch; ++e) __stcs(p + e * kThreads, scaled(y[e], true, c));
+            else
+#pragma unroll
+                for (int e = 0; e < kBatch; ++e) __stcs(p + e * kThreads, scaled(y[e], false, c));
+        } else {
+            for (int e = 0; e < n; ++e) {
+                const Piece x = cursor.at(first + k + e);
+                store(x, scaled(here ? kept[(k + e) * kThreads + threadIdx.x] : load(x), x.half, c));
+            }
+        }
     }
 }
 
