@@ -1,5 +1,6 @@
 // The gated delta rule, one token per world (goib2d_delta_step).
 #include "delta.cuh"
+#include "delta_step.h"
 #include "mma.cuh"
 
 namespace gb {
@@ -10,9 +11,6 @@ namespace {
 // Both products with the state come from one pass, S'^T k = a (S^T k) and S^T q = a (S^T q) + (k.q) u, summed over the row
 // groups in shared memory, where k and q lie as float32 pairs.
 
-// A block's heads in shared memory: k and q [z][K], the row groups' sums [z][y][2][4 X] (with k, with q) and k.q [z][y].
-__host__ __device__ inline int shared_floats(int K, int X, int y) { return 2 * (K + y * 4 * X) + y; }
-
 // Rows of whole 16-byte pieces: a thread's columns are neighbours, read and written 16 bytes at a time.
 constexpr int kRows = 16;  // of a thread. 8: 100 us, 16: 89 us, 32: 125 us for 4096 worlds x 4 heads of 64 x 64
 template <class T>
@@ -20,8 +18,9 @@ __global__ void __launch_bounds__(512) goib2d_delta_step_kernel(const __grid_con
     extern __shared__ __align__(16) float sm[];
     const int K = d.key_dim, V = d.value_dim, RY = blockDim.y, Z = blockDim.z, y = threadIdx.y, z = threadIdx.z;
     const int c = threadIdx.x * 4;
-    float2 *kq = (float2 *)sm + z * K;
-    float *part = sm + 2 * Z * K + z * RY * 2 * V + c, *dots = sm + 2 * Z * (K + RY * V) + z * RY;
+    const StepShared at(K, V, RY, Z);
+    float2 *kq = (float2 *)(sm + at.pairs) + z * K;
+    float *part = sm + at.sums + z * RY * 2 * V + c, *dots = sm + at.dots + z * RY;
     const uint32_t nh = blockIdx.x * Z + z;
     const bool live = nh < (uint32_t)(d.n_worlds * d.heads);
     const int64_t n = live ? nh / (uint32_t)d.heads : 0;
@@ -178,14 +177,10 @@ __global__ void __launch_bounds__(1024) goib2d_delta_step_flat_kernel(const __gr
         for (int i = tid; i < held; i += threads) __stcs(to + i, sm[i]);
 }
 
-// Blocks of about 128 threads: 256 is 2 to 20 % slower at 64 x 64.
-struct Shape {
-    int x, y, z;
-    Shape(const goib2d_delta_desc &d, int rows) : x((d.value_dim + 3) / 4), y((d.key_dim + rows - 1) / rows), z(128 / (x * y)) {
-        z = z < 1 ? 1 : z > 64 ? 64 : z;
-    }
+struct Shape : StepShape {
+    Shape(const goib2d_delta_desc &d, int rows) : StepShape(d.key_dim, d.value_dim, rows) {}
     unsigned blocks(const goib2d_delta_desc &d) const { return (unsigned)((d.n_worlds * d.heads + z - 1) / z); }
-    size_t bytes(const goib2d_delta_desc &d) const { return sizeof(float) * z * shared_floats(d.key_dim, x, y); }
+    size_t bytes(const goib2d_delta_desc &d) const { return sizeof(float) * StepShared(d.key_dim, 4 * x, y, z).end; }
 };
 
 template <class T, bool WIDE>

@@ -7,6 +7,8 @@ result (2^-9) and of the two operands of the product that makes it (2^-9 each) a
 float32 whatever the inputs' type."""
 import ctypes as C
 import math
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -144,6 +146,49 @@ def test_step(n, h, hk, K, V, dtype):
         out = goib2d.delta_step_(state, *(a[x][:, t] for x in ("q", "k", "v", "g", "beta")), reset=a["reset"][:, t])
         assert off(out, want[:, t]) <= TOL[dtype]
     assert off(state, last) <= TOL[F32]
+
+
+STEP_LAYOUT = r"""
+#include <cstdio>
+#include <initializer_list>
+#include "delta_step.h"
+int main() {
+    for (int K = 1; K <= 128; ++K)
+        for (int V = 1; V <= 128; ++V)
+            for (int rows : {16, 8}) {  // rows in fours, others
+                const gb::StepShape b(K, V, rows);
+                const gb::StepShared at(K, 4 * b.x, b.y, b.z);
+                std::printf("%d %d %d %d %d %d %d %d %d %d\n", K, V, rows, b.x, b.y, b.z, at.sums, at.pairs, at.dots, at.end);
+            }
+}
+"""
+
+
+def test_step_layout(tmp_path):
+    """The one-token kernel's shared memory for all 1..128 x 1..128: the row groups' sums, which it reads and writes 16
+    bytes at a time, and the pairs of k and q start at whole pieces, and no two parts overlap."""
+    (tmp_path / "layout.cpp").write_text(STEP_LAYOUT)
+    csrc = Path(native.__file__).resolve().parent.parent / "csrc"
+    subprocess.run(["g++", "-std=c++17", "-I", str(csrc), "layout.cpp", "-o", "layout"], cwd=tmp_path, check=True)
+    lines = subprocess.run([str(tmp_path / "layout")], check=True, capture_output=True, text=True).stdout.splitlines()
+    assert len(lines) == 2 * 128 * 128
+    for line in lines:
+        K, V, rows, x, y, z, sums, pairs, dots, end = map(int, line.split())
+        assert 4 * x >= V and rows * y >= K and 1 <= z <= 64 and x * y * z <= 512, line
+        assert sums % 4 == 0 and pairs % 2 == 0, f"misaligned: K {K}, V {V}, {z} heads a block"
+        parts = sorted([(sums, z * y * 2 * 4 * x), (pairs, 2 * z * K), (dots, z * y), (end, 0)])
+        assert all(at + size <= then for (at, size), (then, _) in zip(parts, parts[1:])), line
+        assert parts[-1] == (end, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+# odd key channels and value channels in fours, with odd numbers of heads to a block; the last block is in part empty
+@pytest.mark.parametrize("n,h,hk,K,V", [(5, 3, 1, 17, 12), (11, 1, 1, 33, 32), (3, 1, 1, 65, 64), (2, 2, 1, 33, 128),
+                                        (3, 1, 1, 127, 128), (7, 4, 2, 9, 100), (7, 1, 1, 1, 100), (27, 2, 2, 3, 20),
+                                        (2, 1, 1, 81, 16), (4, 1, 1, 65, 32)])
+def test_step_odd_keys(n, h, hk, K, V, dtype):
+    test_step(n, h, hk, K, V, dtype)
 
 
 @pytest.mark.gpu
