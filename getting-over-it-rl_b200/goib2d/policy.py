@@ -58,6 +58,13 @@ def _reset(x, shape, device):
     return x.data_ptr(), x.stride()
 
 
+def _like(v):
+    """An uninitialised tensor for o: v's order of axes in memory where that leaves o's channels contiguous (of overlapping
+    windows torch's choice need not)."""
+    out = torch.empty_like(v)
+    return out if out.stride()[-1:] == (1,) else torch.empty(v.shape, dtype=v.dtype, device=v.device)
+
+
 def _sizes(q, v, steps):
     """(worlds, steps, heads, key heads, K, V) of q (N, [T,] key heads, K) and v (N, [T,] heads, V)."""
     dims = 4 if steps else 3
@@ -91,7 +98,7 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     device, dt = v.device, v.dtype
     vs, qs, ks, gs, bs = v.stride(), q.stride(), k.stride(), g.stride(), beta.stride()
     if out is None:
-        out = torch.empty_like(v)
+        out = _like(v)
     shape, heads = v.shape, g.shape
     os_ = out.stride()
     if not (len(vs) == len(qs) == len(os_) == 3 and q.shape == k.shape and heads == beta.shape and heads == shape[:2] and
@@ -161,11 +168,11 @@ def _describe(sizes, q, k, v, g, beta, state, reset, scale, last, out):
 
 
 def _forward(q, k, v, g, beta, state, reset, scale, train):
-    """(o, last state, what the backward pass keeps or None). o has v's order of axes in memory where v is dense."""
+    """(o, last state, what the backward pass keeps or None)."""
     sizes = n, _, h, _, K, V = _sizes(q, v, True)
     device = v.device
     lib = native.load()
-    out = torch.empty_like(v) if v.stride(3) == 1 else torch.empty(v.shape, dtype=v.dtype, device=device)
+    out = _like(v)
     last = torch.empty((n, h, K, V), dtype=torch.float32, device=device) if state is None else torch.empty_like(state)
     desc = _describe(sizes, q, k, v, g, beta, state, reset, scale, last, out)
     saved = None

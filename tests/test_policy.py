@@ -240,6 +240,48 @@ def test_strides(kind, dtype):
     assert torch.equal(o, o2) and torch.equal(state, state2)
 
 
+def windows(n, t, h, V, axis, dtype=F32, device="cpu"):
+    """v as overlapping windows of a signal: neighbours along this axis (1: steps, 2: heads) are shifted by one channel."""
+    step = {1: (t + V, 1, n * (t + V)), 2: (t * (h + V), h + V, 1)}[axis]
+    x = torch.from_numpy(np.random.default_rng(axis).standard_normal(2 * n * (t + V) * (h + V))).to(device, dtype)
+    return x.as_strided((n, t, h, V), (*step, 1))
+
+
+@pytest.mark.parametrize("axis", [1, 2])
+def test_outputs_of_overlapping_inputs_have_contiguous_channels(axis):
+    """The kernels write o's channels as neighbours."""
+    v = windows(3, 5, 4, 8, axis)
+    for x in (v, v[:, 0], v.transpose(0, 1), v[0, 0, 0, 0:1], v.expand(3, 5, 4, 8)[:, :1].expand(3, 5, 4, 8), v[..., :1]):
+        out = policy._like(x)
+        assert out.shape == x.shape and out.dtype == x.dtype and out.stride(-1) == 1
+        assert policy._dense(out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("axis", [1, 2])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_overlapping_inputs(axis, dtype):
+    """Values that are sliding windows give what a copy of them gives, and one token of them is not refused."""
+    a = rollout(3, 37, 4, 2, 16, 8, dtype, seed=12)
+    names = ("q", "k", "v", "g", "beta")
+    v = windows(3, 37, 4, 8, axis, dtype, "cuda")
+    copied, slid = dict(a, v=v.contiguous()), dict(a, v=v)
+    dout = torch.randn(3, 37, 4, 8, device="cuda").to(dtype)
+    out, last, grads = backward(copied, dout, None)
+    out2, last2, grads2 = backward(slid, dout, None)
+    assert out2.stride(3) == 1
+    assert off(out2, out.double().cpu()) <= 2 * TOL[dtype] and off(last2, last.double().cpu()) <= 2 * TOL[F32]
+    for x in grads:
+        assert off(grads2[x], grads[x].double().cpu()) <= 4 * TOL[dtype], x
+    want, _ = recurrence(**wide(copied))
+    assert off(goib2d.delta_rule(**slid)[0], want) <= TOL[dtype]
+    state, state2 = a["state"].clone(), a["state"].clone()
+    for t in range(3):
+        o = goib2d.delta_step_(state, *(copied[x][:, t] for x in names), reset=a["reset"][:, t])
+        o2 = goib2d.delta_step_(state2, *(slid[x][:, t] for x in names), reset=a["reset"][:, t])
+        assert torch.equal(o, o2) and torch.equal(state, state2)
+
+
 @pytest.mark.gpu
 def test_broadcast_inputs_and_gradients():
     """One key for all worlds, one decay for all heads and steps: inputs of stride 0, their gradients summed."""
