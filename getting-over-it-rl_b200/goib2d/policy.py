@@ -168,41 +168,43 @@ def _describe(sizes, q, k, v, g, beta, state, reset, scale, last, out):
 
 
 def _forward(q, k, v, g, beta, state, reset, scale, train):
-    """(o, last state, what the backward pass keeps or None)."""
+    """(o, last state, what the backward pass reads or None, the bytes that it works in)."""
     sizes = n, _, h, _, K, V = _sizes(q, v, True)
     device = v.device
     lib = native.load()
     out = _like(v)
     last = torch.empty((n, h, K, V), dtype=torch.float32, device=device) if state is None else torch.empty_like(state)
     desc = _describe(sizes, q, k, v, g, beta, state, reset, scale, last, out)
-    saved = None
+    saved, work = None, 0
     if train:
-        size = lib.goib2d_delta_saved_bytes(desc)
-        native.check(min(size, 0))
+        size, work = lib.goib2d_delta_saved_bytes(desc), lib.goib2d_delta_workspace_bytes(desc)
+        native.check(min(size, work, 0))
         saved = torch.empty(size, dtype=torch.uint8, device=device)
     _call(device, lib.goib2d_delta_forward, desc, saved.data_ptr() if train else None)
-    return out, last, saved
+    return out, last, saved, work
 
 
 class _DeltaRule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, reset, scale):
         ctx.set_materialize_grads(False)
-        out, last, saved = _forward(q, k, v, g, beta, state, reset, scale, True)
-        ctx.save_for_backward(q, k, v, g, beta, state, reset, last, saved)
+        out, last, saved, ctx.work = _forward(q, k, v, g, beta, state, reset, scale, True)
+        # neither state is read backwards: the caller may go on with the last one, or with the first one's memory
+        ctx.save_for_backward(q, k, v, g, beta, reset, saved)
         ctx.scale = scale
         return out, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dlast):
-        q, k, v, g, beta, state, reset, last, saved = ctx.saved_tensors
+        q, k, v, g, beta, reset, saved = ctx.saved_tensors
         if dout is None and dlast is None:
             return (None,) * 8
         sizes = n, t, h, hk, K, V = _sizes(q, v, True)
         device, dt = v.device, v.dtype
         lib = native.load()
-        desc = _describe(sizes, q, k, v, g, beta, state, reset, ctx.scale, last, last)
+        work = torch.empty(max(ctx.work, 16), dtype=torch.uint8, device=device)
+        desc = _describe(sizes, q, k, v, g, beta, None, reset, ctx.scale, work, v)  # o and the states are not read
         dop, dos = 0, (0, 0, 0)
         if dout is not None:
             dout = dout if dout.stride(-1) == 1 else dout.contiguous()
@@ -212,14 +214,11 @@ class _DeltaRule(torch.autograd.Function):
         dv = torch.empty((n, t, h, V), dtype=dt, device=device)
         dg, dbeta = (torch.empty((n, t, h), dtype=dt, device=device) for _ in range(2))
         first = None
-        if state is not None and ctx.needs_input_grad[5]:
+        if ctx.needs_input_grad[5]:
             first = torch.empty((n, h, K, V), dtype=torch.float32, device=device)
         grads = _GRADS.pack(dop, 0 if dlast is None else dlast.data_ptr(), dq.data_ptr(), dk.data_ptr(),
                             dv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), 0 if first is None else first.data_ptr(),
                             *dos, *dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3], *dg.stride(), *dbeta.stride())
-        size = lib.goib2d_delta_workspace_bytes(desc)
-        native.check(min(size, 0))
-        work = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
         _call(device, lib.goib2d_delta_backward, desc, grads, saved.data_ptr(), work.data_ptr())
         return dq, dk, dv, dg, dbeta, first, None, None
 

@@ -372,8 +372,9 @@ int goib2d_delta_step(const goib2d_delta_desc *desc, void *stream);
 int goib2d_delta_forward(const goib2d_delta_desc *desc, void *saved, void *stream);
 int64_t goib2d_delta_saved_bytes(const goib2d_delta_desc *desc);
 
-/* The gradients. desc as in the forward call (state_out: the state that it left; out is not read), saved what it
- * kept; workspace: goib2d_delta_workspace_bytes(desc) bytes of device memory (16-byte aligned). */
+/* The gradients. desc as in the forward call (state_in, state_out and out are not read and their memory may be gone;
+ * state_out must not be NULL), saved what it kept; workspace: goib2d_delta_workspace_bytes(desc) bytes of device
+ * memory (16-byte aligned). */
 int goib2d_delta_backward(const goib2d_delta_desc *desc, const goib2d_delta_grads *grads, const void *saved,
                           void *workspace, void *stream);
 int64_t goib2d_delta_workspace_bytes(const goib2d_delta_desc *desc);

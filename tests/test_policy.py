@@ -469,6 +469,27 @@ def test_gradients_against_differences():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_states_may_be_written_to_before_the_gradients(dtype):
+    """The gradients need neither the first nor the last state: the world goes on acting with the last one's memory (zeroed
+    where it was reset), and the first one's buffer takes the next rollout's, while the loss is still to be trained on."""
+    a = rollout(5, 40, 2, 2, 32, 24, dtype, seed=31)
+    dout = torch.randn(5, 40, 2, 24, device="cuda").to(dtype)
+    _, _, want = backward(a, dout, None)
+    first = a["state"].clone()
+    leaves = {x: a[x].clone().requires_grad_() for x in GRADS if x != "state"}
+    out, last = goib2d.delta_rule(**leaves, state=first, reset=a["reset"])
+    memory = last.detach()
+    memory[2] = 0
+    first.copy_(memory)
+    with torch.no_grad():
+        goib2d.delta_step_(memory, *(leaves[x][:, 0] for x in ("q", "k", "v", "g", "beta")))
+    got = torch.autograd.grad([out], list(leaves.values()), [dout])
+    for x, y in zip(leaves, got):
+        assert torch.equal(y, want[x]), x
+
+
+@pytest.mark.gpu
 def test_zero_steps_and_worlds():
     a = rollout(3, 4, 2, 1, 16, 16, F32)
     none = {x: y[:, :0] if x not in ("state",) else y for x, y in a.items()}
