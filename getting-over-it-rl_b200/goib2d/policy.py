@@ -21,6 +21,7 @@ from array import array
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import native
 
@@ -97,6 +98,7 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     # everything in one expression first: an acting loop calls this once per world step
     device, dt = v.device, v.dtype
     vs, qs, ks, gs, bs = v.stride(), q.stride(), k.stride(), g.stride(), beta.stride()
+    written = (state,) if out is None else (state, out)
     if out is None:
         out = _like(v)
     shape, heads = v.shape, g.shape
@@ -113,7 +115,7 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     if not (0 < K <= MAX_DIM and 0 < V <= MAX_DIM and hk > 0 and h > 0 and h % hk == 0):
         _sizes(q, v, False)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
-                                    beta.requires_grad or state.requires_grad):
+                                    beta.requires_grad or state.requires_grad or out.requires_grad):
         raise ValueError("delta_step_ is not differentiable: use delta_rule, or torch.no_grad()")
     rp, rs = (0, (0,)) if reset is None else _reset(reset, (n,), device)
     sp = state.data_ptr()
@@ -122,6 +124,7 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
                       qs[0], 0, qs[1], ks[0], 0, ks[1], vs[0], 0, vs[1], gs[0], 0, gs[1], bs[0], 0, bs[1],
                       os_[0], 0, os_[1], rs[0], 0)
     _call(device, native.load().goib2d_delta_step, desc)
+    increment_version(written)  # a graph that saved what was there before raises
     return out
 
 

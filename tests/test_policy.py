@@ -549,6 +549,29 @@ def test_streams_and_graphs():
     assert torch.equal(state, plain) and torch.equal(out, last)
 
 
+@pytest.mark.gpu
+def test_writes_of_a_step_are_seen_by_autograd():
+    """A graph that saved the memory, or a buffer given as `out`, before a step wrote to it raises, as after torch's own
+    writes, instead of giving gradients of the new contents. Tensors of inference mode have no versions."""
+    a = rollout(3, 1, 2, 1, 16, 24, F32, seed=41)
+    token = [a[x][:, 0] for x in ("q", "k", "v", "g", "beta")]
+    weight = torch.ones(24, device="cuda", requires_grad=True)
+    out = torch.zeros(3, 2, 24, device="cuda")
+    for kept in ("state", "out"):
+        state = a["state"].clone()
+        loss = ((state if kept == "state" else out) * weight).sum()
+        goib2d.delta_step_(state, *token, out=out if kept == "out" else None)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with pytest.raises(ValueError, match="differentiable"):
+        goib2d.delta_step_(state, *token, out=torch.zeros(3, 2, 24, device="cuda", requires_grad=True))
+    with torch.inference_mode():
+        memory = a["state"].clone()
+        o = goib2d.delta_step_(memory, *token, out=torch.empty(3, 2, 24, device="cuda"))
+    state = a["state"].clone()
+    assert torch.equal(goib2d.delta_step_(state, *token), o) and torch.equal(memory, state)
+
+
 # ---- clipping
 
 
