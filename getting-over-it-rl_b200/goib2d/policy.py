@@ -257,7 +257,7 @@ def clip_grads_(grads, max_norm):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
-    where, numel, types = [], [], []
+    where, numel, types, written = [], [], [], []
     index = None
     for x in grads:
         if x is None:
@@ -274,7 +274,7 @@ def clip_grads_(grads, max_norm):
             raise ValueError(f"a gradient of shape {tuple(x.shape)} and strides {x.stride()} is not dense in memory")
         n = x.numel()
         if n:
-            where.append(x.data_ptr()), numel.append(n), types.append(dt)
+            where.append(x.data_ptr()), numel.append(n), types.append(dt), written.append(x)
     if index is None:
         raise ValueError("no gradients")
     count = len(where)
@@ -289,4 +289,5 @@ def clip_grads_(grads, max_norm):
     result = torch.empty(size // 4 + 4, dtype=torch.float32, device=device)  # the norm, and the workspace 16 bytes on
     at = result.data_ptr()
     _call(device, lib.goib2d_clip_grads, packed, count, max_norm, at, at + 16)
+    increment_version(written)
     return result[0]

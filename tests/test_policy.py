@@ -634,6 +634,24 @@ def test_clip_values_that_are_not_finite_or_extreme():
     assert float(goib2d.clip_grads_([torch.empty(0, device="cuda")], 1.0)) == 0
 
 
+@pytest.mark.gpu
+def test_writes_of_clipping_are_seen_by_autograd():
+    grads = [torch.ones(5, device="cuda"), torch.ones(70, device="cuda", dtype=BF16), torch.ones(0, device="cuda")]
+    weights = [x.clone().float().requires_grad_() for x in grads[:2]]
+    losses = [(x.float() if x.dtype == BF16 else x).mul(w).sum() for x, w in zip(grads, weights)]
+    square = (grads[1] * torch.ones_like(grads[1], requires_grad=True)).sum()
+    with torch.no_grad():
+        goib2d.clip_grads_(grads, 0.5)
+    for loss in (losses[0], square):
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    losses[1].backward()  # saved a copy
+    assert torch.equal(weights[1].grad, torch.ones(70, device="cuda"))
+    with torch.inference_mode():
+        x = torch.ones(4, device="cuda")
+        assert float(goib2d.clip_grads_([x], 1.0)) == 2.0 and abs(float(x[0]) - 0.5) < 1e-6
+
+
 # ---- what is refused
 
 
