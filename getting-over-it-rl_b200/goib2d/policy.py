@@ -20,6 +20,7 @@ import struct
 from array import array
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 from torch.autograd.graph import increment_version
 
@@ -90,6 +91,12 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _no_tangents(name, tensors):
+    """Raw pointers would drop forward-mode tangents. The level is -1 outside torch.autograd.forward_ad.dual_level()."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise ValueError(f"{name} has no forward-mode derivative")
+
+
 def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     """One token for every world: state (N, H, K, V) float32 is updated in place, and o (N, H, V) in v's type is
     returned. q, k (N, Hk, K), v (N, H, V), g (log decay) and beta (N, H), reset (N,) bool or None; scale defaults
@@ -117,6 +124,7 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
                                     beta.requires_grad or state.requires_grad or out.requires_grad):
         raise ValueError("delta_step_ is not differentiable: use delta_rule, or torch.no_grad()")
+    _no_tangents("delta_step_", (state, q, k, v, g, beta, out))
     rp, rs = (0, (0,)) if reset is None else _reset(reset, (n,), device)
     sp = state.data_ptr()
     desc = _DESC.pack(n, 1, h, hk, K, V, _DTYPE[dt], K ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
@@ -233,6 +241,7 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
     rollout recorded step by step goes in as x.transpose(0, 1). Differentiable in q, k, v, g, beta and state."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
+    _no_tangents("delta_rule", (q, k, v, g, beta) if state is None else (q, k, v, g, beta, state))
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
                                     beta.requires_grad or (state is not None and state.requires_grad)):
         return _DeltaRule.apply(q, k, v, g, beta, state, reset, float(scale))
@@ -277,6 +286,7 @@ def clip_grads_(grads, max_norm):
             where.append(x.data_ptr()), numel.append(n), types.append(dt), written.append(x)
     if index is None:
         raise ValueError("no gradients")
+    _no_tangents("clip_grads_", written)
     count = len(where)
     if len(set(where)) != count:
         raise ValueError("the same gradient twice")

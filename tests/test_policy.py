@@ -688,6 +688,34 @@ def test_refusals():
     assert torch.equal(x, torch.ones_like(x))
 
 
+@pytest.mark.gpu
+def test_forward_mode_tangents_are_refused():
+    """No derivative in forward mode: tangents raise instead of being dropped; without any, the level changes nothing."""
+    from torch.autograd import forward_ad
+    a = rollout(2, 5, 2, 1, 16, 16, F32)
+    want = goib2d.delta_rule(**a)[0]
+    names = ("q", "k", "v", "g", "beta")
+    for x in names + ("state",):
+        for grad in (False, True):
+            with forward_ad.dual_level():
+                b = dict(a, **{x: forward_ad.make_dual(a[x].clone().requires_grad_(grad), torch.ones_like(a[x]))})
+                with pytest.raises((ValueError, NotImplementedError)):
+                    goib2d.delta_rule(**b)
+                if not grad:
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        goib2d.delta_step_(b["state"], *(b[y][:, 0] for y in names))
+    with forward_ad.dual_level():
+        grad = forward_ad.make_dual(torch.ones(3, device="cuda"), torch.ones(3, device="cuda"))
+        with pytest.raises(ValueError, match="forward-mode"):
+            goib2d.clip_grads_([torch.ones(2, device="cuda"), grad], 1.0)
+        assert torch.equal(goib2d.delta_rule(**a)[0], want)
+        state = a["state"].clone()
+        goib2d.delta_step_(state, *(a[y][:, 0] for y in names))
+        assert float(goib2d.clip_grads_([torch.ones(4, device="cuda")], 1.0)) == 2.0
+    with pytest.raises(ValueError, match="forward-mode"):
+        torch.func.jvp(lambda v: goib2d.delta_rule(**dict(a, v=v))[0], (a["v"],), (torch.ones_like(a["v"]),))
+
+
 def test_cpu_tensors_are_refused():
     a = {x: torch.zeros(s) for x, s in (("q", (2, 3, 1, 8)), ("k", (2, 3, 1, 8)), ("v", (2, 3, 1, 8)), ("g", (2, 3, 1)),
                                          ("beta", (2, 3, 1)))}
