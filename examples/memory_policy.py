@@ -57,11 +57,10 @@ class MemoryPolicy(nn.Module):
         return self.act(torch.cat((e, o.flatten(-2)), -1))
 
 
-def rollout(engine, scene, state, start, policy, memory, steps, std, dtype):
-    """Act for `steps` world steps; (observations, actions, resets, rewards), each (worlds, steps, ...)."""
-    n = memory.shape[0]
-    falls = torch.zeros(n, dtype=torch.int32, device="cuda")
-    reset = torch.zeros(n, dtype=torch.bool, device="cuda")
+def rollout(engine, scene, state, start, policy, memory, reset, steps, std, dtype):
+    """Act for `steps` world steps. reset: the worlds that were reset before the first one. Returns (observations, actions,
+    resets, rewards, action means), each (worlds, steps, ...), and the worlds that were reset after the last one."""
+    falls = torch.zeros(memory.shape[0], dtype=torch.int32, device="cuda")
     seen, done, acted, rewards, means = [], [], [], [], []
     for _ in range(steps):
         body = engine.observe(state, [POT])[:, 0]
@@ -77,7 +76,7 @@ def rollout(engine, scene, state, start, policy, memory, steps, std, dtype):
         seen.append(x), done.append(reset), acted.append(action), means.append(mean)
         rewards.append(after[:, 0] - body[:, 0])
         reset = falls > before
-    return (*(torch.stack(y, 1) for y in (seen, acted, done, rewards)), torch.stack(means, 1))
+    return (*(torch.stack(y, 1) for y in (seen, acted, done, rewards, means)), reset)
 
 
 def train(worlds=4096, steps=32, updates=4, dtype=torch.bfloat16, seed=0, std=0.5, max_norm=0.5, lr=1e-3, log=print):
@@ -87,13 +86,13 @@ def train(worlds=4096, steps=32, updates=4, dtype=torch.bfloat16, seed=0, std=0.
     engine = api.Engine(model, state.bodies.type.shape[1], scene.action_joints, scene.action_scale)
     policy = MemoryPolicy().cuda().to(dtype)
     optimiser = torch.optim.Adam(policy.parameters(), lr=lr, eps=1e-4)
-    memory = policy.memory(worlds, "cuda")
+    memory, fell = policy.memory(worlds, "cuda"), torch.zeros(worlds, dtype=torch.bool, device="cuda")
     results = []
     try:
         for update in range(updates):
             t = time.perf_counter()
             first = memory.clone()
-            x, action, reset, reward, acted = rollout(engine, scene, state, start, policy, memory, steps, std, dtype)
+            x, action, reset, reward, acted, fell = rollout(engine, scene, state, start, policy, memory, fell, steps, std, dtype)
             to_go = reward.flip(1).cumsum(1).flip(1)
             advantage = (to_go - to_go.mean(0)) / (to_go.std() + 1e-6)
             mean = policy(x, first, reset)

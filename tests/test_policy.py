@@ -796,3 +796,24 @@ def test_example_acts_and_trains(dtype):
         assert r["replayed"] <= 4 * TOL[dtype]
     assert all(torch.isfinite(p).all() for p in policy.parameters())
     assert any(not torch.equal(p, q) for p, q in zip(policy.parameters(), fresh.parameters()))
+
+
+@pytest.mark.gpu
+def test_example_carries_resets_from_rollout_to_rollout(monkeypatch):
+    """A world that is reset after the last step of a rollout starts the next one with an empty memory."""
+    import sys
+    from pathlib import Path
+    sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "examples"))
+    import memory_policy
+    seen, forward = [], memory_policy.MemoryPolicy.forward
+
+    def recorded(self, x, memory, reset):
+        seen.append(reset.clone())
+        return forward(self, x, memory, reset)
+
+    monkeypatch.setattr(memory_policy.MemoryPolicy, "forward", recorded)
+    monkeypatch.setattr(memory_policy, "FALLEN", 1e6)  # every world, after every step
+    memory_policy.train(worlds=32, steps=3, updates=3, dtype=F32, log=lambda line: None)
+    first, *others = seen
+    assert not first[:, 0].any() and first[:, 1:].all()
+    assert all(reset.all() for reset in others)
