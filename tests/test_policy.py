@@ -191,6 +191,28 @@ def test_step_odd_keys(n, h, hk, K, V, dtype):
     test_step(n, h, hk, K, V, dtype)
 
 
+def test_step_reads_no_state_by_the_read_only_path():
+    """The kernels' state is read and written by one launch, which the read-only path's loads do not allow."""
+    source = (Path(native.__file__).resolve().parent.parent / "csrc" / "delta_step.cu").read_text()
+    assert "__ldg" not in source and "ld.global.nc" not in source and "__restrict__" not in source
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("n,h,hk,K,V", [(300, 4, 2, 64, 64), (37, 3, 3, 33, 128), (41, 2, 1, 40, 71), (9, 1, 1, 7, 3)])
+def test_step_in_place_equals_apart(n, h, hk, K, V, dtype):
+    """The C call on one buffer for the old and the new state, and on two: the same bits."""
+    a = rollout(n, 1, h, hk, K, V, dtype, seed=n)
+    one = {x: a[x][:, 0].contiguous() for x in ("q", "k", "v", "g", "beta")}
+    state, new, out = a["state"].clone(), torch.empty_like(a["state"]), torch.empty_like(one["v"])
+    desc = policy._DESC.pack(n, 1, h, hk, K, V, policy._DTYPE[dtype], K ** -0.5, *(x.data_ptr() for x in one.values()), 0,
+                             state.data_ptr(), new.data_ptr(), out.data_ptr(), *[hk * K, 0, K] * 2, h * V, 0, V,
+                             *[h, 0, 1] * 2, h * V, 0, V, 0, 0)
+    native.check(native.load().goib2d_delta_step(desc, torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(state, a["state"])
+    assert torch.equal(goib2d.delta_step_(state, **one), out) and torch.equal(state, new)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
 def test_rollout_in_pieces_equals_whole(dtype):
