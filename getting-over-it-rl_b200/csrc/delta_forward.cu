@@ -35,7 +35,7 @@ struct Layout {
 
 // A chunk that holds infinities or NaN, token by token: within the products a token meets every other one, if only as 0
 // times it, which these values pass. S: the warp's accumulators, in memory.
-template <class T, class P, int KP, int MT>
+template <class T, class P, class R, int KP, int MT>
 __device__ __noinline__ void odd_chunk(const Forward &f, float *S, const typename P::E *Q, const typename P::E *K,
                                        const typename P::E *V, int vp, int64_t n, int h, int64_t at, int v0, int lane) {
     const goib2d_delta_desc &d = f.d;
@@ -62,14 +62,14 @@ __device__ __noinline__ void odd_chunk(const Forward &f, float *S, const typenam
             if (t == 0 && v < d.value_dim) {
                 row<T>(d.out, d.out_stride, n, at + i, h)[v] = from_float<T>(d.scale * (sq + kq * u));
                 if (f.r)
-                    ((typename P::E *)f.r)[((n * d.heads + h) * d.n_steps + at + i) * d.value_dim + v] =
-                        from_float<typename P::E>(r);
+                    ((R *)f.r)[((n * d.heads + h) * d.n_steps + at + i) * d.value_dim + v] = from_float<R>(r);
             }
         }
     }
 }
 
-template <class T, class P, int KP, int MT, int AHEAD>
+// R: the type of what is kept
+template <class T, class P, class R, int KP, int MT, int AHEAD>
 __global__ void __maxnreg__(AHEAD == 1 ? 232 : 168)  // 168: 12 warps an SM, two blocks ahead
     goib2d_delta_forward_kernel(const __grid_constant__ Forward f) {
     using L = Layout<P, KP, MT, AHEAD != 0>;
@@ -124,14 +124,14 @@ __global__ void __maxnreg__(AHEAD == 1 ? 232 : 168)  // 168: 12 warps an SM, two
     float S[MT][KP / 8][4];  // S^T: rows v, columns k
     load_state<MT, KP>(S, d.state_in ? d.state_in + nh * K * V : nullptr, K, V, block0 + v0, lane);
     T *const out = row<T>(d.out, d.out_stride, n, 0, h) + block0;
-    E *const r = f.r ? (E *)f.r + nh * steps * V + block0 : nullptr;
+    R *const r = f.r ? (R *)f.r + nh * steps * V + block0 : nullptr;
     const int os = (int)d.out_stride[1];
     auto solve = [&](int at, const E *Qs, const E *Ks, E *Vs, const Chunk<P> &c) {
             if (f.kept && at % f.keep == 0) {
                 const int64_t x = (nh * ((steps + f.keep - 1) / f.keep) + at / f.keep) * f.tiles_v + tile0;
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
-                    if (tile0 + m < f.tiles_v) keep_state<KT>((E *)f.kept + (x + m) * 16 * KP, S[m], lane);
+                    if (tile0 + m < f.tiles_v) keep_state<KT>((R *)f.kept + (x + m) * 16 * KP, S[m], lane);
             }
             const uint32_t tokens = steps - at < kChunk ? (1u << (steps - at)) - 1 : 0xffffu;
             float Y[MT][2][4] = {}, O[MT][2][4] = {};
@@ -170,18 +170,18 @@ __global__ void __maxnreg__(AHEAD == 1 ? 232 : 168)  // 168: 12 warps an SM, two
                 float s[MT * (KP / 8) * 4];
 #pragma unroll
                 for (int i = 0; i < MT * (KP / 8) * 4; ++i) s[i] = S[i / (KP / 2)][i / 4 % (KP / 8)][i % 4];
-                odd_chunk<T, P, KP, MT>(f, s, Qs, Ks, Vs + v0, vp, n, h, at, block0 + v0, lane);
+                odd_chunk<T, P, R, KP, MT>(f, s, Qs, Ks, Vs + v0, vp, n, h, at, block0 + v0, lane);
 #pragma unroll
                 for (int i = 0; i < MT * (KP / 8) * 4; ++i) S[i / (KP / 2)][i / 4 % (KP / 8)][i % 4] = s[i];
                 return;
             }
             if (r) {
-                E *to = r + (int64_t)at * V;
-                if (half)
+                R *to = r + (int64_t)at * V;
+                if (sizeof(R) == 2)
                     store_rows<MT>((bf16 *)to, V, tokens, v0, V - block0, f.wide_r, (bf16 *)Vs, vp, Y, lane);
                 else
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) store_direct<E>(to, V, tokens, v0 + 16 * m, V - block0, Y[m], lane);
+                    for (int m = 0; m < MT; ++m) store_direct<R>(to, V, tokens, v0 + 16 * m, V - block0, Y[m], lane);
             }
             typename P::A2 u[MT];
             {
@@ -270,27 +270,27 @@ __global__ void __maxnreg__(AHEAD == 1 ? 232 : 168)  // 168: 12 warps an SM, two
     store_state<MT, KP>(d.state_out + nh * K * V, S, K, V, block0 + v0, lane);
 }
 
-template <class T, class P, int KP, int MT, int AHEAD>
+template <class T, class P, class R, int KP, int MT, int AHEAD>
 cudaError_t forward_of(const Forward &f, const Split &b, cudaStream_t s) {
     const size_t smem = Layout<P, KP, MT, AHEAD != 0>::bytes(b.warps);
-    cudaError_t e = allow_smem(goib2d_delta_forward_kernel<T, P, KP, MT, AHEAD>, smem);
+    cudaError_t e = allow_smem(goib2d_delta_forward_kernel<T, P, R, KP, MT, AHEAD>, smem);
     if (e != cudaSuccess) return e;
-    goib2d_delta_forward_kernel<T, P, KP, MT, AHEAD>
+    goib2d_delta_forward_kernel<T, P, R, KP, MT, AHEAD>
         <<<dim3((unsigned)(f.d.n_worlds * f.d.heads), b.blocks), 32 * (b.warps + (AHEAD ? 2 : 0)), smem, s>>>(f);
     return cudaGetLastError();
 }
 
-template <class T, class P, int KP>
+template <class T, class P, class R, int KP>
 cudaError_t forward_wide(const Forward &f, cudaStream_t s) {
     const Split b(f.d);
-    if (b.ahead == 1) return forward_of<T, P, KP, 1, 1>(f, b, s);
+    if (b.ahead == 1) return forward_of<T, P, R, KP, 1, 1>(f, b, s);
     if constexpr (KP < 128) {
-        if (b.ahead == 0) return b.MT == 2 ? forward_of<T, P, KP, 2, 0>(f, b, s) : forward_of<T, P, KP, 1, 0>(f, b, s);
+        if (b.ahead == 0) return b.MT == 2 ? forward_of<T, P, R, KP, 2, 0>(f, b, s) : forward_of<T, P, R, KP, 1, 0>(f, b, s);
     }
-    return forward_of<T, P, KP, 1, 2>(f, b, s);
+    return forward_of<T, P, R, KP, 1, 2>(f, b, s);
 }
 
-template <class T, class P>
+template <class T, class P, class R>
 cudaError_t forward_typed(const goib2d_delta_desc &d, void *saved, cudaStream_t s) {
     Forward f{d};
     const Saved at = delta_saved(d);
@@ -302,9 +302,9 @@ cudaError_t forward_typed(const goib2d_delta_desc &d, void *saved, cudaStream_t 
     f.wide_o = rows_grain(d.out, d.out_stride, d.n_worlds, d.n_steps, d.heads, V, z) == 16;
     f.wide_r = V % 8 == 0;
     switch (padded_keys(d.key_dim)) {
-        case 32: return forward_wide<T, P, 32>(f, s);
-        case 64: return forward_wide<T, P, 64>(f, s);
-        default: return forward_wide<T, P, 128>(f, s);
+        case 32: return forward_wide<T, P, R, 32>(f, s);
+        case 64: return forward_wide<T, P, R, 64>(f, s);
+        default: return forward_wide<T, P, R, 128>(f, s);
     }
 }
 
@@ -312,9 +312,11 @@ cudaError_t forward_typed(const goib2d_delta_desc &d, void *saved, cudaStream_t 
 
 int64_t delta_saved_bytes(const goib2d_delta_desc &d) { return delta_saved(d).bytes; }
 
+// What is kept for gradients in full products is float32. The forward products do not change with it, so that o and the
+// last state are the same bits whether gradients are wanted or not.
 cudaError_t launch_delta_forward(const goib2d_delta_desc &d, void *saved, cudaStream_t s) {
-    if (d.dtype == GOIB2D_FLOAT32) return forward_typed<float, Full>(d, saved, s);
-    return saved && delta_full(d) ? forward_typed<bf16, Full>(d, saved, s) : forward_typed<bf16, Half>(d, saved, s);
+    if (d.dtype == GOIB2D_FLOAT32) return forward_typed<float, Full, float>(d, saved, s);
+    return saved && delta_full(d) ? forward_typed<bf16, Half, float>(d, saved, s) : forward_typed<bf16, Half, bf16>(d, saved, s);
 }
 
 }  // namespace gb

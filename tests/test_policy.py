@@ -492,6 +492,18 @@ def test_gradients_against_differences():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+@pytest.mark.parametrize("size", SIZES + [(4096, 2, 1, 1, 16, 16)], ids=str)
+def test_outputs_do_not_depend_on_whether_gradients_are_wanted(size, dtype):
+    """The same bits with and without, in calls of few tokens and of many."""
+    a = rollout(*size, dtype, seed=size[1])
+    out, last = goib2d.delta_rule(**a)
+    trained, trained_last = goib2d.delta_rule(**dict(a, v=a["v"].clone().requires_grad_()))
+    assert trained.requires_grad
+    assert torch.equal(trained, out) and torch.equal(trained_last, last)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
 def test_states_may_be_written_to_before_the_gradients(dtype):
     """The gradients need neither the first nor the last state: the world goes on acting with the last one's memory (zeroed
     where it was reset), and the first one's buffer takes the next rollout's, while the loss is still to be trained on."""
