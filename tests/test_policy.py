@@ -490,6 +490,40 @@ def test_gradients_against_differences():
         assert abs(got - slope) <= 2 * TOL[F32] * size, name
 
 
+# What the split operands carry, tighter than TOL. float32: an operand is hi, rounded to tf32's 11 bits, plus lo, at most 2^-11
+# of it, of which the product reads 11 bits (2^-21 of the operand); with the two lo parts' product (2^-22) left out a
+# product is 2.5 * 2^-21 off, a chain of four 10 * 2^-21, gradients twice as many: two bfloat16 parts (2^-17) would not do.
+# bfloat16 gradients of many tokens: four rounded operands or kept rows and the result, each 2^-9 at most and 1.7e-3 of a
+# norm, independent: sqrt(5) * 1.7e-3 < 2 * 2^-9.
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(2, 17, 4, 2, 64, 32), (5, 33, 6, 3, 40, 71), (2, 64, 2, 1, 128, 128), (80, 70, 4, 2, 64, 64)],
+                         ids=str)
+def test_precision_float32(size):
+    n, t, h, hk, K, V = size
+    a = rollout(*size, F32, seed=61)
+    dout = torch.randn(n, t, h, V, generator=torch.Generator("cuda").manual_seed(t), device="cuda")
+    out, last, got = backward(a, dout, None)
+    want_out, want_last, want = backward(wide(a), dout.double().cpu(), None, recurrence)
+    assert off(out, want_out) <= 10 * 2.0**-21 and off(last, want_last) <= 10 * 2.0**-21
+    for x in got:
+        assert off(got[x], want[x]) <= 20 * 2.0**-21, x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [(80, 70, 4, 2, 64, 64), (110, 50, 3, 3, 32, 64), (301, 35, 1, 1, 100, 65), (150, 33, 2, 1, 128, 128)],
+                         ids=str)
+def test_precision_bfloat16_of_many_tokens(size):
+    n, t, h, hk, K, V = size
+    assert n * t * h > 4096
+    a = rollout(*size, BF16, seed=62)
+    dout = torch.randn(n, t, h, V, generator=torch.Generator("cuda").manual_seed(t), device="cuda").to(BF16)
+    _, last, got = backward(a, dout, None)
+    _, want_last, want = backward(wide(a), dout.double().cpu(), None, recurrence)
+    assert off(last, want_last) <= 2.0**-16  # float32, of operands in two bfloat16 parts (2^-17)
+    for x in ("q", "k", "v", "g", "beta"):
+        assert off(got[x], want[x]) <= 2 * 2.0**-9, x
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
 @pytest.mark.parametrize("size", SIZES + [(4096, 2, 1, 1, 16, 16)], ids=str)
@@ -633,6 +667,77 @@ def test_clip(sizes, max_norm):
         else:
             err = (x.double().cpu() - y).abs() - y.abs() * (2.0**-8 if x.dtype == BF16 else 8 * 2.0**-24)
             assert not x.numel() or float(err.max()) <= 0
+
+
+def clip_check(grads, max_norm):
+    """clip_grads_ against the formula in 64 bits, every element, with test_clip's bounds."""
+    wide_grads, before = [x.double() for x in grads], [x.clone() for x in grads]
+    norm_want = math.sqrt(sum(float((x * x).sum()) for x in wide_grads))
+    factor = min(1.0, max_norm / (norm_want + 1e-6))
+    norm = goib2d.clip_grads_(grads, max_norm)
+    assert abs(float(norm) - norm_want) <= 4 * 2.0**-24 * norm_want
+    for x, w, b in zip(grads, wide_grads, before):
+        if factor == 1.0:
+            assert torch.equal(x, b)
+        else:
+            err = (x.double() - w * factor).abs() - (w * factor).abs() * (2.0**-8 if x.dtype == BF16 else 8 * 2.0**-24)
+            assert float(err.max()) <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [0.5, 1e9])
+@pytest.mark.parametrize("megabytes", [20, 29, 31, 45, 62])
+def test_clip_beyond_what_the_blocks_keep(megabytes, max_norm):
+    """The blocks keep 148 x 12 tiles of 16 KB (29 MB) between the norm and the scaling and read the rest again: less than
+    that, as much, and more, in mixed types, with tensors that begin and end within a block's tiles, one of them off
+    the 16-byte boundary. A block's tiles are 8 to 26, whole batches of four and not."""
+    gen = torch.Generator(device="cuda").manual_seed(megabytes)
+    share = megabytes * 1_000_000 // 10  # of bytes
+    sizes = [(3 * share // 4 + 1, F32, 0), (4099, BF16, 1), (2 * share // 2, BF16, 1), (5, F32, 0), (share // 4, F32, 3),
+             (3 * share // 2 + 3, BF16, 0), (share // 4 - 7, F32, 0)]
+    grads = [torch.randn(n + at, generator=gen, device="cuda").to(dtype)[at:] for n, dtype, at in sizes]
+    clip_check(grads, max_norm)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [0.5, 1e9])
+@pytest.mark.parametrize("count", [63, 64, 65, 700, 1023, 1024, 1025, 2048, 2049])
+def test_clip_numbers_of_tensors(count, max_norm):
+    """The table in the launch holds 64 or 1024 tensors: as many, one more, one fewer; more take several launches."""
+    gen = torch.Generator(device="cuda").manual_seed(count)
+    clip_check([torch.randn(1 + 997 * i % 9001, generator=gen, device="cuda").to(BF16 if i % 3 == 0 else F32)
+                for i in range(count)], max_norm)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["float32", "bfloat16"])
+def test_training_in_a_graph(dtype):
+    """Rollouts, their gradients and the clipping, captured and replayed on other inputs: what the calls give by themselves."""
+    a, b = (rollout(70, 33, 2, 1, 32, 24, dtype, seed=s) for s in (51, 52))
+    dout = torch.randn(70, 33, 2, 24, device="cuda").to(dtype)
+
+    def update(a):
+        leaves = {x: a[x].detach().requires_grad_() for x in GRADS}
+        out, last = goib2d.delta_rule(**leaves, reset=a["reset"])
+        grads = torch.autograd.grad([out], list(leaves.values()), [dout])
+        return [out.detach(), last.detach(), goib2d.clip_grads_(grads, 0.5), *grads]
+
+    want = [x.clone() for x in update(b)]
+    now = {x: y.clone() for x, y in a.items()}
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        update(now)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = update(now)
+    for x in now:
+        now[x].copy_(b[x])
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
 
 
 @pytest.mark.gpu
