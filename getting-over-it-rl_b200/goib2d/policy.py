@@ -91,9 +91,10 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def _no_tangents(name, tensors):
-    """Raw pointers would drop forward-mode tangents. The level is -1 outside torch.autograd.forward_ad.dual_level()."""
-    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+def _no_tangents(name, *tensors):
+    """Raw pointers would drop forward-mode tangents. Asked for within torch.autograd.forward_ad.dual_level() only, outside
+    which the level is -1."""
+    if any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors):
         raise ValueError(f"{name} has no forward-mode derivative")
 
 
@@ -105,9 +106,11 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     # everything in one expression first: an acting loop calls this once per world step
     device, dt = v.device, v.dtype
     vs, qs, ks, gs, bs = v.stride(), q.stride(), k.stride(), g.stride(), beta.stride()
-    written = (state,) if out is None else (state, out)
+    written = state
     if out is None:
-        out = _like(v)
+        out = torch.empty_like(v)
+    else:
+        written = (state, out)
     shape, heads = v.shape, g.shape
     os_ = out.stride()
     if not (len(vs) == len(qs) == len(os_) == 3 and q.shape == k.shape and heads == beta.shape and heads == shape[:2] and
@@ -116,6 +119,9 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
             dt is q.dtype is k.dtype is g.dtype is beta.dtype is out.dtype and state.dtype is torch.float32 and
             0 <= v.get_device() == q.get_device() == k.get_device() == g.get_device() == beta.get_device() ==
             out.get_device() == state.get_device() and state.is_contiguous()):
+        if written is state:
+            out = _like(v)
+            os_ = out.stride()
         _check_step(state, q, k, v, g, beta, out)
     n, h, V = shape
     hk, K = q.shape[1:]
@@ -124,7 +130,8 @@ def delta_step_(state, q, k, v, g, beta, reset=None, scale=None, out=None):
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
                                     beta.requires_grad or state.requires_grad or out.requires_grad):
         raise ValueError("delta_step_ is not differentiable: use delta_rule, or torch.no_grad()")
-    _no_tangents("delta_step_", (state, q, k, v, g, beta, out))
+    if forward_ad._current_level >= 0:
+        _no_tangents("delta_step_", state, q, k, v, g, beta, out)
     rp, rs = (0, (0,)) if reset is None else _reset(reset, (n,), device)
     sp = state.data_ptr()
     desc = _DESC.pack(n, 1, h, hk, K, V, _DTYPE[dt], K ** -0.5 if scale is None else scale, q.data_ptr(), k.data_ptr(),
@@ -241,7 +248,8 @@ def delta_rule(q, k, v, g, beta, state=None, reset=None, scale=None):
     rollout recorded step by step goes in as x.transpose(0, 1). Differentiable in q, k, v, g, beta and state."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    _no_tangents("delta_rule", (q, k, v, g, beta) if state is None else (q, k, v, g, beta, state))
+    if forward_ad._current_level >= 0:
+        _no_tangents("delta_rule", q, k, v, g, beta, state)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or
                                     beta.requires_grad or (state is not None and state.requires_grad)):
         return _DeltaRule.apply(q, k, v, g, beta, state, reset, float(scale))
@@ -286,7 +294,8 @@ def clip_grads_(grads, max_norm):
             where.append(x.data_ptr()), numel.append(n), types.append(dt), written.append(x)
     if index is None:
         raise ValueError("no gradients")
-    _no_tangents("clip_grads_", written)
+    if forward_ad._current_level >= 0:
+        _no_tangents("clip_grads_", *written)
     count = len(where)
     if len(set(where)) != count:
         raise ValueError("the same gradient twice")
