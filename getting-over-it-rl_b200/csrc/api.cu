@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -1108,6 +1109,24 @@ int goib2d_delta_backward(const goib2d_delta_desc *d, const goib2d_delta_grads *
     return 0;
 }
 
+namespace {
+// Two tensors of the table that share memory, or -1. Scaled by two blocks, what they share would be scaled twice or not.
+int overlap(const goib2d_grad *grads, int32_t n, int32_t *other, bool *failed) {
+    auto begin = [&](int32_t i) { return (uintptr_t)grads[i].data; };
+    auto end = [&](int32_t i) { return begin(i) + (uintptr_t)grads[i].numel * (grads[i].dtype == GOIB2D_BFLOAT16 ? 2 : 4); };
+    int32_t few[64], *order = n <= 64 ? few : new (std::nothrow) int32_t[n], m = 0, found = -1;
+    *failed = !order;
+    if (!order) return -1;
+    for (int32_t i = 0; i < n; ++i)
+        if (grads[i].numel) order[m++] = i;
+    std::sort(order, order + m, [&](int32_t i, int32_t j) { return begin(i) < begin(j); });
+    for (int32_t i = 1; i < m && found < 0; ++i)
+        if (begin(order[i]) < end(order[i - 1])) found = order[i], *other = order[i - 1];
+    if (order != few) delete[] order;
+    return found;
+}
+}  // namespace
+
 int64_t goib2d_clip_workspace_bytes(const goib2d_grad *grads, int32_t n) {
     if (n < 0 || (n && !grads)) return fail(GOIB2D_EINVAL, "bad gradient table");
     return gb::clip_workspace_bytes(grads, n);
@@ -1129,6 +1148,11 @@ int goib2d_clip_grads(const goib2d_grad *grads, int32_t n, float max_norm, float
             return fail(GOIB2D_EINVAL, "tensor %d: null or misaligned data", i);
     }
     if (pieces > INT32_MAX / 4) return fail(GOIB2D_ELIMIT, "too many elements");
+    int32_t other = 0;
+    bool failed = false;
+    const int32_t tensor = overlap(grads, n, &other, &failed);
+    if (failed) return fail(GOIB2D_ENOMEM, "%d tensors: no host memory for their order", n);
+    if (tensor >= 0) return fail(GOIB2D_EINVAL, "tensors %d and %d overlap", other, tensor);
     CUDA_TRY(gb::launch_clip(grads, n, max_norm, norm, workspace, (cudaStream_t)stream));
     return 0;
 }

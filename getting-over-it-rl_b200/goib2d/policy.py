@@ -269,8 +269,8 @@ def _dense(x):
 def clip_grads_(grads, max_norm):
     """Scale all gradients, in place, by min(1, max_norm / (norm + 1e-6)), where norm is the 2-norm of all their
     elements together; returns norm (a float32 scalar on the device). grads: float32 or bfloat16 CUDA tensors on one
-    device, dense in memory; None entries are skipped. A NaN or an infinity among them makes the result NaN where
-    the formula does."""
+    device, dense in memory and not overlapping; None entries are skipped. A NaN or an infinity among them makes the
+    result NaN where the formula does."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")

@@ -383,7 +383,7 @@ int64_t goib2d_delta_workspace_bytes(const goib2d_delta_desc *desc);
  * element times min(1, max_norm / (norm + 1e-6)), in place. A NaN among the gradients gives NaN everywhere. Sums are
  * float64 in a fixed order (the same inputs give the same bits). The table is host memory and read before the call
  * returns; norm: one device float32, or NULL; workspace: goib2d_clip_workspace_bytes(grads, n) bytes of device
- * memory (16-byte aligned). Tensors are dense and must not overlap. */
+ * memory (16-byte aligned). Tensors are dense; two that overlap are refused. */
 typedef struct goib2d_grad {
     void *data;
     int64_t numel;

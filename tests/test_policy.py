@@ -910,6 +910,31 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.goib2d_clip_workspace_bytes(None, 2) == einval
 
 
+def test_clipping_refuses_tensors_that_overlap():
+    """Before any launch (so this needs no GPU), in any order, with empty tensors between, few and many."""
+    lib, one = native.load(), policy._GRAD.pack
+
+    def call(*tensors):
+        return lib.goib2d_clip_grads(b"".join(one(*t) for t in tensors), len(tensors), 1.0, None, 16, None)
+
+    many = [(4096 + 64 * i, 16, 0) for i in range(100)]
+    for bad in ([(4096, 100, 0), (4096, 100, 0)], [(4096, 100, 0), (4096 + 396, 1, 0)], [(4096 + 198, 5, 1), (4096, 100, 1)],
+                [(8192, 10, 0), (4096, 0, 0), (4096, 1025, 0)], many + [(4096 + 64 * 50 + 60, 2, 0)], many[::-1] + [(4096, 1, 1)]):
+        assert call(*bad) == -1 and b"overlap" in lib.goib2d_last_error()
+
+
+@pytest.mark.gpu
+def test_clipping_takes_neighbours():
+    flat = torch.randn(10_000, device="cuda")
+    want = flat.double() / (flat.double().norm() + 1e-6)
+    views = [flat[7000:], flat[:1], flat[1:500], flat[500:500], flat[500:7000]]
+    goib2d.clip_grads_(views, 1.0)
+    assert off(flat, want.cpu()) <= 1e-6
+    with pytest.raises(RuntimeError, match="overlap"):
+        goib2d.clip_grads_([flat[:100], flat[99:200]], 1.0)
+    assert off(flat, want.cpu()) <= 1e-6
+
+
 def test_struct_layouts():
     """The packed structures are the header's (sizes as a C compiler lays them out)."""
     assert (policy._DESC.size, policy._GRADS.size, policy._GRAD.size) == (272, 208, 24)
