@@ -274,7 +274,7 @@ def clip_grads_(grads, max_norm):
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
-    where, numel, types, written = [], [], [], []
+    words, written = [], []  # words: address, elements, type, one tensor after the other (goib2d_grad)
     index = None
     for x in grads:
         if x is None:
@@ -291,16 +291,16 @@ def clip_grads_(grads, max_norm):
             raise ValueError(f"a gradient of shape {tuple(x.shape)} and strides {x.stride()} is not dense in memory")
         n = x.numel()
         if n:
-            where.append(x.data_ptr()), numel.append(n), types.append(dt), written.append(x)
+            words += x.data_ptr(), n, dt
+            written.append(x)
     if index is None:
         raise ValueError("no gradients")
     if forward_ad._current_level >= 0:
         _no_tangents("clip_grads_", *written)
-    count = len(where)
-    if len(set(where)) != count:
+    count = len(written)
+    if len(set(words[::3])) != count:
         raise ValueError("the same gradient twice")
-    table = array("q", bytes(_GRAD.size * count))
-    table[0::3], table[1::3], table[2::3] = array("q", where), array("q", numel), array("q", types)
+    table = array("q", words)
     packed = table.buffer_info()[0]
     lib = native.load()
     size = lib.goib2d_clip_workspace_bytes(packed, count)
