@@ -53,7 +53,7 @@ inline int dense_grain(int cols, int size) {  // of dense rows from an aligned s
 // bfloat16. A gradient such as dg or db is a sum that may cancel; over many tokens the rounding of bfloat16 operands
 // (2^-9) averages out to 2^-9 of their norm, over a few it need not. Largest error of a gradient (of its norm) over six
 // draws, rounded / full, where rounding the result alone gives 1.7e-3: 1 token of 64 x 64 2.0e-2 / 3.7e-3, 16 tokens
-// 4.5e-3 / 2.2e-3, 256 tokens 3.1e-3 / 1.8e-3, 4096 tokens 2.9e-3 / 1.7e-3; of 1 x 1 at 16 tokens 6.2e-3 / 2.4e-3 and at
+// 4.5e-3 / 2.2e-3, 256 tokens 3.1e-3 / 1.9e-3, 4096 tokens 2.9e-3 / 1.7e-3; of 1 x 1 at 16 tokens 6.2e-3 / 2.4e-3 and at
 // 2048 8.5e-3 / 1.7e-3. So a world's gradients may differ by this much with the number of tokens beside its own. The
 // price, us of a training step: 64 x 16 steps x 2 heads of 64 x 64 68 for either (the host's), 1 x 1024 x 4 heads 178 /
 // 354, 1 x 4096 of 128 x 128 799 / 2041.
@@ -62,7 +62,9 @@ inline bool delta_full(const goib2d_delta_desc &d) {
 }
 
 // What goib2d_delta_forward keeps for goib2d_delta_backward: r [n][h][t][V], and S at every keep-th token, as its S^T
-// [n][h][t / keep][V up to 16s][padded keys]. Both in bfloat16, or in float32 (delta_full).
+// [n][h][t / keep][V up to 16s][padded keys]. In float32 for gradients in full products (delta_full). Otherwise in
+// bfloat16, which the products would round them to anyway: half of what is written and read again (for 4096 worlds x 64
+// steps x 4 heads of 64 x 64 in all 0.27 GB).
 struct Saved {
     int64_t r, states, bytes;   // bytes: both
     int32_t keep, tiles_v, tiles_k, size;
@@ -91,6 +93,8 @@ inline Saved delta_saved(const goib2d_delta_desc &d) {
 //   32 x 32 float32 (three blocks an SM): 444 of 16 steps 6.2 / 5.8, 512: 6.4 / 9.3;
 //   128 x 128, training, 64 steps: 1024 x 4 bfloat16 1311 / 1261, 512 x 4 float32 1931 / 1817;
 //   128 x 128 bfloat16, training, 37 (world, head)s of 512 steps: 206 at 168 registers, 173 at 232.
+// At 444 (world, head)s of 64 x 64 either may win by the number of steps (57 / 50, but 8.4 / 8.8 and 10.5 / 13.1): they are
+// the first that do not run at once ahead, and the rule goes by that alone.
 struct Split {
     int MT, warps, blocks;
     int ahead;  // 0: no; 1: one block to an SM; 2: more

@@ -15,6 +15,10 @@
 // A_ij q_i.k_j + M_ij k_i.k_j, what i >= l reads of S0, what j < l leaves in the last state, and a_end <S0, dS1>. Summing
 // these pairs keeps the relative precision where decays are strong; the difference q.dq - k.dk cancels there.
 //
+// What only bfloat16 results depend on is rounded to bfloat16 (Half): r, S0, dS1, dv, A and M as operands here, of one
+// product each, and held so between the kernels. dq, dk, dg and db are 2.3e-3 to 3.0e-3 off by it where the rounding of the
+// results alone gives 1.7e-3. A and M unrounded on the row side: dq 2.9e-3 -> 2.3e-3, and 5 % more time.
+//
 // 4096 worlds x 64 steps x 4 heads of 64 x 64, bfloat16: 0.42 ms, bound as the forward pass, and 0.61 ms, 38 % of the issue
 // slots at 12 warps an SM (74 KB of rows and 168 registers allow three blocks): loads, barriers and instruction latency.
 // 32 channels of dq and dk a warp instead of 64 (16 warps an SM) makes A and M twice: 0.25 ms slower.

@@ -12,9 +12,15 @@ strength b = beta does
 
 and a token whose `reset` is set (the world's reset came before it), or whose decay is 0 in float32, starts from
 S' = 0 whatever S held. q and k may have fewer heads than v: value head h reads key head h // (heads // key_heads).
-All of q, k, v, g, beta are float32 or all bfloat16; memories and every sum are float32. The kernels are in
-libgoib2d.so (csrc/delta_*.cu, csrc/clip.cu; the C calls are goib2d_delta_* and goib2d_clip_grads): there is no CPU
-path. Calls run on the current stream of the tensors' device and return without waiting for it.
+All of q, k, v, g, beta are float32 or all bfloat16; memories and every sum are float32. Acting computes in float32;
+rollouts multiply on the matrix units, their operands in two parts each where a state depends on them (2e-6 off in
+float32, 3.4e-6 for the states of bfloat16 rollouts) and rounded to bfloat16 where only bfloat16 results do (o 2.0e-3
+off, gradients 1.7e-3 to 3.3e-3, of which their own rounding is 1.7e-3; the gradients of at most 4096 tokens are computed
+in full). So a replayed o is within about 2e-3 of the one acted on, not equal to it.
+
+The kernels are in libgoib2d.so (csrc/delta_*.cu, csrc/clip.cu; the C calls are goib2d_delta_* and goib2d_clip_grads):
+there is no CPU path. Calls run on the current stream of the tensors' device and return without waiting for it. What they
+write in place (a memory, a given out, clipped gradients) counts as modified for autograd. No forward-mode derivatives.
 """
 import struct
 from array import array

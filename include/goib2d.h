@@ -336,7 +336,12 @@ enum { GOIB2D_FLOAT32 = 0, GOIB2D_BFLOAT16 = 1 };
  * state_in / state_out: contiguous [n_worlds][heads][key_dim][value_dim]; state_in NULL = zeros; they may be the
  * same buffer, and may not overlap otherwise. reset: one byte per world and step, or NULL. key_dim and value_dim
  * 1..128, heads a multiple of key_heads; a step's stride below 2^31 elements; pointers aligned to their elements. A value
- * that is not finite spoils the tokens that see it, up to the next one that starts from S' = 0, and no others. */
+ * that is not finite spoils the tokens that see it, up to the next one that starts from S' = 0, and no others.
+ * Precision, as the 2-norm of a result's error over that of the result. One token: float32 throughout (1e-7). Rollouts
+ * multiply on the matrix units. float32: operands in two tf32 parts, 2e-6, gradients included. bfloat16: states 3.4e-6
+ * (operands in two bfloat16 parts); o reads S rounded to bfloat16, 2.0e-3 where rounding o alone gives 1.7e-3, so that a
+ * replayed o and the one acted on differ by up to that; gradients of calls of more than 4096 tokens (n_worlds x n_steps x
+ * heads) 1.7e-3 to 3.3e-3 (to 5e-3 at one channel), of fewer by full products: as near as bfloat16 holds them. */
 typedef struct goib2d_delta_desc {
     int64_t n_worlds, n_steps;
     int32_t heads, key_heads, key_dim, value_dim, dtype;
