@@ -281,7 +281,7 @@ def clip_grads_(grads, max_norm):
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be a number >= 0, got {max_norm}")
     words, written = [], []  # words: address, elements, type, one tensor after the other (goib2d_grad)
-    index = None
+    index, type_of, strided = None, _DTYPE.get, torch.strided
     for x in grads:
         if x is None:
             continue
@@ -289,8 +289,8 @@ def clip_grads_(grads, max_norm):
             device, index = x.device, x.get_device()
             if index < 0:
                 raise TypeError("gradients must be CUDA tensors")
-        dt = _DTYPE.get(x.dtype)
-        if dt is None or x.get_device() != index or x.layout is not torch.strided:
+        dt = type_of(x.dtype)
+        if dt is None or x.get_device() != index or x.layout is not strided:
             raise ValueError(f"gradients must be dense float32 or bfloat16 tensors on {device}, got {x.dtype} on {x.device} "
                              f"({x.layout})")
         if not (x.is_contiguous() or _dense(x)):
